@@ -76,7 +76,7 @@ def lib() -> C.CDLL:
     return _lib
 
 
-_P, _I, _F, _L = C.c_void_p, C.c_int, C.c_float, C.c_long
+_P, _I, _F, _L, _D = C.c_void_p, C.c_int, C.c_float, C.c_long, C.c_double
 
 FH_MAX_CONV = 12
 
@@ -112,6 +112,17 @@ class StudentKdC(C.Structure):
 class TeacherLayerC(C.Structure):
     """fh_teacher_layer (include/fithubert_hip.h): device pointers of one teacher layer's weights"""
     _fields_ = [(n, C.c_void_p) for n in ("wqkv", "bqkv", "wo", "bo", "g1", "b1", "w1", "c1", "w2", "c2", "g2", "b2")]
+
+
+class WindowAttentionC(C.Structure):
+    """fh_window_attention_desc (include/fithubert_hip.h)"""
+    _fields_ = ([(n, C.c_int) for n in ("B", "Tq", "Tk", "Hq", "Hkv", "dh", "left", "right", "sinks")] + [("scale", C.c_float)]
+                + [(n, C.c_void_p) for n in ("key_len", "q_start")] + [(t + n, C.c_long) for t in "qkv" for n in ("_bs", "_ts", "_hs")])
+
+
+class AdapterC(C.Structure):
+    """fh_adapter_desc (include/fithubert_hip.h)"""
+    _fields_ = [(n, C.c_int) for n in ("M", "K", "N", "R", "n_adapters", "n_segments")] + [(n, C.c_void_p) for n in ("seg_start", "seg_adapter", "scaling")]
 
 
 class StudentCallC(C.Structure):
@@ -177,6 +188,12 @@ SIGNATURES = {
     "fh_attention_backward_scratch_floats": (_L, [_I, _I, _I, _I, _I]),
     "fh_attention_backward_ws": (_I, [_I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _F, Drop, _P, _P]),
     "fh_attention_backward_bias": (_I, [_I, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _F, Drop, _P, _P]),
+    "fh_window_attention_scratch_bytes": (_L, [_I, C.POINTER(WindowAttentionC), _I]),
+    "fh_window_attention_forward": (_I, [_I, C.POINTER(WindowAttentionC), _P, _P, _P, _P, _P, _P, _P]),
+    "fh_window_attention_backward": (_I, [_I, C.POINTER(WindowAttentionC)] + [_P] * 11),
+    "fh_adapter_scratch_bytes": (_L, [_I, C.POINTER(AdapterC), _I]),
+    "fh_adapter_linear_forward": (_I, [_I, C.POINTER(AdapterC)] + [_P] * 9),
+    "fh_adapter_linear_backward": (_I, [_I, C.POINTER(AdapterC)] + [_P] * 11),
     "fh_kd_loss_nblk": (_I, [_I, _I, _I, _I]),
     "fh_kd_loss": (_I, [_I, _I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _L, _I, _F, _P]),
     "fh_kd_loss_rows_nblk": (_I, [_I, _I]),
@@ -195,6 +212,8 @@ SIGNATURES = {
     "fh_cast": (_I, [_I, _P, _P, _L, _P]),
     "fh_permute3_cast": (_I, [_I, _P, _P, _I, _I, _I, _I, _I, _I, _P]),
     "fh_adamw": (_I, [_P, _P, _P, _P, _L, _F, _F, _F, _F, _F, _F, _F, _F, _P, _P]),
+    "fh_adamw_many_blocks": (_L, [_P, _I]),
+    "fh_adamw_many": (_I, [_I, _I, _P, _P, _P, _I, _I, _P, _P, _P, _P, _D, _D, _D, _D, _D, _L, _D, C.c_uint32, _P]),
     "fh_adamw_amp": (_I, [_P, _P, _P, _P, _L, _F, _I, _I, _F, _F, _F, _F, _F, _P, _P]),
 }
 

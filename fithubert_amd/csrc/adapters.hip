@@ -1,0 +1,465 @@
+// Low-rank adapters of many requests beside one frozen projection, forward and backward.
+//
+//   h = s_a x A_a^T          y  = x W^T + bias + h B_a^T          a: the adapter of the row's segment
+//   G = s_a dy B_a           dx = dy W + G A_a          dA_a = sum over a's rows G^T x          dB_a = sum over a's rows dy^T h
+//
+// down:   h and G.  A workgroup owns 16 rows, its four waves split the long reduction (K or N) and join in LDS: one pass over x (dy), many
+//         short workgroups, so that a handful of rows is as quick as its longest load chain.  Rows of several segments: one trip per segment
+//         that the tile touches, dealt over grid.y where requests are short.
+// up:     the products with B_a (A_a), added to the shared projection's GEMM as its residual operand.
+// outer:  dA and dB: a workgroup owns 64 columns of one adapter's factor and walks that adapter's rows, whichever segments they lie in, 32
+//         at a time per wave; long walks are dealt over several workgroups whose partial sums are added in order (no atomics).
+#include "gemm.h"
+#include "kernels.h"
+#include "attn_frag.cuh"
+
+namespace {
+
+struct Segs {
+  const int* start;
+  const int* which;
+  const float* scaling;
+  int n, adapters, M;
+  __device__ __forceinline__ int begin(int s) const { return max(0, min(M, start[s])); }
+  __device__ __forceinline__ int adapter(int s) const { const int a = which[s]; return a >= 0 && a < adapters ? a : -1; }
+  // number of segments that end at or before `row`: the first one that may hold it
+  __device__ __forceinline__ int first_at(int row) const {
+    int lo = 0, hi = n;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (start[mid + 1] <= row) lo = mid + 1; else hi = mid;
+    }
+    return lo;
+  }
+};
+
+// eight (16-bit) or four (fp32) consecutive reduction elements k0 + .. of column `col` of a row-major [k][ld] matrix
+template <typename T> __device__ __forceinline__ typename AT<T>::frag column_frag(const T* w, int k0, int kend, long ld, bool live) {
+  constexpr int VEC = ElemTraits<T>::VEC;
+  union { T e[VEC]; typename AT<T>::frag f; } u;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) u.e[e] = live && k0 + e < kend ? w[(long)(k0 + e) * ld] : from_f<T>(0.f);
+  return u.f;
+}
+
+// out[row][r] = scaling[a] * sum_k x[row][k] f_a(r, k);   COLS: f_a(r, k) = f[a][k][r] (B_a), else f[a][r][k] (A_a)
+template <typename T, int NR, bool COLS>
+__global__ void __launch_bounds__(256) adapter_down_kernel(const Segs g, const T* __restrict__ x, const T* __restrict__ f, T* __restrict__ out, int K, int R) {
+  constexpr int KD = AT<T>::KD, VEC = ElemTraits<T>::VEC;
+  typedef typename AT<T>::frag frag;
+  __shared__ f32x4 part[4][NR][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+  const int i0 = blockIdx.x * 16, i1 = min(i0 + 16, g.M);
+  const int s0 = g.first_at(i0);
+  if (blockIdx.y == 0 && threadIdx.x < 16 * NR) {
+    // rows that no adapter's segment holds: zero (their own store below never comes)
+    const int row = i0 + (threadIdx.x & 15), c = (threadIdx.x >> 4) * 16;
+    if (row < i1) {
+      int s = s0;
+      while (s < g.n && g.start[s + 1] <= row) ++s;
+      if (s >= g.n || g.start[s] > row || g.adapter(s) < 0)
+        for (int j = c; j < min(c + 16, R); ++j) out[(long)row * R + j] = from_f<T>(0.f);
+    }
+  }
+  for (int s = s0 + (int)blockIdx.y; s < g.n; s += (int)gridDim.y) {
+    const int b = max(g.begin(s), i0), e = min(g.begin(s + 1), i1);
+    if (g.begin(s) >= i1) break;
+    const int a = g.adapter(s);
+    if (b >= e || a < 0) continue;
+    const T* fa = f + (long)a * K * R;
+    const T* xr = x + (long)min(i0 + r, g.M - 1) * K;
+    f32x4 acc[NR];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+    for (int k = wave * KD; k < K; k += 4 * KD) {
+      const int k0 = k + VEC * q;
+      frag fx = zero_frag((frag*)nullptr);
+      if (k0 < K) {
+        union { V16 v; frag f; } u;
+        u.v = ld16(xr + k0);
+        fx = u.f;
+      }
+#pragma unroll
+      for (int n = 0; n < NR; ++n) {
+        const int col = 16 * n + r;
+        frag ff;
+        if constexpr (COLS) {
+          ff = column_frag<T>(fa + min(col, R - 1), k0, K, R, col < R);
+        } else {
+          ff = zero_frag((frag*)nullptr);
+          if (col < R && k0 < K) {
+            union { V16 v; frag f; } u;
+            u.v = ld16(fa + (long)col * K + k0);
+            ff = u.f;
+          }
+        }
+        acc[n] = mma<T>(fx, ff, acc[n]);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NR; ++n) part[wave][n][lane] = acc[n];
+    __syncthreads();
+    const float sc = g.scaling[a];
+    for (int n = wave; n < NR; n += 4) {
+      f32x4 v = part[0][n][lane];
+#pragma unroll
+      for (int w = 1; w < 4; ++w)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[c] += part[w][n][lane][c];
+      const int col = 16 * n + r;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int row = i0 + 4 * q + c;
+        if (row >= b && row < e && col < R) out[(long)row * R + col] = from_f<T>(v[c] * sc);   // rounded to the element type: the next product's operand
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// out[i][j] = sum_r h[i][r] f_a(r, j) (0 for rows without an adapter);   COLS: f_a(r, j) = f[a][r][j] (A_a), else f[a][j][r] (B_a)
+template <typename T, bool COLS>
+__global__ void __launch_bounds__(256) adapter_up_kernel(const Segs g, const T* __restrict__ h, const T* __restrict__ f, T* __restrict__ out, int N, int R) {
+  constexpr int KD = AT<T>::KD, VEC = ElemTraits<T>::VEC;
+  typedef typename AT<T>::frag frag;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+  const int i0 = blockIdx.x * 16, j0 = blockIdx.y * 256 + wave * 64, i1 = min(i0 + 16, g.M);
+  if (j0 >= N) return;
+  f32x4 acc[4];
+#pragma unroll
+  for (int n = 0; n < 4; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int s = g.first_at(i0); s < g.n; ++s) {
+    const int b = max(g.begin(s), i0), e = min(g.begin(s + 1), i1);
+    if (g.begin(s) >= i1) break;
+    const int a = g.adapter(s);
+    if (b >= e || a < 0) continue;
+    const T* fa = f + (long)a * N * R;
+    const bool mine = i0 + r >= b && i0 + r < e;
+    for (int k = 0; k < R; k += KD) {
+      const int k0 = k + VEC * q;
+      frag fh = zero_frag((frag*)nullptr);
+      if (mine && k0 < R) {
+        union { V16 v; frag f; } u;
+        u.v = ld16(h + (long)(i0 + r) * R + k0);
+        fh = u.f;
+      }
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const int col = j0 + 16 * n + r;
+        frag ff;
+        if constexpr (COLS) {
+          ff = column_frag<T>(fa + min(col, N - 1), k0, R, N, col < N);
+        } else {
+          ff = zero_frag((frag*)nullptr);
+          if (col < N && k0 < R) {
+            union { V16 v; frag f; } u;
+            u.v = ld16(fa + (long)col * R + k0);
+            ff = u.f;
+          }
+        }
+        acc[n] = mma<T>(ff, fh, acc[n]);   // transposed: a lane holds four neighbouring columns of one row
+      }
+    }
+  }
+  const int row = i0 + r;
+  if (row < i1) {
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const int col = j0 + 16 * n + 4 * q;
+      float v[4] = {acc[n][0], acc[n][1], acc[n][2], acc[n][3]};
+      if (col < N) st4(out + (long)row * N + col, v);
+    }
+  }
+}
+
+// dst[a][r][c] (BY_ROW) or dst[a][c][r] = sum over the rows of adapter a of u[row][r] v[row][c];  with several splits: partial sums
+// [split][a] .. in the same layout
+template <typename T, int NR, bool BY_ROW>
+__global__ void __launch_bounds__(256) adapter_outer_kernel(const Segs g, const T* __restrict__ u, const T* __restrict__ v, float* __restrict__ dst, int C, int R) {
+  constexpr int VEC = ElemTraits<T>::VEC, ES = sizeof(T);
+  constexpr int RU = NR * 16 * ES + 16, RV = 64 * ES + 16;           // LDS row strides
+  constexpr int PER = 32 * (RU + RV), SUM = NR * 4 * 64 * 16;        // a wave's tiles; one wave's sums at the end
+  __shared__ __attribute__((aligned(16))) unsigned char lds[4 * PER > SUM ? 4 * PER : SUM];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
+  const int c0 = blockIdx.x * 64, a = blockIdx.y, split = blockIdx.z, ways = 4 * (int)gridDim.z;
+  unsigned char* tu = lds + wave * PER;
+  unsigned char* tv = tu + 32 * RU;
+  f32x4 acc[NR][4];
+#pragma unroll
+  for (int n = 0; n < NR; ++n)
+#pragma unroll
+    for (int m = 0; m < 4; ++m) acc[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  int turn = 0;                                                      // blocks of 32 rows of this adapter seen so far
+  for (int sb = 0; sb < g.n; sb += 64) {
+    const int s = sb + lane;
+    const bool ours = s < g.n && g.adapter(s) == a;
+    const int b_ = ours ? g.begin(s) : 0, e_ = ours ? g.begin(s + 1) : 0;
+    unsigned long long left = __ballot(b_ < e_);
+    while (left) {
+      const int j = __ffsll((unsigned long long)left) - 1;
+      left &= left - 1;
+      const int b = __builtin_amdgcn_readlane(b_, j), e = __builtin_amdgcn_readlane(e_, j), blocks = (e - b + 31) >> 5;
+      // the blocks of this segment whose turn is ours: turn + k = split * 4 + wave modulo ways
+      int k = (split * 4 + wave - turn % ways + ways) % ways;
+      turn += blocks;
+      for (; k < blocks; k += ways) {
+        const int row0 = b + 32 * k;
+        constexpr int PU = 32 * NR * 16 / VEC / 64, PV = 32 * 64 / VEC / 64;
+        V16 xu[PU > 0 ? PU : 1], xv[PV];
+#pragma unroll
+        for (int p = 0; p < PU; ++p) {
+          const int at = p * 64 + lane, row = at / (NR * 16 / VEC), col = (at % (NR * 16 / VEC)) * VEC;
+          xu[p] = v16_zero();
+          if (row0 + row < e && col < R) xu[p] = ld16(u + (long)(row0 + row) * R + col);
+        }
+#pragma unroll
+        for (int p = 0; p < PV; ++p) {
+          const int at = p * 64 + lane, row = at / (64 / VEC), col = (at % (64 / VEC)) * VEC;
+          xv[p] = v16_zero();
+          if (row0 + row < e && c0 + col < C) xv[p] = ld16(v + (long)(row0 + row) * C + c0 + col);
+        }
+#pragma unroll
+        for (int p = 0; p < PU; ++p) {
+          const int at = p * 64 + lane, row = at / (NR * 16 / VEC), col = (at % (NR * 16 / VEC)) * VEC;
+          st16(tu + row * RU + col * ES, xu[p]);
+        }
+#pragma unroll
+        for (int p = 0; p < PV; ++p) {
+          const int at = p * 64 + lane, row = at / (64 / VEC), col = (at % (64 / VEC)) * VEC;
+          st16(tv + row * RV + col * ES, xv[p]);
+        }
+        // (a wave reads only what it wrote itself, and LDS accesses of one wave stay in order)
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if constexpr (ES == 2) {
+          bf16x8 fv[4];
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+            const unsigned char* p0 = tv + (8 * q + (i >> 2)) * RV + (16 * m + 4 * (i & 3)) * 2;
+            union { struct { s16x4 lo, hi; } s; bf16x8 v; } w;
+            w.s.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p0);
+            w.s.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p0 + 4 * RV));
+            fv[m] = w.v;
+          }
+#pragma unroll
+          for (int n = 0; n < NR; ++n) {
+            const unsigned char* p0 = tu + (8 * q + (i >> 2)) * RU + (16 * n + 4 * (i & 3)) * 2;
+            union { struct { s16x4 lo, hi; } s; bf16x8 v; } w;
+            w.s.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p0);
+            w.s.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p0 + 4 * RU));
+#pragma unroll
+            for (int m = 0; m < 4; ++m) acc[n][m] = BY_ROW ? mfma16<T>(fv[m], w.v, acc[n][m]) : mfma16<T>(w.v, fv[m], acc[n][m]);
+          }
+        } else {
+#pragma unroll
+          for (int t = 0; t < 8; ++t) {
+            float fu[NR], fv[4];
+#pragma unroll
+            for (int n = 0; n < NR; ++n) fu[n] = *reinterpret_cast<const float*>(tu + (4 * t + q) * RU + (16 * n + i) * 4);
+#pragma unroll
+            for (int m = 0; m < 4; ++m) fv[m] = *reinterpret_cast<const float*>(tv + (4 * t + q) * RV + (16 * m + i) * 4);
+#pragma unroll
+            for (int n = 0; n < NR; ++n)
+#pragma unroll
+              for (int m = 0; m < 4; ++m)
+                acc[n][m] = BY_ROW ? __builtin_amdgcn_mfma_f32_16x16x4f32(fv[m], fu[n], acc[n][m], 0, 0, 0)
+                                   : __builtin_amdgcn_mfma_f32_16x16x4f32(fu[n], fv[m], acc[n][m], 0, 0, 0);
+          }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+      }
+    }
+  }
+  // the four waves' sums, in their order
+  f32x4* sum = reinterpret_cast<f32x4*>(lds);
+  for (int w = 0; w < 4; ++w) {
+    __syncthreads();
+    if (wave == w) {
+#pragma unroll
+      for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          f32x4 t = acc[n][m];
+          if (w > 0) {
+            const f32x4 o = sum[(n * 4 + m) * 64 + lane];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) t[c] += o[c];
+          }
+          sum[(n * 4 + m) * 64 + lane] = t;
+        }
+    }
+  }
+  __syncthreads();
+  float* d = dst + ((long)split * g.adapters + a) * C * R;
+  for (int t = wave; t < NR * 4; t += 4) {
+    const int n = t >> 2, m = t & 3;
+    const f32x4 o = sum[t * 64 + lane];
+    float w[4] = {o[0], o[1], o[2], o[3]};
+    if constexpr (BY_ROW) {   // tile rows: columns c, tile columns: r
+      const int c = c0 + 16 * m + 4 * q, rr = 16 * n + i;
+      if (c < C && rr < R) st4(d + (long)rr * C + c, w);
+    } else {
+      const int rr = 16 * n + 4 * q, c = c0 + 16 * m + i;
+      if (c < C && rr < R) st4(d + (long)c * R + rr, w);
+    }
+  }
+}
+
+__global__ void __launch_bounds__(256) adapter_join_kernel(const float* __restrict__ part, float* __restrict__ dst, long n4, int splits) {
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n4) return;
+  float s[4] = {0.f, 0.f, 0.f, 0.f}, f[4];
+  for (int k = 0; k < splits; ++k) {
+    ld4(part + ((long)k * n4 + i) * 4, f);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[e] += f[e];
+  }
+  st4(dst + i * 4, s);
+}
+
+// ------------------------------------------------------------------------------------------------ host
+int check(int dtype, const fh_adapter_desc* d) {
+  if (dtype < 0 || dtype > 2) return -941;
+  if (!d || d->M < 0 || d->K < 8 || d->N < 8 || d->K % 8 || d->N % 8) return -942;
+  if (d->R < 8 || d->R > 128 || d->R % 8) return -943;
+  if (d->n_adapters < 1 || d->n_adapters > 65535 || d->n_segments < 0 || d->M > (1 << 30)) return -944;
+  if (d->n_segments > 0 && (!d->seg_start || !d->seg_adapter || !d->scaling)) return -945;
+  return 0;
+}
+Segs segs_of(const fh_adapter_desc* d) {
+  Segs g;
+  g.start = d->seg_start; g.which = d->seg_adapter; g.scaling = d->scaling;
+  g.n = d->n_segments; g.adapters = d->n_adapters; g.M = d->M;
+  return g;
+}
+size_t al16(size_t n) { return (n + 15) & ~(size_t)15; }
+// workgroups per adapter and 64-column tile: about four per CU in all, at least 256 rows each
+int outer_splits(const fh_adapter_desc* d, int C) {
+  const long wgs = (long)d->n_adapters * ((C + 63) / 64);
+  long n = 1024 / wgs;
+  if (n > (d->M + 255) / 256) n = (d->M + 255) / 256;
+  return n < 1 ? 1 : (int)n;
+}
+size_t outer_bytes(const fh_adapter_desc* d, int C) {
+  const int n = outer_splits(d, C);
+  return n > 1 ? al16((size_t)n * d->n_adapters * C * d->R * 4) : 0;
+}
+
+template <typename T, bool COLS> int down(const Segs& g, const void* x, const void* f, void* out, int K, int R, hipStream_t st) {
+  if (g.M == 0) return 0;
+  const int tiles = (g.M + 15) / 16;
+  const long per = 1 + ((long)16 * g.n + g.M - 1) / g.M;   // segments that a tile touches
+  const dim3 grid(tiles, per > 16 ? 16 : (int)per), block(256);
+#define FH_DOWN(NR) hipLaunchKernelGGL((adapter_down_kernel<T, NR, COLS>), grid, block, 0, st, g, (const T*)x, (const T*)f, (T*)out, K, R)
+  if (R <= 16) FH_DOWN(1);
+  else if (R <= 32) FH_DOWN(2);
+  else if (R <= 64) FH_DOWN(4);
+  else FH_DOWN(8);
+#undef FH_DOWN
+  FH_CHECK_LAUNCH();
+  return 0;
+}
+template <typename T, bool COLS> int up(const Segs& g, const void* h, const void* f, void* out, int N, int R, hipStream_t st) {
+  hipLaunchKernelGGL((adapter_up_kernel<T, COLS>), dim3((g.M + 15) / 16, (N + 255) / 256), dim3(256), 0, st, g, (const T*)h, (const T*)f, (T*)out, N, R);
+  FH_CHECK_LAUNCH();
+  return 0;
+}
+template <typename T, bool BY_ROW> int outer(const fh_adapter_desc* d, const void* u, const void* v, float* dst, int C, float* part, hipStream_t st) {
+  const Segs g = segs_of(d);
+  const int n = outer_splits(d, C), R = d->R;
+  float* to = n > 1 ? part : dst;
+  const dim3 grid((C + 63) / 64, d->n_adapters, n), block(256);
+#define FH_OUTER(NR) hipLaunchKernelGGL((adapter_outer_kernel<T, NR, BY_ROW>), grid, block, 0, st, g, (const T*)u, (const T*)v, to, C, R)
+  if (R <= 16) FH_OUTER(1);
+  else if (R <= 32) FH_OUTER(2);
+  else if (R <= 64) FH_OUTER(4);
+  else FH_OUTER(8);
+#undef FH_OUTER
+  FH_CHECK_LAUNCH();
+  if (n > 1) {
+    const long n4 = (long)d->n_adapters * C * R / 4;
+    hipLaunchKernelGGL(adapter_join_kernel, dim3((unsigned)((n4 + 255) / 256)), dim3(256), 0, st, part, dst, n4, n);
+    FH_CHECK_LAUNCH();
+  }
+  return 0;
+}
+
+template <typename T>
+int forward_t(int dtype, const fh_adapter_desc* d, const void* x, const void* w, const float* bias, const void* a, const void* b, void* h, void* y, hipStream_t st) {
+  const Segs g = segs_of(d);
+  if (int rc = down<T, false>(g, x, a, h, d->K, d->R, st)) return rc;
+  if (int rc = up<T, false>(g, h, b, y, d->N, d->R, st)) return rc;
+  GemmParams p = fh_gemm_params();
+  p.X = fh_operand(x, FH_R_CONTIG, d->K);
+  p.Y = fh_operand(w, FH_R_CONTIG, d->K);
+  p.C = y;
+  p.M = d->M; p.N = d->N; p.Kseg = d->K; p.ldc = d->N;
+  p.ep.bias = bias;
+  p.ep.residual = y;
+  return fh_gemm_launch(p, dtype, st);
+}
+template <typename T>
+int backward_t(int dtype, const fh_adapter_desc* d, const void* x, const void* w, const void* a, const void* b, const void* h, const void* dy, void* dx,
+               float* da, float* db, char* scratch, hipStream_t st) {
+  const Segs g = segs_of(d);
+  T* G = (T*)scratch;
+  float* part = (float*)(scratch + al16((size_t)d->M * d->R * sizeof(T)));
+  if (dx || da)
+    if (int rc = down<T, true>(g, dy, b, G, d->N, d->R, st)) return rc;
+  if (dx && d->M > 0) {
+    if (int rc = up<T, true>(g, G, a, dx, d->K, d->R, st)) return rc;
+    GemmParams p = fh_gemm_params();
+    p.X = fh_operand(dy, FH_R_CONTIG, d->N);
+    p.Y = fh_operand(w, FH_R_STRIDED, d->K);
+    p.C = dx;
+    p.M = d->M; p.N = d->K; p.Kseg = d->N; p.ldc = d->K;
+    p.ep.residual = dx;
+    if (int rc = fh_gemm_launch(p, dtype, st)) return rc;
+  }
+  if (da)
+    if (int rc = outer<T, true>(d, G, x, da, d->K, part, st)) return rc;
+  if (db)
+    if (int rc = outer<T, false>(d, h, dy, db, d->N, part, st)) return rc;
+  return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+long fh_adapter_scratch_bytes(int dtype, const fh_adapter_desc* d, int backward) {
+  if (check(dtype, d)) return -1;
+  if (!backward) return 0;
+  const size_t pa = outer_bytes(d, d->K), pb = outer_bytes(d, d->N);
+  return (long)(al16((size_t)d->M * d->R * fh_esize(dtype)) + (pa > pb ? pa : pb));
+}
+
+int fh_adapter_linear_forward(int dtype, const fh_adapter_desc* d, const void* x, const void* w, const float* bias, const void* a, const void* b,
+                              void* h, void* y, void* scratch, fh_stream_t stream) {
+  if (int rc = check(dtype, d)) return rc;
+  (void)scratch;
+  if (d->M == 0) return 0;
+  if (!x || !w || !a || !b || !h || !y) return -946;
+  if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)bias | (uintptr_t)a | (uintptr_t)b | (uintptr_t)h | (uintptr_t)y) & 15) return -947;
+  const hipStream_t st = (hipStream_t)stream;
+  if (dtype == 0) return forward_t<float>(dtype, d, x, w, bias, a, b, h, y, st);
+  if (dtype == 1) return forward_t<bf16>(dtype, d, x, w, bias, a, b, h, y, st);
+  return forward_t<f16>(dtype, d, x, w, bias, a, b, h, y, st);
+}
+
+int fh_adapter_linear_backward(int dtype, const fh_adapter_desc* d, const void* x, const void* w, const void* a, const void* b, const void* h,
+                               const void* dy, void* dx, float* da, float* db, void* scratch, fh_stream_t stream) {
+  if (int rc = check(dtype, d)) return rc;
+  if (!dx && !da && !db) return 0;
+  if (d->M > 0 && (!dy || ((dx || da) && !b) || (dx && (!w || !a)) || (da && !x) || (db && !h) || !scratch)) return -946;
+  if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)a | (uintptr_t)b | (uintptr_t)h | (uintptr_t)dy | (uintptr_t)dx | (uintptr_t)da | (uintptr_t)db | (uintptr_t)scratch) & 15)
+    return -947;
+  const hipStream_t st = (hipStream_t)stream;
+  if (dtype == 0) return backward_t<float>(dtype, d, x, w, a, b, h, dy, dx, da, db, (char*)scratch, st);
+  if (dtype == 1) return backward_t<bf16>(dtype, d, x, w, a, b, h, dy, dx, da, db, (char*)scratch, st);
+  return backward_t<f16>(dtype, d, x, w, a, b, h, dy, dx, da, db, (char*)scratch, st);
+}
+
+}  // extern "C"

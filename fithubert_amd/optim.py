@@ -1,0 +1,174 @@
+"""AdamW over many tensors at once (``fh_adamw_many``, fithubert_amd/csrc/adamw_many.hip), moments in 32 or in 8 bits.
+
+The student's own optimizer step (``fh_adamw`` / ``fh_adamw_amp``, reference train.py:407-421) works on one flat fp32 buffer.  What is
+trained beside the student -- adapters (``fithubert_amd.adapters``), downstream heads, a teacher or upstream that is fine-tuned as an
+ordinary ``nn.Module`` -- comes as a list of tensors, hundreds of them often a few thousand elements long: here the whole list is one
+launch per 160 tensors.
+
+* ``adamw_many``: the functional form; ``adamw_moments`` makes the moments it updates.
+* ``ManyAdamW``: a ``torch.optim.Optimizer`` over it (parameter groups, schedulers, ``state_dict``).
+
+8-bit moments take 2.03 bytes per parameter instead of 8: m and sqrt(v) as e4m3 codes over one fp32 scale per 256 elements, rounded by
+chance with draws that are a function of (seed, place) alone.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import List, Sequence, Tuple
+
+import torch
+
+from . import _lib as L
+
+BLOCK = 256   # elements that share one scale; every tensor's moments begin at a multiple of it
+
+_DT = {torch.float32: L.DT_F32, torch.bfloat16: L.DT_BF16, torch.float16: L.DT_F16}
+
+
+def moment_blocks(sizes: Sequence[int]) -> int:
+    """blocks of 256 elements that tensors of these sizes take in the flat moments"""
+    return sum((n + BLOCK - 1) // BLOCK for n in sizes)
+
+
+def adamw_moments(params: Sequence[torch.Tensor], bits: int = 32) -> List[torch.Tensor]:
+    """Zero moments for ``adamw_many`` over ``params``: [m, v] flat fp32, or with ``bits=8`` [m codes, m scales, root codes, root
+    scales] (float8_e4m3fn, one fp32 scale per 256 elements).  Tensor i's part begins at the block that ``moment_blocks`` of the tensors in
+    front of it gives; what pads its last block stays zero."""
+    if bits not in (8, 32):
+        raise ValueError(f"moments are held in 8 or 32 bits, not {bits}")
+    if not params:
+        raise ValueError("no tensors")
+    nb, dev = moment_blocks([p.numel() for p in params]), params[0].device
+    if bits == 32:
+        return [torch.zeros(nb * BLOCK, device=dev) for _ in range(2)]
+    return [t for _ in range(2) for t in (torch.zeros(nb * BLOCK, device=dev, dtype=torch.uint8).view(torch.float8_e4m3fn), torch.zeros(nb, device=dev))]
+
+
+def adamw_many(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], moments: Sequence[torch.Tensor], *, step: int, lr: float,
+               betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.0, grad_scale: float = 1.0,
+               seed: int = 0) -> None:
+    """One AdamW step in place: m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2 with g = grad * grad_scale, then
+    p = p (1 - lr weight_decay) - lr / (1 - b1^step) m / (sqrt(v) / sqrt(1 - b2^step) + eps); ``step`` counts from 1.
+
+    ``params``: contiguous CUDA tensors of one type (fp32, bf16 or fp16) on one device, none twice and none overlapping another (a tensor given
+    twice is refused; an overlap cannot be seen).  ``grads``: one per parameter, of one type, or None: that parameter and its moments are left
+    alone.  ``moments``: as ``adamw_moments`` makes them, updated in place.  Arithmetic is fp32 throughout; a 16-bit parameter is rounded
+    to nearest once, so a change below half its spacing is lost.  ``seed`` draws the rounding of 8-bit moments: give each step its own
+    (the step's number will do).  Runs on the current stream of the tensors' device; all scalars are part of the launch, so a captured
+    call repeats the same ``step`` and ``seed`` on every replay."""
+    if len(params) != len(grads):
+        raise ValueError(f"{len(params)} parameters and {len(grads)} gradients")
+    if not params:
+        return
+    with torch.no_grad():
+        p0 = params[0]
+        dev, pdt = p0.device, p0.dtype
+        if pdt not in _DT or dev.type != "cuda":
+            raise ValueError(f"parameters are fp32, bf16 or fp16 tensors on the GPU, got {pdt} on {dev}")
+        gdt, held = None, []
+        for p, g in zip(params, grads):
+            if p.dtype != pdt or p.device != dev or not p.is_contiguous():
+                raise ValueError(f"parameters are contiguous, of one type and on one device: got {tuple(p.shape)} {p.dtype} on {p.device} beside {pdt} on {dev}")
+            if g is None:
+                held.append(None)
+                continue
+            if gdt is None:
+                gdt = g.dtype
+            if g.dtype != gdt or g.device != dev or g.shape != p.shape or g.layout != torch.strided:
+                raise ValueError(f"gradients are dense, of one type and of their parameter's shape and device: got {tuple(g.shape)} {g.dtype} on {g.device} for {tuple(p.shape)}")
+            held.append(g if g.is_contiguous() else g.contiguous())
+        if gdt is None:
+            return
+        if gdt not in _DT:
+            raise ValueError(f"gradients are fp32, bf16 or fp16, got {gdt}")
+        sizes = [p.numel() for p in params]
+        at = [p.data_ptr() for p in params]
+        full = [a for a, k in zip(at, sizes) if k]
+        if len(set(full)) != len(full):
+            raise ValueError("a parameter is given twice")
+        bits = {2: 32, 4: 8}.get(len(moments))
+        nb = moment_blocks(sizes)
+        want = [(torch.float32, nb * BLOCK)] * 2 if bits == 32 else [(torch.float8_e4m3fn, nb * BLOCK), (torch.float32, nb)] * 2
+        if bits is None or any(t.dtype != d or t.numel() != k or t.device != dev or not t.is_contiguous() for t, (d, k) in zip(moments, want)):
+            raise ValueError(f"moments do not fit the parameters ({nb} blocks on {dev}): make them with adamw_moments")
+        n = len(params)
+        mp = [t.data_ptr() for t in moments]
+        m, ms, v, vs = (mp[0], None, mp[1], None) if bits == 32 else mp
+        with torch.cuda.device(dev):
+            L.check(L.lib().fh_adamw_many(_DT[pdt], _DT[gdt], (C.c_void_p * n)(*at), (C.c_void_p * n)(*[g.data_ptr() if g is not None else None for g in held]),
+                                          (C.c_long * n)(*sizes), n, bits, m, ms, v, vs, lr, betas[0], betas[1], eps, weight_decay, step, grad_scale,
+                                          seed & 0xFFFFFFFF, torch.cuda.current_stream(dev).cuda_stream), "fh_adamw_many")
+        torch.autograd.graph.increment_version([p for p, g in zip(params, held) if g is not None])
+
+
+class ManyAdamW(torch.optim.Optimizer):
+    """``torch.optim.AdamW`` in one launch per parameter group (and type), with ``bits`` = 32 or 8 bits per moment.
+
+    The step count is the group's own (a parameter without a gradient is left out of a step and still shares the count).  ``step`` takes a
+    ``grad_scale`` (1 / (world * accumulation * loss scale)).  Sparse gradients and steps inside a graph capture are refused: the step number
+    would be the same on every replay."""
+
+    def __init__(self, params, lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, bits: int = 32):
+        if lr < 0 or eps < 0 or weight_decay < 0 or not all(0 <= b < 1 for b in betas):
+            raise ValueError(f"lr {lr}, betas {betas}, eps {eps}, weight_decay {weight_decay}")
+        if bits not in (8, 32):
+            raise ValueError(f"moments are held in 8 or 32 bits, not {bits}")
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, bits=bits, steps=0))
+        self._moments = {}   # (group, device, type) -> [tensors, moments]
+
+    def _sets(self, k, group):
+        sets = {}
+        for p in group["params"]:
+            sets.setdefault((k, str(p.device), str(p.dtype)), []).append(p)
+        for key, ps in sets.items():
+            held = self._moments.get(key)
+            if held is None or len(held[0]) != len(ps) or any(a is not b for a, b in zip(held[0], ps)):
+                if held is not None:
+                    raise RuntimeError("parameters were added to a group after its first step: add them as a group of their own")
+                self._moments[key] = held = [ps, adamw_moments(ps, group["bits"])]
+            yield held
+
+    @torch.no_grad()
+    def step(self, closure=None, grad_scale: float = 1.0):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("ManyAdamW.step inside a graph capture would repeat one step number: call adamw_many with scalars of your own")
+        for k, group in enumerate(self.param_groups):
+            if all(p.grad is None for p in group["params"]):
+                continue
+            group["steps"] += 1
+            for ps, moments in self._sets(k, group):
+                by = {}
+                for p in ps:
+                    if p.grad is not None:
+                        by.setdefault(p.grad.dtype, None)
+                for dt in by:   # one launch per gradient type; the others' tensors sit it out
+                    adamw_many(ps, [p.grad if p.grad is not None and p.grad.dtype == dt else None for p in ps], moments, step=group["steps"], lr=float(group["lr"]),
+                               betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], grad_scale=grad_scale, seed=group["steps"])
+        return loss
+
+    def state_dict(self):
+        """torch's form with the flat moments of each group under 'moments' (in the order of its parameters, one set per device and type)"""
+        d = super().state_dict()
+        d["moments"] = [[[t.clone() for t in held[1]] for held in self._sets(k, g)] if g["steps"] else None for k, g in enumerate(self.param_groups)]
+        return d
+
+    def load_state_dict(self, state_dict):
+        d = dict(state_dict)
+        saved = d.pop("moments")
+        super().load_state_dict(d)
+        self._moments = {}
+        for k, (group, sets) in enumerate(zip(self.param_groups, saved)):
+            if sets is None:
+                continue
+            here = list(self._sets(k, group))
+            if len(here) != len(sets):
+                raise ValueError(f"group {k}: the state holds {len(sets)} sets of moments, the parameters make {len(here)}")
+            for (_, mine), theirs in zip(here, sets):
+                if [(t.shape, t.dtype) for t in mine] != [(t.shape, t.dtype) for t in theirs]:
+                    raise ValueError(f"group {k}: the state's moments do not fit the parameters")
+                for a, b in zip(mine, theirs):
+                    a.copy_(b)

@@ -1,0 +1,138 @@
+"""Attention inside a sliding window with a few first keys that stay visible (``fh_window_attention_*``,
+fithubert_amd/csrc/window_attention.hip): what replaces the full self-attention of modules/module.py:558-564 where a recording is too
+long for every frame against every frame, and in streaming, where a few new frames meet a cache.
+
+    y = window_attention(q, k, v, left=128, right=16, sinks=4, key_len=lengths)
+
+Differentiable in q, k and v; no T x T tensor exists in either direction.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional, Union
+
+import torch
+
+from . import _lib as L
+
+_DT = {torch.float32: L.DT_F32, torch.bfloat16: L.DT_BF16, torch.float16: L.DT_F16}
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """t itself where the kernels can read it in place: channels contiguous, address and strides multiples of 16 bytes (strides of axes of length 1 do
+    not count); a contiguous copy otherwise"""
+    vec = 16 // t.element_size()
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % vec == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _per_entry(x, B: int, dev: torch.device, name: str) -> Optional[torch.Tensor]:
+    if x is None:
+        return None
+    if not torch.is_tensor(x):
+        return torch.full((B,), int(x), dtype=torch.int32, device=dev)
+    if x.dim() != 1 or x.shape[0] != B or x.dtype.is_floating_point or x.dtype == torch.bool:
+        raise ValueError(f"{name}: one integer per entry ({B}), got {tuple(x.shape)} {x.dtype}")
+    return x.to(device=dev, dtype=torch.int32).contiguous()
+
+
+def _desc(q, k, v, left, right, sinks, scale, key_len, q_start) -> L.WindowAttentionC:
+    d = L.WindowAttentionC()
+    d.B, d.Tq, d.Hq, d.dh = q.shape
+    d.Tk, d.Hkv = k.shape[1], k.shape[2]
+    d.left, d.right, d.sinks, d.scale = left, right, sinks, scale
+    d.key_len = key_len.data_ptr() if key_len is not None else None
+    d.q_start = q_start.data_ptr() if q_start is not None else None
+    for n, t in (("q", q), ("k", k), ("v", v)):
+        for axis, i in (("_bs", 0), ("_ts", 1), ("_hs", 2)):
+            setattr(d, n + axis, t.stride(i) if t.shape[i] > 1 else 0)   # (an axis of length 1 is never stepped along)
+    return d
+
+
+def _scratch(dt, d, backward, dev):
+    n = L.lib().fh_window_attention_scratch_bytes(dt, C.byref(d), backward)
+    if n < 0:
+        raise ValueError("fh_window_attention: arguments refused")
+    return torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+
+
+def _ptr(t):
+    return t.data_ptr() if t is not None else None
+
+
+def _forward(q, k, v, conf, want_lse):
+    left, right, sinks, scale, key_len, q_start = conf
+    dt, dev = _DT[q.dtype], q.device
+    d = _desc(q, k, v, left, right, sinks, scale, key_len, q_start)
+    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev) if want_lse else None
+    with torch.cuda.device(dev):
+        scratch = _scratch(dt, d, 0, dev)
+        L.check(L.lib().fh_window_attention_forward(dt, C.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(scratch),
+                                                    torch.cuda.current_stream(dev).cuda_stream), "fh_window_attention_forward")
+    return out, lse
+
+
+class _WindowAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, conf):
+        out, lse = _forward(q, k, v, conf, True)
+        ctx.save_for_backward(q, k, v, out, lse)
+        ctx.conf = conf
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lse = ctx.saved_tensors
+        left, right, sinks, scale, key_len, q_start = ctx.conf
+        dt, dev = _DT[q.dtype], q.device
+        d = _desc(q, k, v, left, right, sinks, scale, key_len, q_start)
+        dout = dout.contiguous()
+        if dout.data_ptr() % 16:
+            dout = dout.clone()
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
+        with torch.cuda.device(dev):
+            scratch = _scratch(dt, d, 1, dev)
+            L.check(L.lib().fh_window_attention_backward(dt, C.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(), lse.data_ptr(),
+                                                         dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(scratch), torch.cuda.current_stream(dev).cuda_stream),
+                    "fh_window_attention_backward")
+        return dq, dk, dv, None
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, left: int = -1, right: int = -1, sinks: int = 0,
+                     key_len: Optional[torch.Tensor] = None, q_start: Union[None, int, torch.Tensor] = None, scale: Optional[float] = None) -> torch.Tensor:
+    """softmax(scale q k^T over the visible keys) v -> [B][Tq][Hq][dh].
+
+    ``q`` [B][Tq][Hq][dh], ``k``, ``v`` [B][Tk][Hkv][dh]: fp32, bf16 or fp16 on one GPU, dh a multiple of 8 up to 128, Hq a multiple of Hkv (query head h
+    reads key head h // (Hq // Hkv)).  Any strides with contiguous channels -- slices of a packed q|k|v projection, a cache longer than it is
+    filled -- are read in place when addresses and strides are multiples of 16 bytes, copied otherwise.
+
+    Query i of entry b stands at position p = ``q_start[b]`` + i (default 0; required as soon as Tq != Tk) and sees key s when s < ``key_len[b]``
+    (default Tk), s <= p + ``right`` and (s >= p - ``left`` or s < ``sinks``); a negative ``left`` or ``right`` is no limit.  A row that sees no key
+    gives zeros and takes part in no gradient.  Keys that no row of the call sees may hold anything; an infinity or NaN in a key that some rows see
+    may reach rows near them that do not (0 x inf).  ``scale`` > 0, default dh ** -0.5.
+
+    16-bit modes round the probabilities (backward: and dS) to the element type in front of the second products; softmax and sums are fp32.  Nothing
+    depends on the order of atomics: equal calls give equal bits."""
+    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+        raise ValueError(f"q [B][Tq][Hq][dh], k and v [B][Tk][Hkv][dh]: got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if q.dtype not in _DT or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"q, k, v are fp32, bf16 or fp16, all of one type: got {q.dtype}, {k.dtype}, {v.dtype}")
+    if q.device.type != "cuda" or k.device != q.device or v.device != q.device:
+        raise ValueError(f"q, k, v live on one GPU: got {q.device}, {k.device}, {v.device}")
+    B, Tq, Hq, dh = q.shape
+    if Hq < 1 or k.shape[2] < 1 or Hq % k.shape[2] or dh % 8 or not 8 <= dh <= 128:
+        raise ValueError(f"heads of 8 to 128 channels (a multiple of 8), query heads a multiple of key heads: got {Hq} x {dh} over {k.shape[2]}")
+    if q_start is None and Tq != k.shape[1]:
+        raise ValueError(f"{Tq} queries and {k.shape[1]} keys: q_start says where the queries stand")
+    scale = dh ** -0.5 if scale is None else float(scale)
+    if not 0 < scale < float("inf"):
+        raise ValueError(f"scale {scale}")
+    far = (1 << 31) - 1
+    conf = (min(int(left), far), min(int(right), far), max(0, min(int(sinks), far)), scale, _per_entry(key_len, B, q.device, "key_len"), _per_entry(q_start, B, q.device, "q_start"))
+    conf = tuple(max(x, -1) if i < 2 else x for i, x in enumerate(conf))
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _WindowAttention.apply(_aligned(q), _aligned(k), _aligned(v), conf)
+    return _forward(_aligned(q), _aligned(k), _aligned(v), conf, False)[0]

@@ -260,6 +260,60 @@ int fh_attention_backward_bias(int dtype, const void* qkv, const void* out, cons
                                float* scratch, fh_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Attention inside a sliding window with a few first keys that stay visible, forward and backward: the self-attention of
+ * modules/module.py:558-564 for recordings on which every frame against every frame is out of reach, and for streaming.
+ * Query i of entry b stands at position p = q_start[b] + i and sees key s when
+ *     s < key_len[b]   and   s <= p + right   and   (s >= p - left  or  s < sinks).
+ *   out = softmax(scale * q k^T over the keys it sees) v;   a row that sees none: out = 0, and it takes part in no gradient.
+ * q [B][Tq][Hq][dh], k, v [B][Tk][Hkv][dh] by the strides below (elements; channels contiguous; addresses and strides multiples of 16
+ * bytes), so a packed q|k|v projection or a longer cache is read in place; query head h reads key head h / (Hq / Hkv).
+ * out, dout, dq [B][Tq][Hq][dh] and dk, dv [B][Tk][Hkv][dh] are contiguous; lse: B * Tq * Hq floats that the backward reads (forward: NULL
+ * when there is none).  dq, dk, dv are written, not added to (keys that no row sees: 0).  dh <= 128, a multiple of 8; 16-bit modes round the
+ * probabilities and dS to the element type before the second products, sums and softmax are fp32.  No atomics: results repeat bit for bit.
+ * scratch: fh_window_attention_scratch_bytes(dtype, d, 0 forward | 1 backward) bytes, 16-byte aligned (0: NULL will do).  A few rows
+ * against long caches are split over the keys and joined through it.
+ * ------------------------------------------------------------------------------------------ */
+typedef struct {
+  int B, Tq, Tk, Hq, Hkv, dh;
+  int left, right, sinks; /* left / right < 0: no limit on that side */
+  float scale;
+  const int* key_len;     /* device [B], clipped to [0, Tk]; NULL: Tk */
+  const int* q_start;     /* device [B]; NULL: 0 */
+  long q_bs, q_ts, q_hs;  /* strides over entries, frames, heads */
+  long k_bs, k_ts, k_hs;
+  long v_bs, v_ts, v_hs;
+} fh_window_attention_desc;
+long fh_window_attention_scratch_bytes(int dtype, const fh_window_attention_desc* d, int backward);
+int fh_window_attention_forward(int dtype, const fh_window_attention_desc* d, const void* q, const void* k, const void* v, void* out,
+                                float* lse, void* scratch, fh_stream_t stream);
+int fh_window_attention_backward(int dtype, const fh_window_attention_desc* d, const void* q, const void* k, const void* v, const void* out,
+                                 const void* dout, const float* lse, void* dq, void* dk, void* dv, void* scratch, fh_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Low-rank adapters of many requests beside one frozen projection (any nn.Linear of modules/module.py:498-515 or of the teacher):
+ *   y[i] = x[i] W^T + bias + scaling[a] (x[i] A_a^T) B_a^T,     a = seg_adapter[s] of the segment s that row i lies in.
+ * x [M][K], W [N][K], A [n_adapters][R][K], B [n_adapters][N][R], y [M][N] (dtype); bias fp32 [N] or NULL; scaling fp32 [n_adapters].
+ * Segment s is the rows [seg_start[s], seg_start[s + 1]) (device, n_segments + 1 values, ascending; clipped to [0, M]); seg_adapter[s] outside
+ * [0, n_adapters), rows in front of the first and behind the last segment: the shared projection alone.  Several segments may name one
+ * adapter.  h [M][R] (dtype) receives scaling[a] x A_a^T, 0 on rows without an adapter: what the backward reads.
+ * Backward (W and bias are frozen): dx = dy W + G A_a with G = scaling[a] dy B_a; da = sum G^T x; db = sum dy^T h -- da, db fp32, written, 0
+ * for an adapter without rows.  dx, da or db may be NULL.  16-bit modes round h and G to the element type, sums are fp32; no atomics.
+ * K, N, R multiples of 8, R <= 128; every tensor contiguous and 16-byte aligned.
+ * scratch: fh_adapter_scratch_bytes(dtype, d, 0 forward | 1 backward) bytes, 16-byte aligned (0: NULL will do).
+ * ------------------------------------------------------------------------------------------ */
+typedef struct {
+  int M, K, N, R, n_adapters, n_segments;
+  const int* seg_start;
+  const int* seg_adapter;
+  const float* scaling;
+} fh_adapter_desc;
+long fh_adapter_scratch_bytes(int dtype, const fh_adapter_desc* d, int backward);
+int fh_adapter_linear_forward(int dtype, const fh_adapter_desc* d, const void* x, const void* w, const float* bias, const void* a, const void* b,
+                              void* h, void* y, void* scratch, fh_stream_t stream);
+int fh_adapter_linear_backward(int dtype, const fh_adapter_desc* d, const void* x, const void* w, const void* a, const void* b, const void* h,
+                               const void* dy, void* dx, float* da, float* db, void* scratch, fh_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
  * Layer-wise KD loss + gradient (train.py:250-293,372-378):  out[l] = mean_{b,t,d} f(pred_l - teacher_{tl[l]}),
  * out[L] = sum_l w[l] * out[l];  dpred_l = grad_scale * w[l] * f'(.) / (B*Tp*P).  loss_type 0 = mse, 1 = l1.
  * pred [L][B][Tp][P] (dtype); teacher [..][B][Tt][P] (teacher_dtype), narrowed to Tp frames (train.py:282).
@@ -306,6 +360,21 @@ typedef struct {
 } fh_amp_state;
 int fh_adamw_amp(float* p, const float* g, float* m, float* v, long n, float lr_peak, int warmup_steps, int total_steps, float beta1,
                  float beta2, float eps, float wd, float grad_scale, fh_amp_state* state, fh_stream_t stream);
+
+/* One AdamW step over `count` tensors at once (what torch.optim.AdamW's foreach path does for the parameters that the flat fh_adamw does not
+ * hold: adapters, downstream heads, a fine-tuned upstream):
+ *   g = g[i] * grad_scale;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;
+ *   p = p (1 - lr wd) - lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps)          step >= 1
+ * p, g, n: HOST arrays of device pointers and element counts (g[i] NULL: tensor i and its moments are left as they are).  The moments of all
+ * tensors lie in one flat buffer of fh_adamw_many_blocks(n, count) blocks of 256 elements, every tensor padded to whole blocks (zeros).
+ * bits = 32: m, v fp32.  bits = 8: m and sqrt(v) as e4m3 codes (bytes) over one fp32 scale per block (m_scale, v_scale; largest magnitude / 448),
+ * rounded up with the probability of their fraction; the draws are a hash of (seed, place), a root that is not zero stays so, an
+ * element that is not finite is held as NaN and stays out of the scale.  p and g may lie at any element's address (16-byte aligned ones are faster); m and v
+ * at 16 bytes.  One launch per 160 tensors; the table travels in the launch's arguments. */
+long fh_adamw_many_blocks(const long* n, int count);
+int fh_adamw_many(int p_dtype, int g_dtype, void* const* p, const void* const* g, const long* n, int count, int bits, void* m, float* m_scale,
+                  void* v, float* v_scale, double lr, double beta1, double beta2, double eps, double wd, long step, double grad_scale,
+                  uint32_t seed, fh_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------
  * Student engine: the whole CustomStudentModel forward (modules/model.py:420-552) and its backward as ONE

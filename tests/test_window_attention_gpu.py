@@ -1,0 +1,266 @@
+"""GPU: window attention (fithubert_amd.window_attention) against its definition in 64 bits, forward and backward.
+
+Tolerances are elementwise and follow from the roundings (u = eps / 2 of the element type, nz = the fp32 part):
+  scores            off by at most ds = (dh + 8) 2^-24 max sum |q k| scale (a dot product of dh terms and the scaling), so a probability by a
+                    factor 1 +- 2 (ds + 2^-21) (its own score and the log-sum-exp's; v_exp_f32 and the sums: the 2^-21)
+  nz                2 (ds + 2^-21) + n 2^-24  (a sum over n keys or rows)
+  out               u sum P|v| (P rounded in front of the product) + u |out| + nz sum P|v|
+  dS = scale P (dP - D): u |dS| (rounded) + nz scale P (|dout||v| + |D|) + scale P eD, eD = sum |dout| e_out (D reads the rounded out)
+  dq, dk            the error of dS times |k|, |q| summed, + u |result| + nz sum |dS||k|;   dv: u sum P|dout| + u |dv| + nz sum P|dout|
+fp16 adds half its smallest spacing, 2^-25, per rounded P, dS and stored value."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from fithubert_amd.window_attention import window_attention  # noqa: E402
+
+DEV = "cuda"
+
+
+def seen(Tq, Tk, key_len, q_start, left, right, sinks):
+    p = (q_start[:, None] + torch.arange(Tq, device=DEV))[:, :, None]
+    s = torch.arange(Tk, device=DEV)[None, None]
+    m = (s < key_len[:, None, None]).expand(-1, Tq, -1)
+    if right >= 0:
+        m = m & (s <= p + right)
+    return m & ((s >= p - left) | (s < sinks)) if left >= 0 else m
+
+
+def reference(q, k, v, dout, mask, scale):
+    """values and bounds in 64 bits: {name: (value, bound)}"""
+    u = torch.finfo(q.dtype).eps / 2 if q.dtype != torch.float32 else 2.0 ** -24
+    low = q.dtype != torch.float32
+    tiny = 2.0 ** -25 if q.dtype == torch.float16 else 0.0
+    B, Tq, Hq, dh = q.shape
+    G = Hq // k.shape[2]
+    Q, K, V = q.double().permute(0, 2, 1, 3), k.double().permute(0, 2, 1, 3).repeat_interleave(G, 1), v.double().permute(0, 2, 1, 3).repeat_interleave(G, 1)
+    hidden = ~mask[:, None]
+    K, V = (torch.where(mask.any(1)[:, None, :, None], t, 0.0) for t in (K, V))        # (what nobody sees may be anything)
+    x = (Q @ K.transpose(2, 3) * scale).masked_fill(hidden, -math.inf)
+    ds_max = (dh + 8) * 2.0 ** -24 * (Q.abs() @ K.abs().transpose(2, 3) * scale).max().item()
+    P = torch.exp(x - x.amax(-1, keepdim=True).clamp_min(-1e300))
+    P = torch.where(hidden, 0.0, P)
+    P = P / P.sum(-1, keepdim=True).clamp_min(1e-300)
+    n = max(mask.sum(-1).max().item(), mask.sum(1).max().item() * G) + 8
+    nz = 2 * (ds_max + 2.0 ** -21) + n * 2.0 ** -24
+    up = u if low else 0.0
+    vis = mask[:, None].double()
+    out = P @ V
+    pv = P @ V.abs()
+    e_out = (up + nz) * pv + u * out.abs() + tiny * (vis @ V.abs()) + tiny
+    back = lambda t: t.permute(0, 2, 1, 3)  # noqa: E731
+    fold = lambda t: back(t).reshape(B, -1, k.shape[2], G, dh).sum(3)  # noqa: E731
+    res = {"out": (back(out), back(e_out))}
+    if dout is None:
+        return res
+    dO = dout.double().permute(0, 2, 1, 3)
+    D = (dO * out).sum(-1, keepdim=True)
+    eD = (dO.abs() * e_out).sum(-1, keepdim=True) + dh * 2.0 ** -24 * (dO.abs() * out.abs()).sum(-1, keepdim=True)
+    dS = scale * P * (dO @ V.transpose(2, 3) - D)
+    e_dS = up * dS.abs() + nz * scale * P * (dO.abs() @ V.abs().transpose(2, 3) + D.abs()) + scale * P * eD + tiny * vis
+    Pt, St, Et = P.transpose(2, 3), dS.transpose(2, 3), e_dS.transpose(2, 3)
+    dq, dk, dv = dS @ K, St @ Q, Pt @ dO
+    res["dq"] = (back(dq), back(e_dS @ K.abs() + u * dq.abs() + nz * (dS.abs() @ K.abs()) + tiny))
+    dk, dv = fold(dk), fold(dv)
+    res["dk"] = (dk, fold(Et @ Q.abs() + nz * (St.abs() @ Q.abs())) + u * dk.abs() + tiny)
+    res["dv"] = (dv, fold((up + nz) * (Pt @ dO.abs()) + tiny * (vis.transpose(2, 3) @ dO.abs())) + u * dv.abs() + tiny)
+    return res
+
+
+def near(name, got, value, bound):
+    off = (got.double() - value).abs()
+    assert torch.isfinite(got).all(), name
+    worst = (off / bound.clamp_min(1e-300)).max().item()
+    assert (off <= bound + 1e-30).all(), f"{name}: {worst:.2f} times its bound"
+
+
+def inputs(seed, dtype, B, Tq, Tk, Hq, Hkv, dh, packed=False):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    if packed:
+        x = torch.randn(B, Tk, (Hq + 2 * Hkv) * dh, device=DEV, generator=g).to(dtype)
+        q, k, v = x.split([Hq * dh, Hkv * dh, Hkv * dh], -1)
+        return q.view(B, Tq, Hq, dh), k.view(B, Tk, Hkv, dh), v.view(B, Tk, Hkv, dh), torch.randn(B, Tq, Hq, dh, device=DEV, generator=g).to(dtype)
+    return tuple(torch.randn(*s, device=DEV, generator=g).to(dtype) for s in ((B, Tq, Hq, dh), (B, Tk, Hkv, dh), (B, Tk, Hkv, dh), (B, Tq, Hq, dh)))
+
+
+def run(q, k, v, dout, **kw):
+    q, k, v = (t.detach().requires_grad_(True) for t in (q, k, v))
+    out = window_attention(q, k, v, **kw)
+    return dict(zip(("out", "dq", "dk", "dv"), (out.detach(),) + torch.autograd.grad(out, (q, k, v), dout)))
+
+
+def check(q, k, v, dout, left, right, sinks, key_len=None, q_start=None, scale=None):
+    B, Tq = q.shape[:2]
+    kl = torch.full((B,), k.shape[1], device=DEV) if key_len is None else torch.tensor(key_len, device=DEV)
+    qs = torch.zeros(B, dtype=torch.long, device=DEV) if q_start is None else torch.tensor(q_start, device=DEV)
+    ref = reference(q, k, v, dout, seen(Tq, k.shape[1], kl, qs, left, right, sinks), scale or q.shape[3] ** -0.5)
+    kw = dict(left=left, right=right, sinks=sinks, scale=scale, key_len=None if key_len is None else kl.int(), q_start=None if q_start is None else qs.int())
+    got = run(q, k, v, dout, **kw) if dout is not None else {"out": window_attention(q, k, v, **kw)}
+    for n in got:
+        near(n, got[n], *ref[n])
+    return got
+
+
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,Hq,Hkv,dh,left,right,sinks", [
+    (1, 1, 1, 8, 0, 0, 0), (2, 3, 1, 40, 0, 0, 1), (63, 4, 4, 64, 10, 0, 0), (64, 2, 1, 128, 5, 5, 2), (65, 12, 12, 40, 64, 64, 0),
+    (129, 8, 2, 64, 31, 0, 4), (200, 6, 2, 80, 17, 40, 130), (257, 4, 1, 96, 100, 3, 64), (321, 5, 1, 48, -1, 0, 0), (190, 2, 2, 56, 20, -1, 3),
+    (130, 2, 2, 64, -1, -1, 0), (515, 4, 2, 128, 70, 0, 16), (700, 2, 1, 64, 0, 0, 0), (400, 3, 3, 72, 5, 200, 1000)])
+def test_self_attention(dtype, T, Hq, Hkv, dh, left, right, sinks):
+    q, k, v, dout = inputs(T + dh, dtype, 2, T, T, Hq, Hkv, dh)
+    check(q, k, v, dout, left, right, sinks)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("left,right,sinks", [(20, 0, 0), (20, 10, 5), (0, 0, 0), (-1, 0, 0), (3, -1, 0)])
+def test_ragged_lengths_leave_rows_without_keys(dtype, left, right, sinks):
+    T = 150
+    q, k, v, dout = inputs(7, dtype, 5, T, T, 4, 2, 40)
+    got = check(q, k, v, dout, left, right, sinks, key_len=[T, 0, 1, 64, 97])
+    assert (got["out"][1] == 0).all() and all((got[n][1] == 0).all() for n in ("dq", "dk", "dv"))
+    if left == 20 and sinks == 0:
+        assert (got["out"][2, 22:] == 0).all() and (got["dq"][2, 22:] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_what_no_row_sees_may_be_anything(dtype):
+    T = 200
+    q, k, v, dout = inputs(3, dtype, 2, T, T, 4, 2, 64)
+    clean = run(q, k, v, dout, left=16, right=0, sinks=2, key_len=torch.tensor([120, T], device=DEV))
+    for bad in (math.inf, -math.inf, math.nan, torch.finfo(dtype).min):
+        k2, v2 = k.clone(), v.clone()
+        k2[0, 120:], v2[0, 120:] = bad, bad
+        dirty = run(q, k2, v2, dout, left=16, right=0, sinks=2, key_len=torch.tensor([120, T], device=DEV))
+        for n in clean:
+            assert torch.equal(clean[n], dirty[n]), (n, bad)
+        # a cache that is longer than what it holds, and whose oldest frames have been given back
+        new = window_attention(q[:, 90:92], k, v, left=16, right=0, sinks=2, q_start=torch.tensor([90, 90], device=DEV))
+        k2, v2 = k.clone(), v.clone()
+        k2[:, 92:], v2[:, 92:] = bad, bad
+        k2[:, 2:74], v2[:, 2:74] = bad, bad
+        assert torch.equal(new, window_attention(q[:, 90:92], k2, v2, left=16, right=0, sinks=2, q_start=torch.tensor([90, 90], device=DEV))), bad
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,Tq,Tk,Hq,Hkv,dh,left,sinks", [(3, 1, 1000, 8, 2, 64, 255, 4), (2, 1, 4097, 4, 4, 40, -1, 0), (1, 1, 9000, 16, 1, 128, 5000, 7), (2, 7, 640, 6, 6, 96, 64, 70),
+                                                          (1, 16, 3001, 16, 2, 128, -1, 0), (2, 33, 700, 4, 2, 80, 100, 0), (70, 1, 300, 4, 2, 64, 63, 1), (1, 3, 5, 1, 1, 8, 2, 0)])
+def test_a_few_frames_against_a_cache(dtype, B, Tq, Tk, Hq, Hkv, dh, left, sinks):
+    q, k, v, dout = inputs(Tk + Tq, dtype, B, Tq, Tk, Hq, Hkv, dh)
+    lens = [max(Tq, Tk - 13 * b * b) for b in range(B)]
+    check(q, k, v, None, left, 0, sinks, key_len=lens, q_start=[n - Tq for n in lens])
+    check(q, k, v, dout, left, 2, sinks, key_len=lens, q_start=[n - Tq - 1 for n in lens])     # (and its gradients)
+    check(q, k, v, None, left, 0, sinks, key_len=[0] * B, q_start=[n - Tq for n in lens])        # nothing to see
+
+
+def test_chunks_of_a_stream_give_the_whole():
+    T, n = 230, 23
+    q, k, v, _ = inputs(5, torch.float16, 2, T, T, 4, 2, 64)
+    whole = window_attention(q, k, v, left=50, right=0, sinks=3)
+    for i in range(0, T, n):
+        part = window_attention(q[:, i:i + n], k, v, left=50, right=0, sinks=3, q_start=i)
+        value, bound = reference(q[:, i:i + n], k, v, None, seen(n, T, torch.full((2,), T, device=DEV), torch.full((2,), i, device=DEV), 50, 0, 3), 0.125)["out"]
+        near("chunk", part, value, bound)
+        near("whole", whole[:, i:i + n], value, bound)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_packed_projections_and_odd_strides(dtype):
+    q, k, v, dout = inputs(11, dtype, 2, 100, 100, 6, 2, 40, packed=True)
+    assert not q.is_contiguous()
+    a = check(q, k, v, dout, 30, 5, 2)
+    b = run(*(t.contiguous() for t in (q, k, v)), dout, left=30, right=5, sinks=2)
+    assert all(torch.equal(a[n], b[n]) for n in a)
+    # head-major tensors, and slices whose addresses and strides no 16-byte access fits
+    hm = [t.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3) for t in (q, k, v)]
+    odd = []
+    for t in (q, k, v):
+        w = torch.zeros(*t.shape[:3], t.shape[3] + 3, device=DEV, dtype=dtype)
+        w[..., 1:-2] = t
+        odd.append(w[..., 1:-2])
+    for other in (hm, odd):
+        c = run(*other, dout.transpose(1, 2).contiguous().transpose(1, 2), left=30, right=5, sinks=2)
+        assert all(torch.equal(a[n], c[n]) for n in a)
+
+
+def test_gradients_against_differences():
+    T = 40
+    q, k, v, dout = (t.double() for t in inputs(2, torch.float32, 1, T, T, 4, 2, 16))
+    f = lambda a, b, c: (window_attention(a.float(), b.float(), c.float(), left=9, right=2, sinks=2).double() * dout).sum().item()  # noqa: E731
+    got = run(q.float(), k.float(), v.float(), dout.float(), left=9, right=2, sinks=2)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    for i, n in enumerate(("dq", "dk", "dv")):
+        for _ in range(3):
+            d = torch.randn(q.shape if i == 0 else k.shape, device=DEV, generator=g, dtype=torch.float64)
+            h, a, b = 1e-2, [q, k, v], [q, k, v]
+            a[i], b[i] = a[i] + h * d, b[i] - h * d
+            diff = (f(*a) - f(*b)) / (2 * h)
+            # third-order term of the difference (h^2 times values of order 10) and 2^-24 sqrt(2560) |out| of fp32 noise over 2 h
+            assert abs(diff - (got[n].double() * d).sum().item()) < 2e-2 * max(1.0, abs(diff)), n
+
+
+def test_equal_calls_give_equal_bits_and_scale_is_taken():
+    q, k, v, dout = inputs(9, torch.bfloat16, 2, 300, 300, 8, 2, 64)
+    a = check(q, k, v, dout, 60, 0, 140, scale=0.3)
+    for _ in range(3):
+        b = run(q, k, v, dout, left=60, right=0, sinks=140, scale=0.3)
+        assert all(torch.equal(a[n], b[n]) for n in a)
+
+
+def test_streams_and_a_captured_call():
+    q, k, v, dout = inputs(21, torch.bfloat16, 2, 200, 200, 4, 2, 64)
+    want = run(q, k, v, dout, left=40, right=0, sinks=4)
+    token = window_attention(q[:, 150:151], k, v, left=150, right=0, q_start=150)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        got = run(q, k, v, dout, left=40, right=0, sinks=4)
+    torch.cuda.current_stream().wait_stream(st)
+    assert all(torch.equal(want[n], got[n]) for n in want)
+    leaves = [t.detach().clone().requires_grad_(True) for t in (q, k, v)]
+    g = torch.cuda.CUDAGraph()
+    start = torch.tensor([150, 150], dtype=torch.int32, device=DEV)
+    with torch.cuda.stream(st):
+        for _ in range(2):
+            torch.autograd.grad(window_attention(*leaves, left=40, right=0, sinks=4), leaves, dout)
+            window_attention(q[:, 150:151], k, v, left=150, right=0, q_start=start)
+    torch.cuda.current_stream().wait_stream(st)
+    with torch.cuda.graph(g):
+        out = window_attention(*leaves, left=40, right=0, sinks=4)
+        grads = torch.autograd.grad(out, leaves, dout)
+        one = window_attention(q[:, 150:151], k, v, left=150, right=0, q_start=start)
+    for i in range(4):
+        for t in (out, one) + grads:
+            t.detach().zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        for n, t in zip(("out", "dq", "dk", "dv"), (out,) + grads):
+            assert torch.equal(want[n], t), (n, i)
+        assert torch.equal(one, token)
+        torch.randn(1000, 1000, device=DEV).sum().item()
+    with torch.no_grad():                                # new inputs and new positions in the captured buffers
+        leaves[0].copy_(q.flip(1))
+        start.fill_(100)
+    g.replay()
+    torch.cuda.synchronize()
+    again = run(q.flip(1), k, v, dout, left=40, right=0, sinks=4)
+    assert torch.equal(again["dk"], grads[1]) and torch.equal(again["out"], out)
+    assert torch.equal(one, window_attention(q[:, 150:151], k, v, left=150, right=0, q_start=100))
+
+
+def test_a_cache_past_32_bit_offsets():
+    """the last entries of a cache of more than 2^31 elements"""
+    B, Tk, Hkv, dh = 3, 700_000, 8, 128
+    k = torch.empty(B, Tk, Hkv, dh, device=DEV, dtype=torch.float16)
+    k[2, -600:] = torch.randn(600, Hkv, dh, device=DEV)
+    q = torch.randn(B, 1, 16, dh, device=DEV).half()
+    got = window_attention(q, k, k, left=511, right=0, q_start=torch.full((B,), Tk - 1, device=DEV), key_len=torch.tensor([0, 0, Tk], device=DEV))
+    tail = k[2:, -512:].clone()
+    value, bound = reference(q[2:], tail, tail, None, torch.ones(1, 1, 512, dtype=torch.bool, device=DEV), dh ** -0.5)["out"]
+    near("out", got[2:], value, bound)
+    assert (got[:2] == 0).all()
