@@ -4,8 +4,8 @@
 //   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
 // The moments of all tensors lie in one flat buffer, every tensor padded to whole blocks of 256 elements.  A wave owns four
-// neighbouring blocks, whatever tensors they belong to: a lane holds four consecutive elements of each, and all loads of the four
-// blocks are in flight before the first is used.  The tensors travel as a table in the kernel's arguments (no device-side table to
+// neighbouring blocks, whatever tensors they belong to; where they are whole blocks of one tensor (nearly always) all loads of the four
+// are in flight before the first is used.  The tensors travel as a table in the kernel's arguments (no device-side table to
 // upload, so a captured launch is self-contained); a wave finds its tensor by counting, 64 entries per load, how many begin at or
 // before its block.  More than FH_MANY tensors take several launches.
 //
@@ -19,8 +19,10 @@
 // This file is compiled without contraction into fused multiply-adds: codes are a discontinuous function of the moments, and this
 // way each is the same on every path and in any restatement that follows the formulas in fp32.
 //
-// Bound by HBM: 28 bytes per fp32 element with fp32 gradients and 32-bit moments, 16.06 with 8-bit ones, 10.06 with bf16 parameters
-// and gradients.
+// Bound by HBM: 28 bytes per fp32 element with fp32 gradients and 32-bit moments, 16.06 with 8-bit ones, 10.06 with bf16 parameters and
+// gradients.  Measured (a copy runs at 5.2 TB/s): 300 M bf16 parameters, 8-bit moments, 380 tensors: 600 us = 5.0 TB/s; 30 M fp32
+// parameters, 8-bit moments, 200 tensors: 102 us = 4.8 TB/s of kernel time (two launches).  With the compiler's IEEE division and square
+// root, a software rounding to e4m3 and four elements per lane everywhere the first took 934 us: the arithmetic was the bound, not the bytes.
 #include "common.cuh"
 #include "kernels.h"
 #include <cmath>
@@ -45,8 +47,8 @@ struct ManyArgs {
   long block0;                    // this launch's first block in the flat moments
 };
 
-__device__ __forceinline__ float wave_max_dpp(float v) {
-  // max over the 16 lanes of a row by four lane rotations inside the row, then over the rows
+// max over the 64 (HALF: over each 32) lanes of a wave, in every one of them: four lane rotations inside the rows of 16, then over the rows
+template <bool HALF> __device__ __forceinline__ float wave_max_dpp(float v) {
 #define FH_ROW_MAX(ctrl) v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), ctrl, 0xf, 0xf, false)))
   FH_ROW_MAX(0x121);  // row_ror:1
   FH_ROW_MAX(0x122);
@@ -55,19 +57,17 @@ __device__ __forceinline__ float wave_max_dpp(float v) {
 #undef FH_ROW_MAX
   auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  if constexpr (HALF) return v;
   r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-__device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
-
-// |x| * inv as an e4m3 code, rounded up where its fraction exceeds 1 - u; the quantum is 2^(e - 3), e >= -6 (subnormal codes below)
-__device__ __forceinline__ uint32_t e4m3_code(float x, float inv, float u) {
-  const float a = fabsf(x) * inv;
-  const uint32_t ex = max(__float_as_uint(a) >> 23, 121u);
-  const float k = floorf(a * __uint_as_float((257u - ex) << 23) + u);   // a / 2^(ex - 130): exact, below 16
-  const uint32_t c = min(((ex - 120u) << 3) + (uint32_t)k - 8u, 0x7eu);
-  return c | ((__float_as_uint(x) >> 24) & 0x80u);
+// square root to nearest: v_sqrt_f32 is off by one unit at most, and s is too large (small) when x lies below (above) the product of s and its
+// neighbour.  (hipcc's own adds a rescue of x < 2^-96; there this one may be a unit off.)
+__device__ __forceinline__ float sqrt_near(float x) {
+  const float s = __builtin_amdgcn_sqrtf(x), dn = __uint_as_float(__float_as_uint(s) - 1u), up = __uint_as_float(__float_as_uint(s) + 1u);
+  float y = __builtin_fmaf(-dn, s, x) <= 0.f ? dn : s;
+  return __builtin_fmaf(-up, s, x) > 0.f ? up : y;
 }
 __device__ __forceinline__ void e4m3_values(uint32_t c, float (&f)[4]) {
   const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
@@ -92,9 +92,157 @@ template <typename T> __device__ __forceinline__ void st_upto4(T* p, int cnt, bo
   }
 }
 
+// The step on N neighbouring elements of a lane, whose block is the N / 4th part of a wave.  BITS = 8: m, v hold code values on entry, ms / vs the block's
+// scales; `at`: the first element's place in the flat moments.
+template <int BITS, int N>
+__device__ __forceinline__ void update(const ManyArgs& a, float (&p)[N], const float (&g)[N], float (&m)[N], float (&v)[N], float& ms, float& vs, uint32_t at,
+                                       int (&cm)[N / 4], int (&cr)[N / 4]) {
+  float m_top = 0.f, r_top = 0.f;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const float gr = g[e] * a.gscale;
+    if constexpr (BITS == 8) {
+      const float r0 = v[e] * vs;
+      m[e] = m[e] * ms;
+      v[e] = r0 * r0;
+    }
+    m[e] = m[e] * a.b1 + gr * a.c1;
+    v[e] = v[e] * a.b2 + (gr * gr) * a.c2;
+    const float r = sqrt_near(v[e]);
+    // (v_rcp_f32 is off by one unit: nothing beside the 2^-24 of the other steps, and a tenth of a division)
+    p[e] = p[e] * a.decay - a.rate * (m[e] * __builtin_amdgcn_rcpf(r * a.rbc2 + a.eps));
+    if constexpr (BITS == 8) {
+      v[e] = r;
+      m_top = fmaxf(m_top, fabsf(m[e]));   // (a NaN loses against any number)
+      r_top = fmaxf(r_top, r);
+    }
+  }
+  if constexpr (BITS == 8) {
+    constexpr bool HALF = N == 8;
+    m_top = wave_max_dpp<HALF>(m_top);
+    r_top = wave_max_dpp<HALF>(r_top);
+    if (__any(!(m_top < INFINITY) || !(r_top < INFINITY))) {   // an infinity somewhere: the largest of the others
+      m_top = r_top = 0.f;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        m_top = fmaxf(m_top, fabsf(m[e]) < INFINITY ? fabsf(m[e]) : 0.f);
+        r_top = fmaxf(r_top, v[e] < INFINITY ? v[e] : 0.f);
+      }
+      m_top = wave_max_dpp<HALF>(m_top);
+      r_top = wave_max_dpp<HALF>(r_top);
+    }
+    m_top = fmaxf(m_top, TINY);
+    r_top = fmaxf(r_top, TINY);
+    const float m_inv = (1.f / m_top) * E4M3_MAX, r_inv = (1.f / r_top) * E4M3_MAX;
+    ms = m_top * (1.f / E4M3_MAX);
+    vs = r_top * (1.f / E4M3_MAX);
+    // v_cvt_sr_fp8_f32 adds the draw below the code's last bit and cuts: floor(|x| / spacing + draw), subnormal codes included; infinities and
+    // NaN become the code's NaN.  The largest element comes to 448 (1 + 2 2^-24) at most, which no draw of 16 bits lifts to the next code.
+#define FH_CODE(i, e)                                                                                                  \
+  {                                                                                                                    \
+    const uint32_t h = fh_mix32((at + 4 * i + e) ^ a.key);                                                             \
+    const float x = v[4 * i + e] * r_inv;                                                                              \
+    cm[i] = __builtin_amdgcn_cvt_sr_fp8_f32(m[4 * i + e] * m_inv, (int)(h << 16), cm[i], e);                           \
+    cr[i] = __builtin_amdgcn_cvt_sr_fp8_f32(x > 0.f ? fmaxf(x, 0x1p-9f) : x, (int)(h & 0xffff0000u), cr[i], e);        \
+  }
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      cm[i] = cr[i] = 0;
+      FH_CODE(i, 0) FH_CODE(i, 1) FH_CODE(i, 2) FH_CODE(i, 3)
+    }
+#undef FH_CODE
+  }
+}
+
+template <int N> __device__ __forceinline__ void ld_codes(const uint8_t* p, int (&c)[N / 4]) {
+  if constexpr (N == 8) {
+    const int2 x = *(const int2*)p;
+    c[0] = x.x; c[1] = x.y;
+  } else {
+    c[0] = *(const int*)p;
+  }
+}
+template <int N> __device__ __forceinline__ void st_codes(uint8_t* p, const int (&c)[N / 4]) {
+  if constexpr (N == 8) *(int2*)p = make_int2(c[0], c[1]);
+  else *(int*)p = c[0];
+}
+template <typename T, int N> __device__ __forceinline__ void ld_n(const T* p, float (&f)[N]) {
+  if constexpr (N == 8 && sizeof(T) == 2) {
+    unpack16<T>(ld16(p), f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) ld4(p + i, f + i);
+  }
+}
+template <typename T, int N> __device__ __forceinline__ void st_n(T* p, const float (&f)[N]) {
+  if constexpr (N == 8 && sizeof(T) == 2) {
+    st16(p, pack16<T>(f));
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) st4(p + i, f + i);
+  }
+}
+
+// four whole blocks of one tensor, everything aligned: N elements per lane and step, all loads in front of the first use
+template <typename P, typename G, int BITS, int N>
+__device__ __forceinline__ void four_blocks(const ManyArgs& a, P* __restrict__ p_, const G* __restrict__ g_, void* __restrict__ m_, float* __restrict__ m_scale,
+                                            void* __restrict__ v_, float* __restrict__ v_scale, long blk, int lane) {
+  constexpr int STEPS = 16 / N, LB = 256 / N;   // lanes per block
+  float p[STEPS][N], g[STEPS][N], m[STEPS][N], v[STEPS][N], ms[STEPS], vs[STEPS];
+  int cm[STEPS][N / 4], cr[STEPS][N / 4];
+#pragma unroll
+  for (int k = 0; k < STEPS; ++k) {
+    const int off = k * 64 * N + lane * N;
+    const long at = blk * 256 + off, b = blk + k * (N / 4) + lane / LB;
+    ld_n<G, N>(g_ + off, g[k]);
+    ld_n<P, N>(p_ + off, p[k]);
+    if constexpr (BITS == 8) {
+      ld_codes<N>((const uint8_t*)m_ + at, cm[k]);
+      ld_codes<N>((const uint8_t*)v_ + at, cr[k]);
+      ms[k] = m_scale[b];
+      vs[k] = v_scale[b];
+    } else {
+      ld_n<float, N>((const float*)m_ + at, m[k]);
+      ld_n<float, N>((const float*)v_ + at, v[k]);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < STEPS; ++k) {
+    const int off = k * 64 * N + lane * N;
+    const long at = blk * 256 + off, b = blk + k * (N / 4) + lane / LB;
+    if constexpr (BITS == 8) {
+#pragma unroll
+      for (int i = 0; i < N / 4; ++i) {
+        float f[4];
+        e4m3_values((uint32_t)cm[k][i], f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m[k][4 * i + e] = f[e];
+        e4m3_values((uint32_t)cr[k][i], f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[k][4 * i + e] = f[e];
+      }
+    }
+    update<BITS, N>(a, p[k], g[k], m[k], v[k], ms[k], vs[k], (uint32_t)at, cm[k], cr[k]);
+    st_n<P, N>(p_ + off, p[k]);
+    if constexpr (BITS == 8) {
+      st_codes<N>((uint8_t*)m_ + at, cm[k]);
+      st_codes<N>((uint8_t*)v_ + at, cr[k]);
+      if (lane % LB == 0) {
+        m_scale[b] = ms[k];
+        v_scale[b] = vs[k];
+      }
+    } else {
+      st_n<float, N>((float*)m_ + at, m[k]);
+      st_n<float, N>((float*)v_ + at, v[k]);
+    }
+  }
+}
+
 template <typename P, typename G, int BITS>
 __global__ void __launch_bounds__(256) adamw_many_kernel(const ManyTable tab, const ManyArgs a, void* __restrict__ m_, float* __restrict__ m_scale,
                                                          void* __restrict__ v_, float* __restrict__ v_scale) {
+  // 16-bit parameters with 8-bit moments: eight elements per lane, so that parameters and gradients move 16 bytes at a time
+  constexpr int N = BITS == 8 && sizeof(P) == 2 ? 8 : 4;
   const int lane = threadIdx.x & 63;
   const int b0 = __builtin_amdgcn_readfirstlane(blockIdx.x * WG_BLOCKS + (threadIdx.x >> 6) * WAVE_BLOCKS);
   if (b0 >= a.blocks) return;
@@ -105,92 +253,52 @@ __global__ void __launch_bounds__(256) adamw_many_kernel(const ManyTable tab, co
     t += __popcll(__ballot(j < a.count && tab.first[min(j, FH_MANY - 1)] <= b0));
   }
   t = __builtin_amdgcn_readfirstlane(t);
-  float p[WAVE_BLOCKS][4], g[WAVE_BLOCKS][4], m[WAVE_BLOCKS][4], v[WAVE_BLOCKS][4], ms[WAVE_BLOCKS], vs[WAVE_BLOCKS];
-  uint32_t mc[WAVE_BLOCKS], vc[WAVE_BLOCKS];
-  P* pp[WAVE_BLOCKS];
-  int cnt[WAVE_BLOCKS];
-  bool vec[WAVE_BLOCKS];
-#pragma unroll
-  for (int k = 0; k < WAVE_BLOCKS; ++k) {
-    const int b = b0 + k;
-    cnt[k] = -1;                  // (-1: nothing to do here)
-    if (b < a.blocks) {
-      while (t + 1 < a.count && tab.first[t + 1] <= b) ++t;
-      const G* gp = (const G*)tab.g[t];
-      if (gp) {
-        const int last = (t + 1 < a.count ? tab.first[t + 1] : a.blocks) - 1;
-        const long off = (long)(b - tab.first[t]) * 256 + lane * 4;
-        const int in_block = b < last ? 256 : (int)tab.tail[t];
-        pp[k] = (P*)tab.p[t] + off;
-        cnt[k] = max(0, min(4, in_block - lane * 4));
-        vec[k] = (((uintptr_t)tab.p[t] & (4 * sizeof(P) - 1)) | ((uintptr_t)gp & (4 * sizeof(G) - 1))) == 0;
-        ld_upto4(gp + off, cnt[k], vec[k], g[k]);
-        ld_upto4((const P*)pp[k], cnt[k], vec[k], p[k]);
-        const long at = (a.block0 + b) * 256 + lane * 4;
-        if constexpr (BITS == 8) {
-          mc[k] = *(const uint32_t*)((const uint8_t*)m_ + at);
-          vc[k] = *(const uint32_t*)((const uint8_t*)v_ + at);
-          ms[k] = m_scale[a.block0 + b];
-          vs[k] = v_scale[a.block0 + b];
-        } else {
-          ld4((const float*)m_ + at, m[k]);
-          ld4((const float*)v_ + at, v[k]);
-        }
-      }
+  {
+    const int first = tab.first[t], end = t + 1 < a.count ? tab.first[t + 1] : a.blocks;
+    P* pt = (P*)tab.p[t];
+    const G* gt = (const G*)tab.g[t];
+    if (gt && b0 + WAVE_BLOCKS + (tab.tail[t] < 256) <= end && (((uintptr_t)pt & (N * sizeof(P) - 1) & 15) | ((uintptr_t)gt & (N * sizeof(G) - 1) & 15)) == 0) {
+      const long off = (long)(b0 - first) * 256;
+      four_blocks<P, G, BITS, N>(a, pt + off, gt + off, m_, m_scale, v_, v_scale, a.block0 + b0, lane);
+      return;
     }
   }
-#pragma unroll
-  for (int k = 0; k < WAVE_BLOCKS; ++k) {
-    if (cnt[k] < 0) continue;
-    const long blk = a.block0 + b0 + k, at = blk * 256 + lane * 4;
+  // the ends of tensors, short and unaligned ones: block by block
+  for (int k = 0; k < WAVE_BLOCKS && b0 + k < a.blocks; ++k) {
+    const int b = b0 + k;
+    while (t + 1 < a.count && tab.first[t + 1] <= b) ++t;
+    const G* gp = (const G*)tab.g[t];
+    if (!gp) continue;
+    const int last = (t + 1 < a.count ? tab.first[t + 1] : a.blocks) - 1;
+    const long off = (long)(b - tab.first[t]) * 256 + lane * 4, blk = a.block0 + b, at = blk * 256 + lane * 4;
+    const int cnt = max(0, min(4, (b < last ? 256 : (int)tab.tail[t]) - lane * 4));
+    P* pp = (P*)tab.p[t] + off;
+    const bool vec = (((uintptr_t)tab.p[t] & (4 * sizeof(P) - 1)) | ((uintptr_t)gp & (4 * sizeof(G) - 1))) == 0;
+    float p[4], g[4], m[4], v[4], ms = 0.f, vs = 0.f;
+    int cm[1] = {0}, cr[1] = {0};
+    ld_upto4(gp + off, cnt, vec, g);
+    ld_upto4((const P*)pp, cnt, vec, p);
     if constexpr (BITS == 8) {
-      e4m3_values(mc[k], m[k]);
-      e4m3_values(vc[k], v[k]);
+      e4m3_values(*(const uint32_t*)((const uint8_t*)m_ + at), m);
+      e4m3_values(*(const uint32_t*)((const uint8_t*)v_ + at), v);
+      ms = m_scale[blk];
+      vs = v_scale[blk];
+    } else {
+      ld4((const float*)m_ + at, m);
+      ld4((const float*)v_ + at, v);
     }
-    float r[4], m_top = 0.f, r_top = 0.f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float gr = g[k][e] * a.gscale;
-      if constexpr (BITS == 8) {
-        const float r0 = v[k][e] * vs[k];
-        m[k][e] = m[k][e] * ms[k];
-        v[k][e] = r0 * r0;
-      }
-      m[k][e] = m[k][e] * a.b1 + gr * a.c1;
-      v[k][e] = v[k][e] * a.b2 + (gr * gr) * a.c2;
-      r[e] = sqrtf(v[k][e]);
-      p[k][e] = p[k][e] * a.decay - a.rate * (m[k][e] / (r[e] * a.rbc2 + a.eps));
-      if constexpr (BITS == 8) {
-        m_top = fmaxf(m_top, finite(m[k][e]) ? fabsf(m[k][e]) : 0.f);
-        r_top = fmaxf(r_top, finite(r[e]) ? r[e] : 0.f);
-      }
-    }
-    st_upto4(pp[k], cnt[k], vec[k], p[k]);
+    update<BITS, 4>(a, p, g, m, v, ms, vs, (uint32_t)at, cm, cr);
+    st_upto4(pp, cnt, vec, p);
     if constexpr (BITS == 8) {
-      m_top = fmaxf(wave_max_dpp(m_top), TINY);
-      r_top = fmaxf(wave_max_dpp(r_top), TINY);
-      const float m_inv = (1.f / m_top) * E4M3_MAX, r_inv = (1.f / r_top) * E4M3_MAX;
-      uint32_t cm = 0, cr = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t h = fh_mix32(((uint32_t)at + e) ^ a.key);
-        uint32_t x = e4m3_code(m[k][e], m_inv, (float)(h & 0xffffu) * (1.f / 65536.f));
-        uint32_t y = e4m3_code(r[e], r_inv, (float)(h >> 16) * (1.f / 65536.f));
-        if (r[e] > 0.f && y == 0u) y = 1u;
-        if (!finite(m[k][e])) x = 0x7fu;
-        if (!finite(r[e])) y = 0x7fu;
-        cm |= x << (8 * e);
-        cr |= y << (8 * e);
-      }
-      *(uint32_t*)((uint8_t*)m_ + at) = cm;
-      *(uint32_t*)((uint8_t*)v_ + at) = cr;
+      *(int*)((uint8_t*)m_ + at) = cm[0];
+      *(int*)((uint8_t*)v_ + at) = cr[0];
       if (lane == 0) {
-        m_scale[blk] = m_top * (1.f / E4M3_MAX);
-        v_scale[blk] = r_top * (1.f / E4M3_MAX);
+        m_scale[blk] = ms;
+        v_scale[blk] = vs;
       }
     } else {
-      st4((float*)m_ + at, m[k]);
-      st4((float*)v_ + at, v[k]);
+      st4((float*)m_ + at, m);
+      st4((float*)v_ + at, v);
     }
   }
 }

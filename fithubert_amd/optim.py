@@ -13,7 +13,8 @@ chance with draws that are a function of (seed, place) alone.
 """
 from __future__ import annotations
 
-import ctypes as C
+from array import array
+from operator import attrgetter
 from typing import List, Sequence, Tuple
 
 import torch
@@ -22,6 +23,7 @@ from . import _lib as L
 
 BLOCK = 256   # elements that share one scale; every tensor's moments begin at a multiple of it
 
+_dtype, _device, _contiguous, _numel, _data_ptr = attrgetter("dtype"), torch.Tensor.get_device, torch.Tensor.is_contiguous, torch.Tensor.numel, torch.Tensor.data_ptr
 _DT = {torch.float32: L.DT_F32, torch.bfloat16: L.DT_BF16, torch.float16: L.DT_F16}
 
 
@@ -51,8 +53,8 @@ def adamw_many(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mo
     p = p (1 - lr weight_decay) - lr / (1 - b1^step) m / (sqrt(v) / sqrt(1 - b2^step) + eps); ``step`` counts from 1.
 
     ``params``: contiguous CUDA tensors of one type (fp32, bf16 or fp16) on one device, none twice and none overlapping another (a tensor given
-    twice is refused; an overlap cannot be seen).  ``grads``: one per parameter, of one type, or None: that parameter and its moments are left
-    alone.  ``moments``: as ``adamw_moments`` makes them, updated in place.  Arithmetic is fp32 throughout; a 16-bit parameter is rounded
+    twice is refused; an overlap cannot be seen).  ``grads``: one per parameter, of its size (in the order of its elements) and all of one type, or None: that parameter and its
+    moments are left alone.  ``moments``: as ``adamw_moments`` makes them, updated in place.  Arithmetic is fp32 throughout; a 16-bit parameter is rounded
     to nearest once, so a change below half its spacing is lost.  ``seed`` draws the rounding of 8-bit moments: give each step its own
     (the step's number will do).  Runs on the current stream of the tensors' device; all scalars are part of the launch, so a captured
     call repeats the same ``step`` and ``seed`` on every replay."""
@@ -61,31 +63,31 @@ def adamw_many(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mo
     if not params:
         return
     with torch.no_grad():
-        p0 = params[0]
-        dev, pdt = p0.device, p0.dtype
+        dev, pdt = params[0].device, params[0].dtype
         if pdt not in _DT or dev.type != "cuda":
             raise ValueError(f"parameters are fp32, bf16 or fp16 tensors on the GPU, got {pdt} on {dev}")
-        gdt, held = None, []
-        for p, g in zip(params, grads):
-            if p.dtype != pdt or p.device != dev or not p.is_contiguous():
-                raise ValueError(f"parameters are contiguous, of one type and on one device: got {tuple(p.shape)} {p.dtype} on {p.device} beside {pdt} on {dev}")
-            if g is None:
-                held.append(None)
-                continue
-            if gdt is None:
-                gdt = g.dtype
-            if g.dtype != gdt or g.device != dev or g.shape != p.shape or g.layout != torch.strided:
-                raise ValueError(f"gradients are dense, of one type and of their parameter's shape and device: got {tuple(g.shape)} {g.dtype} on {g.device} for {tuple(p.shape)}")
-            held.append(g if g.is_contiguous() else g.contiguous())
-        if gdt is None:
+        held = [g for g in grads if g is not None]
+        if not held:
             return
+        gdt = held[0].dtype
         if gdt not in _DT:
             raise ValueError(f"gradients are fp32, bf16 or fp16, got {gdt}")
-        sizes = [p.numel() for p in params]
-        at = [p.data_ptr() for p in params]
-        full = [a for a, k in zip(at, sizes) if k]
-        if len(set(full)) != len(full):
+        # (a call's time on the host is these looks at every tensor: each is one pass of a C function over the list)
+        if set(map(_dtype, params)) != {pdt} or set(map(_dtype, held)) != {gdt} or set(map(_device, params)) | set(map(_device, held)) != {dev.index}:
+            raise ValueError(f"parameters are of one type, gradients are of one type, all on one GPU ({pdt}, {gdt}, {dev})")
+        if not all(map(_contiguous, params)):
+            raise ValueError("parameters are contiguous")
+        if len(held) == len(grads) and all(map(_contiguous, held)):
+            held = grads
+        else:
+            held = [g if g is None or g.is_contiguous() else g.contiguous() for g in grads]
+        sizes = list(map(_numel, params))
+        if sizes != (list(map(_numel, held)) if held is grads else [n if g is None else g.numel() for n, g in zip(sizes, held)]):
+            raise ValueError("a gradient has another size than its parameter")
+        at = list(map(_data_ptr, params))
+        if len(set(at)) != len(at) and len({a for a, k in zip(at, sizes) if k}) != len([k for k in sizes if k]):
             raise ValueError("a parameter is given twice")
+        gat = list(map(_data_ptr, held)) if held is grads else [0 if g is None else g.data_ptr() for g in held]
         bits = {2: 32, 4: 8}.get(len(moments))
         nb = moment_blocks(sizes)
         want = [(torch.float32, nb * BLOCK)] * 2 if bits == 32 else [(torch.float8_e4m3fn, nb * BLOCK), (torch.float32, nb)] * 2
@@ -94,11 +96,11 @@ def adamw_many(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mo
         n = len(params)
         mp = [t.data_ptr() for t in moments]
         m, ms, v, vs = (mp[0], None, mp[1], None) if bits == 32 else mp
+        at, gat, sizes = array("Q", at), array("Q", gat), array("q", sizes)
         with torch.cuda.device(dev):
-            L.check(L.lib().fh_adamw_many(_DT[pdt], _DT[gdt], (C.c_void_p * n)(*at), (C.c_void_p * n)(*[g.data_ptr() if g is not None else None for g in held]),
-                                          (C.c_long * n)(*sizes), n, bits, m, ms, v, vs, lr, betas[0], betas[1], eps, weight_decay, step, grad_scale,
-                                          seed & 0xFFFFFFFF, torch.cuda.current_stream(dev).cuda_stream), "fh_adamw_many")
-        torch.autograd.graph.increment_version([p for p, g in zip(params, held) if g is not None])
+            L.check(L.lib().fh_adamw_many(_DT[pdt], _DT[gdt], at.buffer_info()[0], gat.buffer_info()[0], sizes.buffer_info()[0], n, bits, m, ms, v, vs, lr, betas[0],
+                                          betas[1], eps, weight_decay, step, grad_scale, seed & 0xFFFFFFFF, torch.cuda.current_stream(dev).cuda_stream), "fh_adamw_many")
+        torch.autograd.graph.increment_version(params if held is grads else [p for p, g in zip(params, held) if g is not None])
 
 
 class ManyAdamW(torch.optim.Optimizer):
