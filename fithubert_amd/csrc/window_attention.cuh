@@ -8,12 +8,12 @@
 // then staged once for all G heads, the sums of dk / dv over the group happen in registers, and one frame of a stream fills G rows of a
 // tile instead of one.
 //
-// Forward: a workgroup owns 32 rows per wave, walks the 64-key tiles that its rows see (first the sinks' tiles, then the window's) through
+// Forward: a workgroup owns 16 or 32 rows per wave, walks the 64-key tiles that its rows see (first the sinks' tiles, then the window's) through
 // two LDS buffers, and keeps running maximum and sum per row.  Scores are computed transposed (keys x rows): a lane holds ONE row, the
 // reductions are two row exchanges, and the probabilities are the second product's operand without leaving the registers.  A wave
 // skips tiles that none of its rows sees; only tiles on a border of the window pay for the mask.  Few rows against many keys: the tiles
 // are dealt over several workgroups, whose partial sums a second kernel joins.
-// Backward: a pass over the rows for dq (the forward's walk), one over 128-key blocks for dk / dv (its rows are those between the block's
+// Backward: a pass over the rows for dq (the forward's walk), one over 64- or 128-key blocks for dk / dv (its rows are those between the block's
 // window borders).  The blocks that hold sinks see every later row: their rows are dealt over several workgroups and joined.
 // Two passes cost 7 products instead of 5, but no atomics: results repeat bit for bit.
 #pragma once
@@ -29,31 +29,49 @@ template <typename T, int NDT> struct WT {
   static constexpr int TILE = 64 * RS;
   static constexpr int VEC = ElemTraits<T>::VEC;
   typedef typename AT<T>::frag frag;
-  // waves per SIMD that the register budget is cut for: wide heads hold their accumulators in registers alone
-  static constexpr int OCC = NDT >= (sizeof(T) == 4 ? 6 : 9) ? 1 : 2;
-  static constexpr int OCC_DKV = NDT >= (sizeof(T) == 4 ? 4 : 6) ? 1 : 2;
 };
 
 template <typename T, int NDT> __device__ __forceinline__ typename AT<T>::frag wfrag(const unsigned char* lds, int row, int ks, int lane) {
   return *reinterpret_cast<const typename AT<T>::frag*>(lds + row * WT<T, NDT>::RS + ks * 64 + (lane >> 4) * 16);
 }
 
-// acc[dt] += Tile^T[d tile dt][rows 32 m2 .. 32 m2 + 31] * P: P0 / P1 are the accumulator tiles of rows 0..15 / 16..31 of that range
-template <typename T, int NDT>
-__device__ __forceinline__ void wmma_transposed(const unsigned char* tile, int m2, const f32x4& P0, const f32x4& P1, f32x4 (&acc)[NDT], int lane) {
+typedef __attribute__((ext_vector_type(2))) float f32x2;
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+// two floats to two elements of T, to nearest: one instruction
+template <typename T> __device__ __forceinline__ uint32_t pack_pair(float a, float b) {
+  if constexpr (ElemTraits<T>::DT == 2) {
+    union { f16x2 v; uint32_t u; } c;
+    c.v = __builtin_convertvector(f32x2{a, b}, f16x2);
+    return c.u;
+  } else {
+    union { bf16x2 v; uint32_t u; } c;
+    c.v = __builtin_convertvector(f32x2{a, b}, bf16x2);
+    return c.u;
+  }
+}
+
+// acc[t][dt] += Tile^T[d tile dt][rows 32 m2 .. 32 m2 + 31] * P[t]: P0 / P1 are the accumulator tiles of rows 0..15 / 16..31 of that range.
+// 16-bit modes round P (the probabilities, or dS) to the element type here: off by at most 2^-8 (bf16), 2^-11 (fp16) of each.
+template <typename T, int NDT, int RT>
+__device__ __forceinline__ void wmma_transposed(const unsigned char* tile, int m2, const f32x4 (&P0)[RT], const f32x4 (&P1)[RT], f32x4 (&acc)[RT][NDT], int lane) {
   constexpr int RS = WT<T, NDT>::RS;
   const int i = lane & 15, q = lane >> 4;
   if constexpr (sizeof(T) == 2) {
-    union { V16 w; bf16x8 v; } pb;   // the rounding of the probabilities (or dS) to the element type: half a unit in 2^-8 (bf16) / 2^-11 of each
-    pb.w.w[0] = pack2<T>(P0[0], P0[1]); pb.w.w[1] = pack2<T>(P0[2], P0[3]);
-    pb.w.w[2] = pack2<T>(P1[0], P1[1]); pb.w.w[3] = pack2<T>(P1[2], P1[3]);
+    union { V16 w; bf16x8 v; } pb[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      pb[t].w.w[0] = pack_pair<T>(P0[t][0], P0[t][1]); pb[t].w.w[1] = pack_pair<T>(P0[t][2], P0[t][3]);
+      pb[t].w.w[2] = pack_pair<T>(P1[t][0], P1[t][1]); pb[t].w.w[3] = pack_pair<T>(P1[t][2], P1[t][3]);
+    }
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) {
       const unsigned char* a0 = tile + (32 * m2 + 4 * q + (i >> 2)) * RS + (16 * dt + 4 * (i & 3)) * 2;
       union { struct { s16x4 lo, hi; } s; bf16x8 v; } u;
       u.s.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)a0);
       u.s.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a0 + 16 * RS));
-      acc[dt] = mfma16<T>(u.v, pb.v, acc[dt]);
+#pragma unroll
+      for (int t = 0; t < RT; ++t) acc[t][dt] = mfma16<T>(u.v, pb[t].v, acc[t][dt]);
     }
   } else {
 #pragma unroll
@@ -64,7 +82,8 @@ __device__ __forceinline__ void wmma_transposed(const unsigned char* tile, int m
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) {
           const float a = *reinterpret_cast<const float*>(tile + row * RS + (16 * dt + i) * 4);
-          acc[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, half ? P1[e] : P0[e], acc[dt], 0, 0, 0);
+#pragma unroll
+          for (int t = 0; t < RT; ++t) acc[t][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, half ? P1[t][e] : P0[t][e], acc[t][dt], 0, 0, 0);
         }
       }
   }
@@ -144,8 +163,50 @@ __device__ __forceinline__ int tile_sight(const WinArgs& a, int klen, int s0, in
 }
 
 // ------------------------------------------------------------------------------------------------ forward
-template <typename T, int NDT, int NW, bool SPLIT>
-__global__ void __launch_bounds__(NW * 64, (WT<T, NDT>::OCC)) win_fwd_kernel(const WinArgs a, const T* __restrict__ q_, const T* __restrict__ k_, const T* __restrict__ v_,
+// One 64-key tile of the online softmax: s (keys x rows; a lane holds row t's keys 16 kb + 4 q + e) becomes the tile's probabilities up to the rows' running
+// maximum; m, l and the sums o are brought to it.
+template <int RT, bool MASKED, int NDT>
+__device__ __forceinline__ void softmax_step(const WinArgs& a, f32x4 (&s)[4][RT], int s0, int klen, const int (&pos)[RT], float (&m)[RT], float (&l)[RT],
+                                             f32x4 (&o)[RT][NDT], int q) {
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    float mx = -INFINITY;
+    const int hi = min(klen - 1, pos[t] + a.right), lo = pos[t] - a.left;
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (MASKED) {
+          const int key = s0 + 16 * kb + 4 * q + e;
+          if (key > hi || (key < lo && key >= a.sinks)) s[kb][t][e] = -INFINITY;
+        }
+        mx = fmaxf(mx, s[kb][t][e]);
+      }
+    const float mnew = fmaxf(m[t], xor_max(mx) * a.c);                        // c > 0: the maximum commutes with it
+    const float ref = mnew == -INFINITY ? 0.f : mnew;                         // (a row that has seen nothing yet)
+    const float alpha = fast_exp2(m[t] - ref);
+    m[t] = mnew;
+    float rs = 0.f;
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float p = fast_exp2(fmaf(s[kb][t][e], a.c, -ref));
+        rs += p;
+        s[kb][t][e] = p;
+      }
+    l[t] = l[t] * alpha + xor_sum(rs);
+    if (__any(alpha != 1.0f)) {                                               // (a maximum that did not move: times 2^0 in every lane)
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[t][dt][e] *= alpha;
+    }
+  }
+}
+
+template <typename T, int NDT, int RT, bool SPLIT>
+__global__ void __launch_bounds__(256, NDT * RT * (int)sizeof(T) > 32 ? 1 : 2) win_fwd_kernel(const WinArgs a, const T* __restrict__ q_, const T* __restrict__ k_, const T* __restrict__ v_,
                                                           T* __restrict__ out, float* __restrict__ lse, float* __restrict__ part) {
   typedef WT<T, NDT> W;
   constexpr int NK = W::NK;
@@ -155,25 +216,25 @@ __global__ void __launch_bounds__(NW * 64, (WT<T, NDT>::OCC)) win_fwd_kernel(con
   win_block(blk, h, bz);
   const int split = SPLIT ? bz % a.nsplit : 0, b = SPLIT ? bz / a.nsplit : bz;
   const int base = a.q_start ? clip_pos(a.q_start[b]) : 0;
-  const int g0 = blk * 32 * NW, g1 = min(g0 + 32 * NW, a.rows) - 1;            // the workgroup's rows
-  const int w0 = g0 + wave * 32, w1 = min(w0 + 31, a.rows - 1);                // the wave's
-  const TileWalk walk(a, b, base + g0 / a.G, base + g1 / a.G);
-  const int wp0 = base + w0 / a.G, wp1 = base + w1 / a.G;
+  const int g0 = blk * 64 * RT, g1 = min(g0 + 64 * RT, a.rows) - 1;            // the workgroup's rows
+  const int w0 = g0 + wave * 16 * RT, w1 = min(w0 + 16 * RT, a.rows) - 1;                // the wave's
+  const TileWalk walk(a, b, base + a.frame(g0), base + a.frame(g1));
+  const int wp0 = base + a.frame(min(w0, g1)), wp1 = base + a.frame(max(w1, 0));
   const T* qb = q_ + b * a.q_bs;
   const T* kb_ = k_ + b * a.k_bs + h * a.k_hs;
   const T* vb_ = v_ + b * a.v_bs + h * a.v_hs;
   zero_lds<T>(lds, 4 * W::TILE);                                               // (channels past dh are never written again)
-  typename W::frag qf[2][NK];
-  int pos[2];
+  typename W::frag qf[RT][NK];
+  int pos[RT];
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const int row = w0 + 16 * t + r, i = row / a.G, g = row - i * a.G;
+  for (int t = 0; t < RT; ++t) {
+    const int row = w0 + 16 * t + r, i = a.frame(row), g = row - i * a.G;
     pos[t] = base + i;
 #pragma unroll
     for (int ks = 0; ks < NK; ++ks) qf[t][ks] = gfrag<T>(qb + i * a.q_ts + (long)(h * a.G + g) * a.q_hs, row < a.rows, ks, lane, a.dh);
   }
   __syncthreads();
-  Mover<T, NDT, NW * 64> mv;
+  Mover<T, NDT, 256> mv;
   mv.init(a.dh);
   const int per = SPLIT ? (walk.n + a.nsplit - 1) / a.nsplit : walk.n;
   const int kt0 = split * per, kt1 = min(walk.n, kt0 + per);
@@ -185,66 +246,34 @@ __global__ void __launch_bounds__(NW * 64, (WT<T, NDT>::OCC)) win_fwd_kernel(con
       return s < walk.hi && (s >= walk.lo || s < a.sinks);                     // what no row here sees is not read
     });
   };
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  f32x4 o[2][NDT];
+  float m[RT], l[RT];
+  f32x4 o[RT][NDT];
 #pragma unroll
-  for (int t = 0; t < 2; ++t)
+  for (int t = 0; t < RT; ++t) {
+    m[t] = -INFINITY;
+    l[t] = 0.f;
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) o[t][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
 
   auto compute = [&](const unsigned char* Ks, int s0, auto masked_c) {
     constexpr bool MASKED = decltype(masked_c)::value;
     const unsigned char* Vs = Ks + W::TILE;
-    f32x4 s[4][2];
+    f32x4 s[4][RT];
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb) {
-      s[kb][0] = s[kb][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int t = 0; t < RT; ++t) s[kb][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int ks = 0; ks < NK; ++ks) {
         const typename W::frag f = wfrag<T, NDT>(Ks, 16 * kb + r, ks, lane);
-        s[kb][0] = mma<T>(f, qf[0][ks], s[kb][0]);
-        s[kb][1] = mma<T>(f, qf[1][ks], s[kb][1]);
+#pragma unroll
+        for (int t = 0; t < RT; ++t) s[kb][t] = mma<T>(f, qf[t][ks], s[kb][t]);
       }
     }
+    softmax_step<RT, MASKED>(a, s, s0, walk.klen, pos, m, l, o, q);
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      float mx = -INFINITY;
-      const int hi = min(walk.klen - 1, pos[t] + a.right), lo = pos[t] - a.left;
-#pragma unroll
-      for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if constexpr (MASKED) {
-            const int key = s0 + 16 * kb + 4 * q + e;
-            if (key > hi || (key < lo && key >= a.sinks)) s[kb][t][e] = -INFINITY;
-          }
-          mx = fmaxf(mx, s[kb][t][e]);
-        }
-      const float mnew = fmaxf(m[t], xor_max(mx) * a.c);                        // c > 0: the maximum commutes with it
-      const float ref = mnew == -INFINITY ? 0.f : mnew;                         // (a row that has seen nothing yet)
-      const float alpha = fast_exp2(m[t] - ref);
-      m[t] = mnew;
-      float rs = 0.f;
-#pragma unroll
-      for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float p = fast_exp2(fmaf(s[kb][t][e], a.c, -ref));
-          rs += p;
-          s[kb][t][e] = p;
-        }
-      l[t] = l[t] * alpha + xor_sum(rs);
-      if (__any(alpha != 1.0f)) {
-#pragma unroll
-        for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[t][dt][e] *= alpha;
-      }
-    }
-#pragma unroll
-    for (int m2 = 0; m2 < 2; ++m2)
-#pragma unroll
-      for (int t = 0; t < 2; ++t) wmma_transposed<T, NDT>(Vs, m2, s[2 * m2][t], s[2 * m2 + 1][t], o[t], lane);
+    for (int m2 = 0; m2 < 2; ++m2) wmma_transposed<T, NDT, RT>(Vs, m2, s[2 * m2], s[2 * m2 + 1], o, lane);
   };
 
   if (kt0 < kt1) fetch(walk.key0(kt0));
@@ -260,10 +289,10 @@ __global__ void __launch_bounds__(NW * 64, (WT<T, NDT>::OCC)) win_fwd_kernel(con
   }
 
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
+  for (int t = 0; t < RT; ++t) {
     const int row = w0 + 16 * t + r;
     if (row >= a.rows) continue;
-    const int i = row / a.G, g = row - i * a.G;
+    const int i = a.frame(row), g = row - i * a.G;
     if constexpr (SPLIT) {
       // partial sums of this workgroup's keys: [entry][head][split][row][dh + 2] with the maximum and the sum behind the channels
       float* dst = part + ((((long)b * a.Hkv + h) * a.nsplit + split) * a.rows + row) * (a.dh + 2);
@@ -294,12 +323,142 @@ __global__ void __launch_bounds__(NW * 64, (WT<T, NDT>::OCC)) win_fwd_kernel(con
   }
 }
 
-// joins the partial sums of a row: one wave per row, two channels per lane
+// A few rows (at most 16 TT per key head: one new frame's query heads, or some frames') against a cache.  What counts is how many keys are on their way at a
+// time, so the four waves of a workgroup walk tiles of their own, without a barrier: keys go straight from memory into the first product's operand
+// registers, values through a tile of LDS that only this wave uses, and both are requested a tile ahead.  The waves' sums meet at the end.
+template <typename T, int NDT, int TT>
+__global__ void __launch_bounds__(256, NDT * TT * (int)sizeof(T) > 16 ? 1 : 2) win_few_kernel(const WinArgs a, const T* __restrict__ q_, const T* __restrict__ k_,
+                                                                                    const T* __restrict__ v_, T* __restrict__ out, float* __restrict__ lse,
+                                                                                    float* __restrict__ part) {
+  typedef WT<T, NDT> W;
+  constexpr int NK = W::NK, CP = NDT * 16 / W::VEC;    // 16-byte pieces of a row = per lane and tile
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+  const int split = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+  const int base = a.q_start ? clip_pos(a.q_start[b]) : 0;
+  const int wp0 = base, wp1 = base + a.Tq - 1;
+  const TileWalk walk(a, b, wp0, wp1);
+  const T* qb = q_ + b * a.q_bs;
+  const T* kb_ = k_ + b * a.k_bs + h * a.k_hs;
+  const T* vb_ = v_ + b * a.v_bs + h * a.v_hs;
+  unsigned char* tile = lds + wave * W::TILE;
+  typename W::frag qf[TT][NK], kf[4][NK];
+  V16 vf[CP];
+  int pos[TT];
+#pragma unroll
+  for (int t = 0; t < TT; ++t) {
+    const int row = 16 * t + r, i = a.frame(row), g = row - i * a.G;
+    pos[t] = base + i;
+#pragma unroll
+    for (int ks = 0; ks < NK; ++ks) qf[t][ks] = gfrag<T>(qb + i * a.q_ts + (long)(h * a.G + g) * a.q_hs, row < a.rows, ks, lane, a.dh);
+  }
+  const int per = (walk.n + a.nsplit - 1) / a.nsplit, kt1 = min(walk.n, (split + 1) * per);
+  auto fetch = [&](int s0) {
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb) {
+      const int s = s0 + 16 * kb + r;
+      const bool live = s < walk.hi && (s >= walk.lo || s < a.sinks);
+#pragma unroll
+      for (int ks = 0; ks < NK; ++ks) kf[kb][ks] = gfrag<T>(kb_ + s * a.k_ts, live, ks, lane, a.dh);
+    }
+#pragma unroll
+    for (int j = 0; j < CP; ++j) {
+      const int at = j * 64 + lane, row = at / CP, col = (at % CP) * W::VEC, s = s0 + row;
+      vf[j] = v16_zero();
+      if (s < walk.hi && (s >= walk.lo || s < a.sinks) && col < a.dh) vf[j] = ld16(vb_ + s * a.v_ts + col);
+    }
+  };
+  float m[TT], l[TT];
+  f32x4 o[TT][NDT];
+#pragma unroll
+  for (int t = 0; t < TT; ++t) {
+    m[t] = -INFINITY;
+    l[t] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) o[t][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  int kt = split * per + wave;
+  if (kt < kt1) fetch(walk.key0(kt));
+  for (; kt < kt1; kt += 4) {
+    const int s0 = walk.key0(kt);
+    f32x4 s[4][TT];
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        s[kb][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < NK; ++ks) s[kb][t] = mma<T>(kf[kb][ks], qf[t][ks], s[kb][t]);
+      }
+#pragma unroll
+    for (int j = 0; j < CP; ++j) {
+      const int at = j * 64 + lane;
+      st16(tile + (at / CP) * W::RS + (at % CP) * 16, vf[j]);
+    }
+    if (kt + 4 < kt1) fetch(walk.key0(kt + 4));
+    if (tile_sight(a, walk.klen, s0, wp0, wp1) == 2) softmax_step<TT, false>(a, s, s0, walk.klen, pos, m, l, o, q);
+    else softmax_step<TT, true>(a, s, s0, walk.klen, pos, m, l, o, q);
+    // (a wave reads only what it wrote itself, and the LDS serves one wave's accesses in order: only the compiler has to be held back)
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int m2 = 0; m2 < 2; ++m2) wmma_transposed<T, NDT, TT>(tile, m2, s[2 * m2], s[2 * m2 + 1], o, lane);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+  // the four waves' sums: [wave][row][NDT * 16] over the tiles, the maxima and sums behind them
+  constexpr int D = NDT * 16;
+  __syncthreads();
+  float* sums = reinterpret_cast<float*>(lds);
+  float* ml = sums + 4 * 16 * TT * D;
+#pragma unroll
+  for (int t = 0; t < TT; ++t) {
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) *reinterpret_cast<f32x4*>(sums + ((wave * TT + t) * 16 + r) * D + 16 * dt + 4 * q) = o[t][dt];
+    if (q == 0) {
+      ml[((wave * TT + t) * 16 + r) * 2] = m[t];
+      ml[((wave * TT + t) * 16 + r) * 2 + 1] = l[t];
+    }
+  }
+  __syncthreads();
+  for (int n = threadIdx.x; n < a.rows * (D / 4); n += 256) {
+    const int row = n / (D / 4), d = (n - row * (D / 4)) * 4;
+    float top = -INFINITY, w[4], sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) top = fmaxf(top, ml[(k * 16 * TT + row) * 2]);
+    const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      w[k] = fast_exp2(ml[(k * 16 * TT + row) * 2] - ref);
+      sum += w[k] * ml[(k * 16 * TT + row) * 2 + 1];
+      const f32x4 x = *reinterpret_cast<const f32x4*>(sums + (k * 16 * TT + row) * D + d);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += w[k] * x[e];
+    }
+    if (d >= a.dh) continue;
+    if (a.nsplit > 1) {
+      float* dst = part + ((((long)b * a.Hkv + h) * a.nsplit + split) * a.rows + row) * (a.dh + 2);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dst[d + e] = v[e];
+      if (d == 0) { dst[a.dh] = top; dst[a.dh + 1] = sum; }
+    } else {
+      const float inv = sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);
+      const int i = a.frame(row), g = row - i * a.G;
+      const long orow = ((long)b * a.Tq + i) * a.Hq + h * a.G + g;
+      if (d == 0 && lse) lse[orow] = sum == 0.f ? INFINITY : top + log2f(sum);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] *= inv;
+      st4(out + orow * a.dh + d, v);
+    }
+  }
+}
+
+// joins the partial sums of a row: a workgroup per row, its four waves take every fourth share, a lane two channels
 template <typename T>
 __global__ void __launch_bounds__(256) win_join_kernel(const WinArgs a, const float* __restrict__ part, T* __restrict__ out, float* __restrict__ lse) {
-  const int lane = threadIdx.x & 63;
-  const long n = (long)blockIdx.x * 4 + (threadIdx.x >> 6);     // row of [entry][head][row]
-  if (n >= (long)a.B * a.Hkv * a.rows) return;
+  __shared__ float acc[4][132];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long n = blockIdx.x;                                     // row of [entry][head][row]
   const int row = (int)(n % a.rows);
   const long bh = n / a.rows;
   const int h = (int)(bh % a.Hkv), b = (int)(bh / a.Hkv), W = a.dh + 2;
@@ -309,26 +468,32 @@ __global__ void __launch_bounds__(256) win_join_kernel(const WinArgs a, const fl
   for (int s = lane; s < a.nsplit; s += 64) m = fmaxf(m, src[s * step + a.dh]);
   m = wave_max(m);
   const float ref = m == -INFINITY ? 0.f : m;
+  const int c = min(2 * lane, a.dh - 2);
   float l = 0.f, o0 = 0.f, o1 = 0.f;
-  for (int s = 0; s < a.nsplit; ++s) {
+#pragma unroll 4
+  for (int s = wave; s < a.nsplit; s += 4) {
     const float* p = src + s * step;
     const float w = fast_exp2(p[a.dh] - ref);
     l += w * p[a.dh + 1];
-    if (2 * lane < a.dh) { o0 += w * p[2 * lane]; o1 += w * p[2 * lane + 1]; }
+    o0 += w * p[c];
+    o1 += w * p[c + 1];
   }
-  const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
-  const int i = row / a.G, g = row - i * a.G;
+  acc[wave][2 * lane] = o0;
+  acc[wave][2 * lane + 1] = o1;
+  if (lane == 0) acc[wave][128] = l;
+  __syncthreads();
+  const int i = a.frame(row), g = row - i * a.G;
   const long orow = ((long)b * a.Tq + i) * a.Hq + h * a.G + g;
-  if (lane == 0 && lse) lse[orow] = l == 0.f ? INFINITY : m + log2f(l);
-  if (2 * lane < a.dh) {
-    out[orow * a.dh + 2 * lane] = from_f<T>(o0 * inv);
-    out[orow * a.dh + 2 * lane + 1] = from_f<T>(o1 * inv);
-  }
+  l = acc[0][128] + acc[1][128] + acc[2][128] + acc[3][128];
+  const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
+  if (threadIdx.x == 0 && lse) lse[orow] = l == 0.f ? INFINITY : m + log2f(l);
+  const int d = threadIdx.x;
+  if (d < a.dh) out[orow * a.dh + d] = from_f<T>((acc[0][d] + acc[1][d] + acc[2][d] + acc[3][d]) * inv);
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dq, and D for the other pass
-template <typename T, int NDT, int NW>
-__global__ void __launch_bounds__(NW * 64, (WT<T, NDT>::OCC)) win_dq_kernel(const WinArgs a, const T* __restrict__ q_, const T* __restrict__ k_, const T* __restrict__ v_,
+template <typename T, int NDT, int RT>
+__global__ void __launch_bounds__(256, 2) win_dq_kernel(const WinArgs a, const T* __restrict__ q_, const T* __restrict__ k_, const T* __restrict__ v_,
                                                          const T* __restrict__ out, const T* __restrict__ dout, const float* __restrict__ lse,
                                                          float* __restrict__ delta, T* __restrict__ dq) {
   typedef WT<T, NDT> W;
@@ -338,20 +503,20 @@ __global__ void __launch_bounds__(NW * 64, (WT<T, NDT>::OCC)) win_dq_kernel(cons
   int blk, h, b;
   win_block(blk, h, b);
   const int base = a.q_start ? clip_pos(a.q_start[b]) : 0;
-  const int g0 = blk * 32 * NW, g1 = min(g0 + 32 * NW, a.rows) - 1;
-  const int w0 = g0 + wave * 32, w1 = min(w0 + 31, a.rows - 1);
-  const TileWalk walk(a, b, base + g0 / a.G, base + g1 / a.G);
-  const int wp0 = base + w0 / a.G, wp1 = base + w1 / a.G;
+  const int g0 = blk * 64 * RT, g1 = min(g0 + 64 * RT, a.rows) - 1;
+  const int w0 = g0 + wave * 16 * RT, w1 = min(w0 + 16 * RT, a.rows) - 1;
+  const TileWalk walk(a, b, base + a.frame(g0), base + a.frame(g1));
+  const int wp0 = base + a.frame(min(w0, g1)), wp1 = base + a.frame(max(w1, 0));
   const T* qb = q_ + b * a.q_bs;
   const T* kb_ = k_ + b * a.k_bs + h * a.k_hs;
   const T* vb_ = v_ + b * a.v_bs + h * a.v_hs;
   zero_lds<T>(lds, 4 * W::TILE);
-  typename W::frag qf[2][NK], gf[2][NK];
-  int pos[2];
-  float ls[2], dl[2];
+  typename W::frag qf[RT][NK], gf[RT][NK];
+  int pos[RT];
+  float ls[RT], dl[RT];
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const int row = w0 + 16 * t + r, i = row / a.G, g = row - i * a.G;
+  for (int t = 0; t < RT; ++t) {
+    const int row = w0 + 16 * t + r, i = a.frame(row), g = row - i * a.G;
     const bool live = row < a.rows;
     const long orow = ((long)b * a.Tq + i) * a.Hq + h * a.G + g;
     pos[t] = base + i;
@@ -375,7 +540,7 @@ __global__ void __launch_bounds__(NW * 64, (WT<T, NDT>::OCC)) win_dq_kernel(cons
     if (live && q == 0) delta[orow] = dl[t];
   }
   __syncthreads();
-  Mover<T, NDT, NW * 64> mv;
+  Mover<T, NDT, 256> mv;
   mv.init(a.dh);
   auto fetch = [&](int s0) {
     mv.fetch([&](int row, const T*& x, const T*& y) {
@@ -385,9 +550,9 @@ __global__ void __launch_bounds__(NW * 64, (WT<T, NDT>::OCC)) win_dq_kernel(cons
       return s < walk.hi && (s >= walk.lo || s < a.sinks);                     // what no row here sees is not read
     });
   };
-  f32x4 acc[2][NDT];
+  f32x4 acc[RT][NDT];
 #pragma unroll
-  for (int t = 0; t < 2; ++t)
+  for (int t = 0; t < RT; ++t)
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) acc[t][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   auto compute = [&](const unsigned char* Ks, int s0, auto masked_c) {
@@ -395,22 +560,27 @@ __global__ void __launch_bounds__(NW * 64, (WT<T, NDT>::OCC)) win_dq_kernel(cons
     const unsigned char* Vs = Ks + W::TILE;
 #pragma unroll
     for (int m2 = 0; m2 < 2; ++m2) {
-      f32x4 s[2][2], dp[2][2];
+      f32x4 s[2][RT];
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
         const int kb = 2 * m2 + kk;
-        s[kk][0] = s[kk][1] = dp[kk][0] = dp[kk][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+        f32x4 dp[RT];
 #pragma unroll
-        for (int ks = 0; ks < NK; ++ks) {
-          const typename W::frag f = wfrag<T, NDT>(Ks, 16 * kb + r, ks, lane);
-          s[kk][0] = mma<T>(f, qf[0][ks], s[kk][0]);
-          s[kk][1] = mma<T>(f, qf[1][ks], s[kk][1]);
-          const typename W::frag fv = wfrag<T, NDT>(Vs, 16 * kb + r, ks, lane);
-          dp[kk][0] = mma<T>(fv, gf[0][ks], dp[kk][0]);
-          dp[kk][1] = mma<T>(fv, gf[1][ks], dp[kk][1]);
+        for (int t = 0; t < RT; ++t) {
+          s[kk][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+          dp[t] = f32x4{-dl[t], -dl[t], -dl[t], -dl[t]};   // dP - D out of the product itself
         }
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int ks = 0; ks < NK; ++ks) {
+          const typename W::frag f = wfrag<T, NDT>(Ks, 16 * kb + r, ks, lane), fv = wfrag<T, NDT>(Vs, 16 * kb + r, ks, lane);
+#pragma unroll
+          for (int t = 0; t < RT; ++t) {
+            s[kk][t] = mma<T>(f, qf[t][ks], s[kk][t]);
+            dp[t] = mma<T>(fv, gf[t][ks], dp[t]);
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
           const int hi = min(walk.klen - 1, pos[t] + a.right), lo = pos[t] - a.left;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -419,12 +589,11 @@ __global__ void __launch_bounds__(NW * 64, (WT<T, NDT>::OCC)) win_dq_kernel(cons
               const int key = s0 + 16 * kb + 4 * q + e;
               if (key > hi || (key < lo && key >= a.sinks)) p = 0.f;
             }
-            s[kk][t][e] = p * a.scale * (dp[kk][t][e] - dl[t]);
+            s[kk][t][e] = p * dp[t][e];                     // dS / scale
           }
         }
       }
-#pragma unroll
-      for (int t = 0; t < 2; ++t) wmma_transposed<T, NDT>(Ks, m2, s[0][t], s[1][t], acc[t], lane);
+      wmma_transposed<T, NDT, RT>(Ks, m2, s[0], s[1], acc, lane);
     }
   };
   if (walk.n > 0) fetch(walk.key0(0));
@@ -438,10 +607,10 @@ __global__ void __launch_bounds__(NW * 64, (WT<T, NDT>::OCC)) win_dq_kernel(cons
     else if (sight == 1) compute(Ks, s0, std::true_type{});
   }
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
+  for (int t = 0; t < RT; ++t) {
     const int row = w0 + 16 * t + r;
     if (row >= a.rows) continue;
-    const int i = row / a.G, g = row - i * a.G;
+    const int i = a.frame(row), g = row - i * a.G;
     const long orow = ((long)b * a.Tq + i) * a.Hq + h * a.G + g;
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) {
@@ -449,7 +618,7 @@ __global__ void __launch_bounds__(NW * 64, (WT<T, NDT>::OCC)) win_dq_kernel(cons
       if (d < a.dh) {
         float w[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = acc[t][dt][e];
+        for (int e = 0; e < 4; ++e) w[e] = acc[t][dt][e] * a.scale;
         st4(dq + orow * a.dh + d, w);
       }
     }
@@ -457,10 +626,10 @@ __global__ void __launch_bounds__(NW * 64, (WT<T, NDT>::OCC)) win_dq_kernel(cons
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dk, dv
-// A workgroup owns 128 keys (32 per wave) of one key head and walks the 64-row tiles that see them.  grid.x: nsink * nsplit workgroups for the
+// A workgroup owns 64 KT keys (16 KT per wave) of one key head and walks the 64-row tiles that see them.  grid.x: nsink * nsplit workgroups for the
 // blocks that hold sinks (partial sums), then one per remaining block.
-template <typename T, int NDT>
-__global__ void __launch_bounds__(256, (WT<T, NDT>::OCC_DKV)) win_dkv_kernel(const WinArgs a, const T* __restrict__ q_, const T* __restrict__ k_, const T* __restrict__ v_,
+template <typename T, int NDT, int KT>
+__global__ void __launch_bounds__(256, NDT * (int)sizeof(T) > 24 ? 1 : 2) win_dkv_kernel(const WinArgs a, const T* __restrict__ q_, const T* __restrict__ k_, const T* __restrict__ v_,
                                                       const T* __restrict__ dout, const float* __restrict__ lse, const float* __restrict__ delta,
                                                       T* __restrict__ dk, T* __restrict__ dv, float* __restrict__ part) {
   typedef WT<T, NDT> W;
@@ -474,13 +643,13 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC_DKV)) win_dkv_kernel(con
   const int kb = shared ? x / a.nsplit : x - a.nsink * a.nsplit + a.nsink, split = shared ? x % a.nsplit : 0;
   const int base = a.q_start ? clip_pos(a.q_start[b]) : 0;
   const int klen = a.key_len ? max(0, min(a.key_len[b], a.Tk)) : a.Tk;
-  const int s0 = kb * 128, k0 = s0 + wave * 32;                   // first key of the workgroup, of the wave
+  const int s0 = kb * 64 * KT, k0 = s0 + wave * 16 * KT;                   // first key of the workgroup, of the wave
   const T* qb = q_ + b * a.q_bs;
   zero_lds<T>(lds, 4 * W::TILE);
-  typename W::frag kf[2][NK], vf[2][NK];
-  int plo[2], phi[2];                                             // positions that see this lane's keys
+  typename W::frag kf[KT][NK], vf[KT][NK];
+  int plo[KT], phi[KT];                                             // positions that see this lane's keys
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
+  for (int t = 0; t < KT; ++t) {
     const int s = k0 + 16 * t + r;
     plo[t] = s - a.right;
     phi[t] = s >= klen ? -2 * FAR : s < a.sinks ? 2 * FAR : s + a.left;
@@ -491,7 +660,7 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC_DKV)) win_dkv_kernel(con
     }
   }
   // rows that see a key of this block: frames [f0, f1), then the workgroup's share of their 64-row tiles
-  const int last = min(s0 + 127, klen - 1);
+  const int last = min(s0 + 64 * KT, klen) - 1;
   const int f0 = max(0, min(a.Tq, s0 - a.right - base));
   const int f1 = last < s0 ? f0 : s0 < a.sinks ? a.Tq : max(f0, min(a.Tq, last + a.left - base + 1));
   const int row0 = f0 * a.G, row1 = f1 * a.G;
@@ -504,21 +673,21 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC_DKV)) win_dkv_kernel(con
   auto fetch = [&](int rt) {
     const int first = row0 + rt * 64;
     mv.fetch([&](int n, const T*& x, const T*& y) {
-      const int row = first + n, i = row / a.G, g = row - i * a.G;
+      const int row = first + n, i = a.frame(row), g = row - i * a.G;
       x = qb + i * a.q_ts + (long)(h * a.G + g) * a.q_hs;
       y = dout + (((long)b * a.Tq + i) * a.Hq + h * a.G + g) * a.dh;
       return row < row1;
     });
     if (threadIdx.x < 64) {
-      const int row = first + (int)threadIdx.x, i = row / a.G, g = row - i * a.G;
+      const int row = first + (int)threadIdx.x, i = a.frame(row), g = row - i * a.G;
       const long orow = ((long)b * a.Tq + i) * a.Hq + h * a.G + g;
       pre_l = row < row1 ? lse[orow] : INFINITY;                  // +inf: the row's probabilities are 0
       pre_d = row < row1 ? delta[orow] : 0.f;
     }
   };
-  f32x4 ak[2][NDT], av[2][NDT];
+  f32x4 ak[KT][NDT], av[KT][NDT];
 #pragma unroll
-  for (int t = 0; t < 2; ++t)
+  for (int t = 0; t < KT; ++t)
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) ak[t][dt] = av[t][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   auto compute = [&](const unsigned char* Qs, const float* rd, auto masked_c) {
@@ -526,25 +695,29 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC_DKV)) win_dkv_kernel(con
     const unsigned char* Gs = Qs + W::TILE;
 #pragma unroll
     for (int m2 = 0; m2 < 2; ++m2) {
-      f32x4 p[2][2], ds[2][2];
+      f32x4 p[2][KT], ds[2][KT];
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
         const int rb = 2 * m2 + kk;
-        p[kk][0] = p[kk][1] = ds[kk][0] = ds[kk][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int ks = 0; ks < NK; ++ks) {
-          const typename W::frag f = wfrag<T, NDT>(Qs, 16 * rb + r, ks, lane);
-          p[kk][0] = mma<T>(f, kf[0][ks], p[kk][0]);
-          p[kk][1] = mma<T>(f, kf[1][ks], p[kk][1]);
-          const typename W::frag fg = wfrag<T, NDT>(Gs, 16 * rb + r, ks, lane);
-          ds[kk][0] = mma<T>(fg, vf[0][ks], ds[kk][0]);
-          ds[kk][1] = mma<T>(fg, vf[1][ks], ds[kk][1]);
-        }
         const f32x4 l4 = *reinterpret_cast<const f32x4*>(rd + 16 * rb + 4 * q);
         const f32x4 d4 = *reinterpret_cast<const f32x4*>(rd + 64 + 16 * rb + 4 * q);
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+          p[kk][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+          ds[kk][t] = d4;                                  // -D: dP - D out of the product itself
+        }
+#pragma unroll
+        for (int ks = 0; ks < NK; ++ks) {
+          const typename W::frag f = wfrag<T, NDT>(Qs, 16 * rb + r, ks, lane), fg = wfrag<T, NDT>(Gs, 16 * rb + r, ks, lane);
+#pragma unroll
+          for (int t = 0; t < KT; ++t) {
+            p[kk][t] = mma<T>(f, kf[t][ks], p[kk][t]);
+            ds[kk][t] = mma<T>(fg, vf[t][ks], ds[kk][t]);
+          }
+        }
         const int* p4 = reinterpret_cast<const int*>(rd + 128 + 16 * rb + 4 * q);
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < KT; ++t)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             float w = fast_exp2(fmaf(p[kk][t][e], a.c, -l4[e]));
@@ -553,14 +726,11 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC_DKV)) win_dkv_kernel(con
               if (at < plo[t] || at > phi[t]) w = 0.f;
             }
             p[kk][t][e] = w;
-            ds[kk][t][e] = w * a.scale * (ds[kk][t][e] - d4[e]);
+            ds[kk][t][e] *= w;                             // dS / scale
           }
       }
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        wmma_transposed<T, NDT>(Gs, m2, p[0][t], p[1][t], av[t], lane);
-        wmma_transposed<T, NDT>(Qs, m2, ds[0][t], ds[1][t], ak[t], lane);
-      }
+      wmma_transposed<T, NDT, KT>(Gs, m2, p[0], p[1], av, lane);
+      wmma_transposed<T, NDT, KT>(Qs, m2, ds[0], ds[1], ak, lane);
     }
   };
   if (t0 < t1) fetch(t0);
@@ -570,19 +740,19 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC_DKV)) win_dkv_kernel(con
     mv.deposit(Qs);
     if (threadIdx.x < 64) {
       rd[threadIdx.x] = pre_l;
-      rd[64 + threadIdx.x] = pre_d;
-      reinterpret_cast<int*>(rd)[128 + threadIdx.x] = base + (row0 + rt * 64 + (int)threadIdx.x) / a.G;
+      rd[64 + threadIdx.x] = -pre_d;
+      reinterpret_cast<int*>(rd)[128 + threadIdx.x] = base + a.frame(row0 + rt * 64 + (int)threadIdx.x);
     }
     __syncthreads();
     if (rt + 1 < t1) fetch(rt + 1);
     // positions of the tile's rows against those that see the wave's keys
-    const int p0 = base + (row0 + rt * 64) / a.G, p1 = base + min(row0 + rt * 64 + 63, row1 - 1) / a.G, ke = min(k0 + 31, klen - 1);
+    const int p0 = base + a.frame(row0 + rt * 64), p1 = base + a.frame(min(row0 + rt * 64 + 63, row1 - 1)), ke = min(k0 + 16 * KT, klen) - 1;
     if (ke < k0 || p1 < k0 - a.right || (p0 > ke + a.left && k0 >= a.sinks)) continue;
-    if (k0 + 31 < klen && p0 >= k0 + 31 - a.right && (p1 <= k0 + a.left || k0 + 31 < a.sinks)) compute(Qs, rd, std::false_type{});
+    if (k0 + 16 * KT - 1 < klen && p0 >= k0 + 16 * KT - 1 - a.right && (p1 <= k0 + a.left || k0 + 16 * KT - 1 < a.sinks)) compute(Qs, rd, std::false_type{});
     else compute(Qs, rd, std::true_type{});
   }
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
+  for (int t = 0; t < KT; ++t) {
     const int s = k0 + 16 * t + r;
     if (s >= a.Tk) continue;
 #pragma unroll
@@ -591,12 +761,12 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC_DKV)) win_dkv_kernel(con
       if (d >= a.dh) continue;
       float wk[4], wv[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) { wk[e] = ak[t][dt][e]; wv[e] = av[t][dt][e]; }
+      for (int e = 0; e < 4; ++e) { wk[e] = ak[t][dt][e] * a.scale; wv[e] = av[t][dt][e]; }
       if (shared) {
-        // [entry][head][sink block][split][dk | dv][128][dh]
-        float* dst = part + (((((long)b * a.Hkv + h) * a.nsink + kb) * a.nsplit + split) * 2 * 128 + (s - s0)) * a.dh + d;
+        // [entry][head][sink block][split][dk | dv][keys][dh]
+        float* dst = part + (((((long)b * a.Hkv + h) * a.nsink + kb) * a.nsplit + split) * 2 * 64 * KT + (s - s0)) * a.dh + d;
         st4(dst, wk);
-        st4(dst + 128 * a.dh, wv);
+        st4(dst + 64 * KT * a.dh, wv);
       } else {
         const long at = (((long)b * a.Tk + s) * a.Hkv + h) * a.dh + d;
         st4(dk + at, wk);
@@ -608,24 +778,24 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC_DKV)) win_dkv_kernel(con
 
 // sums the partial dk / dv of the sink blocks, in the order of the splits; a thread owns four channels of one key
 template <typename T>
-__global__ void __launch_bounds__(256) win_dkv_join_kernel(const WinArgs a, const float* __restrict__ part, T* __restrict__ dk, T* __restrict__ dv) {
+__global__ void __launch_bounds__(256) win_dkv_join_kernel(const WinArgs a, const float* __restrict__ part, T* __restrict__ dk, T* __restrict__ dv, int keys) {
   const int c4 = a.dh / 4;
-  const long n = (long)blockIdx.x * 256 + threadIdx.x, total = (long)a.B * a.Hkv * a.nsink * 2 * 128 * c4;
+  const long n = (long)blockIdx.x * 256 + threadIdx.x, total = (long)a.B * a.Hkv * a.nsink * 2 * keys * c4;
   if (n >= total) return;
   const int c = (int)(n % c4);
   long k = n / c4;
-  const int key = (int)(k % 128);
-  k /= 128;
+  const int key = (int)(k % keys);
+  k /= keys;
   const int which = (int)(k % 2);
   k /= 2;
-  const int kb = (int)(k % a.nsink), s = kb * 128 + key;
+  const int kb = (int)(k % a.nsink), s = kb * keys + key;
   k /= a.nsink;
   const int h = (int)(k % a.Hkv), b = (int)(k / a.Hkv);
   if (s >= a.Tk) return;
-  const float* src = part + (((((long)b * a.Hkv + h) * a.nsink + kb) * a.nsplit * 2 + which) * 128 + key) * a.dh + c * 4;
+  const float* src = part + (((((long)b * a.Hkv + h) * a.nsink + kb) * a.nsplit * 2 + which) * keys + key) * a.dh + c * 4;
   float sum[4] = {0.f, 0.f, 0.f, 0.f}, f[4];
   for (int i = 0; i < a.nsplit; ++i) {
-    ld4(src + (long)i * 2 * 128 * a.dh, f);
+    ld4(src + (long)i * 2 * keys * a.dh, f);
 #pragma unroll
     for (int e = 0; e < 4; ++e) sum[e] += f[e];
   }
@@ -638,47 +808,88 @@ template <typename K> int set_lds(K kernel, size_t bytes) {
   return (int)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
 }
 
-template <typename T, int NDT, int NW, bool SPLIT>
+template <typename T, int NDT, int RT, bool SPLIT>
 int run_fwd(const WinArgs& a, const void* q, const void* k, const void* v, void* out, float* lse, float* part, hipStream_t st) {
   const size_t smem = 4 * WT<T, NDT>::TILE;
-  if (int rc = set_lds(win_fwd_kernel<T, NDT, NW, SPLIT>, smem)) return rc;
-  const dim3 grid((a.rows + 32 * NW - 1) / (32 * NW), a.Hkv, a.B * a.nsplit), block(NW * 64);
-  hipLaunchKernelGGL((win_fwd_kernel<T, NDT, NW, SPLIT>), grid, block, smem, st, a, (const T*)q, (const T*)k, (const T*)v, (T*)out, lse, part);
+  if (int rc = set_lds(win_fwd_kernel<T, NDT, RT, SPLIT>, smem)) return rc;
+  const dim3 grid((a.rows + 64 * RT - 1) / (64 * RT), a.Hkv, a.B * a.nsplit), block(256);
+  hipLaunchKernelGGL((win_fwd_kernel<T, NDT, RT, SPLIT>), grid, block, smem, st, a, (const T*)q, (const T*)k, (const T*)v, (T*)out, lse, part);
   FH_CHECK_LAUNCH();
-  if (SPLIT) {
-    const long rows = (long)a.B * a.Hkv * a.rows;
-    hipLaunchKernelGGL((win_join_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, part, (T*)out, lse);
-    FH_CHECK_LAUNCH();
-  }
+  return 0;
+}
+template <typename T, int NDT, int TT>
+int run_few(const WinArgs& a, const void* q, const void* k, const void* v, void* out, float* lse, float* part, hipStream_t st) {
+  const size_t ends = 4 * 16 * TT * (NDT * 16 + 2) * 4, tiles = 4 * WT<T, NDT>::TILE, smem = ends > tiles ? ends : tiles;
+  if (int rc = set_lds(win_few_kernel<T, NDT, TT>, smem)) return rc;
+  hipLaunchKernelGGL((win_few_kernel<T, NDT, TT>), dim3(a.nsplit, a.Hkv, a.B), dim3(256), smem, st, a, (const T*)q, (const T*)k, (const T*)v, (T*)out, lse, part);
+  FH_CHECK_LAUNCH();
   return 0;
 }
 template <typename T, int NDT>
 int fwd_t(WinArgs a, const void* q, const void* k, const void* v, void* out, float* lse, float* part, hipStream_t st) {
-  a.nsplit = fwd_splits(a);
-  return a.nsplit > 1 ? run_fwd<T, NDT, 4, true>(a, q, k, v, out, lse, part, st) : run_fwd<T, NDT, 4, false>(a, q, k, v, out, lse, part, st);
+  const WinPlan p = fwd_plan(a, ElemTraits<T>::DT);
+  a.nsplit = p.nsplit;
+  int rc;
+  if (p.few) {
+    if constexpr (sizeof(T) == 2 || NDT <= 4) rc = a.rows <= 16 ? run_few<T, NDT, 1>(a, q, k, v, out, lse, part, st) : run_few<T, NDT, 2>(a, q, k, v, out, lse, part, st);
+    else rc = run_few<T, NDT, 1>(a, q, k, v, out, lse, part, st);
+  }
+  else if (p.nsplit > 1) rc = p.rt == 2 ? run_fwd<T, NDT, 2, true>(a, q, k, v, out, lse, part, st) : run_fwd<T, NDT, 1, true>(a, q, k, v, out, lse, part, st);
+  else rc = p.rt == 2 ? run_fwd<T, NDT, 2, false>(a, q, k, v, out, lse, part, st) : run_fwd<T, NDT, 1, false>(a, q, k, v, out, lse, part, st);
+  if (rc || p.nsplit == 1) return rc;
+  hipLaunchKernelGGL((win_join_kernel<T>), dim3((unsigned)((long)a.B * a.Hkv * a.rows)), dim3(256), 0, st, a, part, (T*)out, lse);
+  FH_CHECK_LAUNCH();
+  return 0;
+}
+template <typename T, int NDT, int RT>
+int run_dq(const WinArgs& a, const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse, float* delta, void* dq, hipStream_t st) {
+  const size_t smem = 4 * WT<T, NDT>::TILE;
+  if (int rc = set_lds(win_dq_kernel<T, NDT, RT>, smem)) return rc;
+  hipLaunchKernelGGL((win_dq_kernel<T, NDT, RT>), dim3((a.rows + 64 * RT - 1) / (64 * RT), a.Hkv, a.B), dim3(256), smem, st, a, (const T*)q, (const T*)k, (const T*)v,
+                     (const T*)out, (const T*)dout, lse, delta, (T*)dq);
+  FH_CHECK_LAUNCH();
+  return 0;
+}
+template <typename T, int NDT, int KT>
+int run_dkv(const WinArgs& a, const void* q, const void* k, const void* v, const void* dout, const float* lse, const float* delta, void* dk, void* dv, float* part,
+            hipStream_t st) {
+  const size_t smem = 4 * WT<T, NDT>::TILE + 2 * 192 * 4;
+  if (int rc = set_lds(win_dkv_kernel<T, NDT, KT>, smem)) return rc;
+  const int nkb = (a.Tk + 64 * KT - 1) / (64 * KT);
+  hipLaunchKernelGGL((win_dkv_kernel<T, NDT, KT>), dim3(a.nsink * a.nsplit + nkb - a.nsink, a.Hkv, a.B), dim3(256), smem, st, a, (const T*)q, (const T*)k, (const T*)v,
+                     (const T*)dout, lse, delta, (T*)dk, (T*)dv, part);
+  FH_CHECK_LAUNCH();
+  return 0;
 }
 template <typename T, int NDT>
 int bwd_t(WinArgs a, const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse, void* dq, void* dk, void* dv,
           char* scratch, hipStream_t st) {
+  constexpr int DT = ElemTraits<T>::DT;
   float* delta = (float*)scratch;
   float* part = (float*)(scratch + al16((size_t)a.B * a.Tq * a.Hq * 4));
-  const size_t smem = 4 * WT<T, NDT>::TILE, smem2 = smem + 2 * 192 * 4;
-  if (int rc = set_lds(win_dq_kernel<T, NDT, 4>, smem)) return rc;
-  if (int rc = set_lds(win_dkv_kernel<T, NDT>, smem2)) return rc;
   if (a.rows > 0) {
-    hipLaunchKernelGGL((win_dq_kernel<T, NDT, 4>), dim3((a.rows + 127) / 128, a.Hkv, a.B), dim3(256), smem, st, a, (const T*)q, (const T*)k, (const T*)v,
-                       (const T*)out, (const T*)dout, lse, delta, (T*)dq);
-    FH_CHECK_LAUNCH();
+    int rc;
+    if constexpr (NDT <= (DT == 0 ? 4 : 6)) {
+      rc = bwd_tiles(a, DT, (long)a.B * a.Hkv * ((a.rows + 127) / 128), false) == 2 ? run_dq<T, NDT, 2>(a, q, k, v, out, dout, lse, delta, dq, st)
+                                                                                     : run_dq<T, NDT, 1>(a, q, k, v, out, dout, lse, delta, dq, st);
+    } else {
+      rc = run_dq<T, NDT, 1>(a, q, k, v, out, dout, lse, delta, dq, st);
+    }
+    if (rc) return rc;
   }
   if (a.Tk > 0) {
-    bwd_sinks(a);
-    const int nkb = (a.Tk + 127) / 128;
-    hipLaunchKernelGGL((win_dkv_kernel<T, NDT>), dim3(a.nsink * a.nsplit + nkb - a.nsink, a.Hkv, a.B), dim3(256), smem2, st, a, (const T*)q, (const T*)k,
-                       (const T*)v, (const T*)dout, lse, delta, (T*)dk, (T*)dv, part);
-    FH_CHECK_LAUNCH();
+    const int keys = dkv_keys(a, DT);
+    bwd_sinks(a, keys);
+    int rc;
+    if constexpr (NDT <= (DT == 0 ? 3 : 4)) {
+      rc = keys == 128 ? run_dkv<T, NDT, 2>(a, q, k, v, dout, lse, delta, dk, dv, part, st) : run_dkv<T, NDT, 1>(a, q, k, v, dout, lse, delta, dk, dv, part, st);
+    } else {
+      rc = run_dkv<T, NDT, 1>(a, q, k, v, dout, lse, delta, dk, dv, part, st);
+    }
+    if (rc) return rc;
     if (a.nsink > 0) {
-      const long n = (long)a.B * a.Hkv * a.nsink * 2 * 128 * (a.dh / 4);
-      hipLaunchKernelGGL((win_dkv_join_kernel<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a, part, (T*)dk, (T*)dv);
+      const long n = (long)a.B * a.Hkv * a.nsink * 2 * keys * (a.dh / 4);
+      hipLaunchKernelGGL((win_dkv_join_kernel<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a, part, (T*)dk, (T*)dv, keys);
       FH_CHECK_LAUNCH();
     }
   }

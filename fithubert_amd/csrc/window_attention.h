@@ -11,25 +11,47 @@ struct WinArgs {
   const int* q_start;
   long q_bs, q_ts, q_hs, k_bs, k_ts, k_hs, v_bs, v_ts, v_hs;
   int rows;                        // Tq * G
+  unsigned magic;                  // floor(2^32 / G) + 1 (G = 1: 0)
   int nsplit;                      // forward: workgroups that share a row block's keys; dk / dv: that share a sink block's rows
   int nsink;                       // dk / dv: key blocks that hold sinks
+  // frame of a row (row < 2^29: the product is at most one too large)
+  __device__ __forceinline__ int frame(int row) const {
+    if (magic == 0u) return row;
+    const int f = (int)__umulhi((unsigned)row, magic);
+    return f * G > row ? f - 1 : f;
+  }
 };
 
-// Workgroups per row block: enough for every CU to hold a few, where the rows alone do not make them; at least two tiles of keys each.
-static inline int fwd_splits(const WinArgs& a) {
-  const long wgs = (long)a.B * a.Hkv * ((a.rows + 127) / 128), want = 768;
+// How a forward call is laid out.  few: at most 32 rows per key head (win_few_kernel); otherwise rt 16-row tiles per wave, four waves; nsplit workgroups
+// share each row block's keys.
+struct WinPlan { int few, rt, nsplit; };
+static inline WinPlan fwd_plan(const WinArgs& a, int dtype) {
+  WinPlan p;
+  const long heads = (long)a.B * a.Hkv, blocks2 = heads * ((a.rows + 127) / 128), blocks1 = heads * ((a.rows + 63) / 64);
   const long span = (long)a.left + a.right + 128 / a.G + 1;
-  const long tiles = ((span < a.Tk ? span : a.Tk) + 63) / 64 + (a.sinks + 63) / 64;
-  long n = want / (wgs > 0 ? wgs : 1);
-  if (n > tiles / 2) n = tiles / 2;
-  return n < 2 ? 1 : n > 256 ? 256 : (int)n;
+  const long tiles = ((span < a.Tk ? span : a.Tk) + 63) / 64 + (a.sinks + 63) / 64;   // 64-key tiles that a row block sees
+  p.few = a.rows <= (dtype == 0 && a.dh > 64 ? 16 : 32);   // (wide fp32 heads of 32 rows outgrow its registers)
+  // 128-row blocks halve the reads of K and V; 64-row ones where those would leave CUs without work and the walk is short
+  p.rt = !p.few && blocks2 < 512 && tiles < 16 ? 1 : 2;
+  const long wgs = p.few ? heads : p.rt == 2 ? blocks2 : blocks1;
+  // one workgroup per CU at least; a share is worth its join from eight tiles on (a wave's tiles of the few-row kernel: two)
+  long n = wgs >= 256 ? 1 : (a.dh > 64 && !p.few ? 256 : 512) / (wgs > 0 ? wgs : 1);
+  if (n > tiles / 8) n = tiles / 8;
+  p.nsplit = n < 2 ? 1 : n > 256 ? 256 : (int)n;
+  return p;
 }
-// sink blocks and the workgroups that share each one's rows
-static inline void bwd_sinks(WinArgs& a) {
-  a.nsink = (a.sinks + 127) / 128;
+// sink blocks (of `keys` keys) and the workgroups that share each one's rows
+static inline void bwd_sinks(WinArgs& a, int keys) {
+  a.nsink = (a.sinks + keys - 1) / keys;
   long n = (a.rows + 1023) / 1024;
   a.nsplit = n < 1 ? 1 : n > 64 ? 64 : (int)n;
 }
+// 16-key (16-row) tiles per wave of the backward passes: two where that still gives every CU two workgroups, and where the accumulators fit
+static inline int bwd_tiles(const WinArgs& a, int dtype, long blocks128, bool dkv) {
+  const int widest = dkv ? (dtype == 0 ? 48 : 64) : (dtype == 0 ? 64 : 96);
+  return a.dh <= widest && blocks128 >= 512 ? 2 : 1;
+}
+static inline int dkv_keys(const WinArgs& a, int dtype) { return 64 * bwd_tiles(a, dtype, (long)a.B * a.Hkv * ((a.Tk + 127) / 128), true); }
 static inline size_t al16(size_t n) { return (n + 15) & ~(size_t)15; }
 
 #define WIN_DECLARE(name)                                                                                                                     \

@@ -26,6 +26,7 @@ WinArgs args_of(const fh_window_attention_desc* d) {
   a.k_bs = d->k_bs; a.k_ts = d->k_ts; a.k_hs = d->k_hs;
   a.v_bs = d->v_bs; a.v_ts = d->v_ts; a.v_hs = d->v_hs;
   a.rows = d->Tq * a.G;
+  a.magic = a.G == 1 ? 0u : (unsigned)(0x100000000ull / (unsigned)a.G) + 1u;
   a.nsplit = 1;
   a.nsink = 0;
   return a;
@@ -39,11 +40,12 @@ long fh_window_attention_scratch_bytes(int dtype, const fh_window_attention_desc
   if (check(dtype, d)) return -1;
   WinArgs a = args_of(d);
   if (!backward) {
-    const int n = fwd_splits(a);
+    const int n = fwd_plan(a, dtype).nsplit;
     return n > 1 ? (long)a.B * a.Hkv * n * a.rows * (a.dh + 2) * 4 : 0;
   }
-  bwd_sinks(a);
-  return (long)al16((size_t)a.B * a.Tq * a.Hq * 4) + (a.nsink ? (long)a.B * a.Hkv * a.nsink * a.nsplit * 2 * 128 * a.dh * 4 : 0);
+  const int keys = dkv_keys(a, dtype);
+  bwd_sinks(a, keys);
+  return (long)al16((size_t)a.B * a.Tq * a.Hq * 4) + (long)a.B * a.Hkv * a.nsink * a.nsplit * 2 * keys * a.dh * 4;
 }
 
 int fh_window_attention_forward(int dtype, const fh_window_attention_desc* d, const void* q, const void* k, const void* v, void* out,

@@ -34,20 +34,15 @@ def _per_entry(x, B: int, dev: torch.device, name: str) -> Optional[torch.Tensor
         return torch.full((B,), int(x), dtype=torch.int32, device=dev)
     if x.dim() != 1 or x.shape[0] != B or x.dtype.is_floating_point or x.dtype == torch.bool:
         raise ValueError(f"{name}: one integer per entry ({B}), got {tuple(x.shape)} {x.dtype}")
-    return x.to(device=dev, dtype=torch.int32).contiguous()
+    return x if x.dtype == torch.int32 and x.device == dev and x.is_contiguous() else x.to(device=dev, dtype=torch.int32).contiguous()
 
 
 def _desc(q, k, v, left, right, sinks, scale, key_len, q_start) -> L.WindowAttentionC:
-    d = L.WindowAttentionC()
-    d.B, d.Tq, d.Hq, d.dh = q.shape
-    d.Tk, d.Hkv = k.shape[1], k.shape[2]
-    d.left, d.right, d.sinks, d.scale = left, right, sinks, scale
-    d.key_len = key_len.data_ptr() if key_len is not None else None
-    d.q_start = q_start.data_ptr() if q_start is not None else None
-    for n, t in (("q", q), ("k", k), ("v", v)):
-        for axis, i in (("_bs", 0), ("_ts", 1), ("_hs", 2)):
-            setattr(d, n + axis, t.stride(i) if t.shape[i] > 1 else 0)   # (an axis of length 1 is never stepped along)
-    return d
+    (B, Tq, Hq, dh), (_, Tk, Hkv, _) = q.shape, k.shape
+    sq, sk, sv = q.stride(), k.stride(), v.stride()
+    many = (B > 1, Tq > 1, Hq > 1), (B > 1, Tk > 1, Hkv > 1)   # (an axis of length 1 is never stepped along: its stride may be anything)
+    return L.WindowAttentionC(B, Tq, Tk, Hq, Hkv, dh, left, right, sinks, scale, _ptr(key_len), _ptr(q_start), sq[0] * many[0][0], sq[1] * many[0][1],
+                              sq[2] * many[0][2], sk[0] * many[1][0], sk[1] * many[1][1], sk[2] * many[1][2], sv[0] * many[1][0], sv[1] * many[1][1], sv[2] * many[1][2])
 
 
 def _scratch(dt, d, backward, dev):
@@ -61,10 +56,8 @@ def _ptr(t):
     return t.data_ptr() if t is not None else None
 
 
-def _forward(q, k, v, conf, want_lse):
-    left, right, sinks, scale, key_len, q_start = conf
+def _forward(q, k, v, d, want_lse):
     dt, dev = _DT[q.dtype], q.device
-    d = _desc(q, k, v, left, right, sinks, scale, key_len, q_start)
     out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev) if want_lse else None
     with torch.cuda.device(dev):
@@ -76,19 +69,17 @@ def _forward(q, k, v, conf, want_lse):
 
 class _WindowAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, conf):
-        out, lse = _forward(q, k, v, conf, True)
-        ctx.save_for_backward(q, k, v, out, lse)
-        ctx.conf = conf
+    def forward(ctx, q, k, v, key_len, q_start, d):
+        out, lse = _forward(q, k, v, d, True)
+        ctx.save_for_backward(q, k, v, out, lse, key_len, q_start)   # (d holds addresses: what they belong to lives as long)
+        ctx.d = d
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse = ctx.saved_tensors
-        left, right, sinks, scale, key_len, q_start = ctx.conf
-        dt, dev = _DT[q.dtype], q.device
-        d = _desc(q, k, v, left, right, sinks, scale, key_len, q_start)
+        q, k, v, out, lse, _, _ = ctx.saved_tensors
+        dt, dev, d = _DT[q.dtype], q.device, ctx.d
         dout = dout.contiguous()
         if dout.data_ptr() % 16:
             dout = dout.clone()
@@ -98,7 +89,7 @@ class _WindowAttention(torch.autograd.Function):
             L.check(L.lib().fh_window_attention_backward(dt, C.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(), lse.data_ptr(),
                                                          dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(scratch), torch.cuda.current_stream(dev).cuda_stream),
                     "fh_window_attention_backward")
-        return dq, dk, dv, None
+        return dq, dk, dv, None, None, None
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, left: int = -1, right: int = -1, sinks: int = 0,
@@ -131,8 +122,9 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, left:
     if not 0 < scale < float("inf"):
         raise ValueError(f"scale {scale}")
     far = (1 << 31) - 1
-    conf = (min(int(left), far), min(int(right), far), max(0, min(int(sinks), far)), scale, _per_entry(key_len, B, q.device, "key_len"), _per_entry(q_start, B, q.device, "q_start"))
-    conf = tuple(max(x, -1) if i < 2 else x for i, x in enumerate(conf))
+    q, k, v = _aligned(q), _aligned(k), _aligned(v)
+    key_len, q_start = _per_entry(key_len, B, q.device, "key_len"), _per_entry(q_start, B, q.device, "q_start")
+    d = _desc(q, k, v, max(-1, min(int(left), far)), max(-1, min(int(right), far)), max(0, min(int(sinks), far)), scale, key_len, q_start)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _WindowAttention.apply(_aligned(q), _aligned(k), _aligned(v), conf)
-    return _forward(_aligned(q), _aligned(k), _aligned(v), conf, False)[0]
+        return _WindowAttention.apply(q, k, v, key_len, q_start, d)
+    return _forward(q, k, v, d, False)[0]
