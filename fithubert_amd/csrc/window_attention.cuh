@@ -51,29 +51,54 @@ template <typename T> __device__ __forceinline__ uint32_t pack_pair(float a, flo
   }
 }
 
-// acc[t][dt] += Tile^T[d tile dt][rows 32 m2 .. 32 m2 + 31] * P[t]: P0 / P1 are the accumulator tiles of rows 0..15 / 16..31 of that range.
-// 16-bit modes round P (the probabilities, or dS) to the element type here: off by at most 2^-8 (bf16), 2^-11 (fp16) of each.
-template <typename T, int NDT, int RT>
-__device__ __forceinline__ void wmma_transposed(const unsigned char* tile, int m2, const f32x4 (&P0)[RT], const f32x4 (&P1)[RT], f32x4 (&acc)[RT][NDT], int lane) {
+// The second products' operand, a 16-row accumulator tile at a time.  16-bit modes round the probabilities (or dS) to the element type here: off by at most
+// 2^-8 (bf16), 2^-11 (fp16) of each; they are packed as soon as they exist, which halves the registers that wait for the other half.
+template <typename T> struct Half2 {
+  typedef uint2 type;
+  static __device__ __forceinline__ uint2 pack(const f32x4& p) { return make_uint2(pack_pair<T>(p[0], p[1]), pack_pair<T>(p[2], p[3])); }
+};
+template <> struct Half2<float> {
+  typedef f32x4 type;
+  static __device__ __forceinline__ f32x4 pack(const f32x4& p) { return p; }
+};
+
+// The columns of rows 32 m2 .. 32 m2 + 31 of an LDS tile as first operands (one per 16 channels): transposing reads (16-bit).
+template <typename T, int NDT> __device__ __forceinline__ void tile_columns(const unsigned char* tile, int m2, bf16x8 (&col)[NDT], int lane) {
   constexpr int RS = WT<T, NDT>::RS;
   const int i = lane & 15, q = lane >> 4;
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) {
+    const unsigned char* a0 = tile + (32 * m2 + 4 * q + (i >> 2)) * RS + (16 * dt + 4 * (i & 3)) * 2;
+    union { struct { s16x4 lo, hi; } s; bf16x8 v; } u;
+    u.s.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)a0);
+    u.s.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a0 + 16 * RS));
+    col[dt] = u.v;
+  }
+}
+// acc[t][dt] += Tile^T[d tile dt][rows 32 m2 .. 32 m2 + 31] * P[t]: P0 / P1 are the packed accumulator tiles of rows 0..15 / 16..31 of that range
+template <typename T, int NDT, int RT>
+__device__ __forceinline__ void mma_columns(const bf16x8 (&col)[NDT], const uint2 (&P0)[RT], const uint2 (&P1)[RT], f32x4 (&acc)[RT][NDT]) {
+  union { struct { uint2 lo, hi; } w; bf16x8 v; } pb[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    pb[t].w.lo = P0[t];
+    pb[t].w.hi = P1[t];
+  }
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+    for (int t = 0; t < RT; ++t) acc[t][dt] = mfma16<T>(col[dt], pb[t].v, acc[t][dt]);
+}
+template <typename T, int NDT, int RT>
+__device__ __forceinline__ void wmma_transposed(const unsigned char* tile, int m2, const typename Half2<T>::type (&P0)[RT], const typename Half2<T>::type (&P1)[RT],
+                                                f32x4 (&acc)[RT][NDT], int lane) {
   if constexpr (sizeof(T) == 2) {
-    union { V16 w; bf16x8 v; } pb[RT];
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      pb[t].w.w[0] = pack_pair<T>(P0[t][0], P0[t][1]); pb[t].w.w[1] = pack_pair<T>(P0[t][2], P0[t][3]);
-      pb[t].w.w[2] = pack_pair<T>(P1[t][0], P1[t][1]); pb[t].w.w[3] = pack_pair<T>(P1[t][2], P1[t][3]);
-    }
-#pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) {
-      const unsigned char* a0 = tile + (32 * m2 + 4 * q + (i >> 2)) * RS + (16 * dt + 4 * (i & 3)) * 2;
-      union { struct { s16x4 lo, hi; } s; bf16x8 v; } u;
-      u.s.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)a0);
-      u.s.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a0 + 16 * RS));
-#pragma unroll
-      for (int t = 0; t < RT; ++t) acc[t][dt] = mfma16<T>(u.v, pb[t].v, acc[t][dt]);
-    }
+    bf16x8 col[NDT];
+    tile_columns<T, NDT>(tile, m2, col, lane);
+    mma_columns<T, NDT, RT>(col, P0, P1, acc);
   } else {
+    constexpr int RS = WT<T, NDT>::RS;
+    const int i = lane & 15, q = lane >> 4;
 #pragma unroll
     for (int half = 0; half < 2; ++half)
 #pragma unroll
@@ -89,22 +114,48 @@ __device__ __forceinline__ void wmma_transposed(const unsigned char* tile, int m
   }
 }
 
+// Waits for a fragment's loads here: left to its first use inside a loop, the wait would count the loop's own loads in flight as well (the counter is in
+// order, and on the way into the loop there are none behind it) -- every tile would wait for the next one's.
+template <typename F> __device__ __forceinline__ void landed(F& f) { asm volatile("" : "+v"(f)); }
+
 // 64 rows of two tensors (K and V, or q and dout) on their way from memory to an LDS tile pair: fetch() requests them into registers, deposit()
-// stores them -- a tile later, so that the latency lies under the tile in between.  A thread owns one 16-byte column of every RP-th row.
+// stores them -- a tile later, so that the latency lies under the tile in between.  A thread owns one 16-byte column of every RP-th row; where
+// its rows lie from the tile's first one is the same for every tile (x_of, y_of: 32-bit byte offsets), so a whole tile costs a load per
+// piece and no address arithmetic.
 template <typename T, int NDT, int NT> struct Mover {
   static constexpr int VEC = WT<T, NDT>::VEC;
   static constexpr int CP = NDT * 16 / VEC;        // columns at the widest head
   static constexpr int RP = NT / CP;               // rows per pass
   static constexpr int NP = (64 + RP - 1) / RP;    // passes
   V16 pre[2][NP];
+  unsigned x_of[NP], y_of[NP];
   int row, col, dst;
   bool live;
-  __device__ __forceinline__ void init(int dh) {
+  // off(row, x, y): element offsets of a row from the tile's first row
+  template <typename F> __device__ __forceinline__ void init(int dh, F&& off) {
     row = (int)threadIdx.x / CP;
     const int c = (int)threadIdx.x - row * CP;
     col = c * VEC;
     live = row < RP && col < dh;
     dst = row * WT<T, NDT>::RS + c * 16;
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+      unsigned x, y;
+      off(min(row + j * RP, 63), x, y);
+      x_of[j] = (x + col) * sizeof(T);
+      y_of[j] = (y + col) * sizeof(T);
+    }
+  }
+  // the whole tile whose first rows are x, y
+  __device__ __forceinline__ void fetch_whole(const T* x, const T* y) {
+    if (live) {
+#pragma unroll
+      for (int j = 0; j < NP; ++j)
+        if (64 % RP == 0 || j < NP - 1 || row + j * RP < 64) {
+          pre[0][j] = ld16((const char*)x + x_of[j]);
+          pre[1][j] = ld16((const char*)y + y_of[j]);
+        }
+    }
   }
   // at(row, first, second): the addresses of a row's channels in the two tensors; false: zeros
   template <typename F> __device__ __forceinline__ void fetch(F&& at) {
@@ -119,12 +170,14 @@ template <typename T, int NDT, int NT> struct Mover {
     }
   }
   __device__ __forceinline__ void deposit(unsigned char* pair) const {
+    if (live) {
 #pragma unroll
-    for (int j = 0; j < NP; ++j)
-      if (live && row + j * RP < 64) {
-        st16(pair + dst + j * RP * WT<T, NDT>::RS, pre[0][j]);
-        st16(pair + WT<T, NDT>::TILE + dst + j * RP * WT<T, NDT>::RS, pre[1][j]);
-      }
+      for (int j = 0; j < NP; ++j)
+        if (64 % RP == 0 || j < NP - 1 || row + j * RP < 64) {
+          st16(pair + dst + j * RP * WT<T, NDT>::RS, pre[0][j]);
+          st16(pair + WT<T, NDT>::TILE + dst + j * RP * WT<T, NDT>::RS, pre[1][j]);
+        }
+    }
   }
 };
 
@@ -163,45 +216,66 @@ __device__ __forceinline__ int tile_sight(const WinArgs& a, int klen, int s0, in
 }
 
 // ------------------------------------------------------------------------------------------------ forward
+// Which of a tile's 64 keys (or rows) a lane's row (key) meets, as one bit each: [lo, hi) and [0, first).  The lane keeps those at 4 q + e of every 16.
+struct Meets {
+  unsigned w[2];
+  Meets() = default;
+  static __device__ __forceinline__ unsigned long long below(int n) { return n >= 64 ? ~0ull : (1ull << max(n, 0)) - 1ull; }
+  __device__ __forceinline__ Meets(int lo, int hi, int first, int q) {
+    const unsigned long long m = (below(hi) & ~below(lo)) | below(first);
+    w[0] = (unsigned)m >> (4 * q);
+    w[1] = (unsigned)(m >> 32) >> (4 * q);
+  }
+  __device__ __forceinline__ int bits(int n16, int e) const { return __builtin_amdgcn_sbfe((int)w[n16 >> 1], 16 * (n16 & 1) + e, 1); }   // 0 or -1
+  __device__ __forceinline__ float or_less(float x, int n16, int e) const {                                                             // x, or -inf
+    const unsigned m = (unsigned)bits(n16, e);
+    return __uint_as_float((__float_as_uint(x) & m) | (0xff800000u & ~m));
+  }
+  __device__ __forceinline__ float or_zero(float x, int n16, int e) const { return __uint_as_float(__float_as_uint(x) & (unsigned)bits(n16, e)); }
+};
+
 // One 64-key tile of the online softmax: s (keys x rows; a lane holds row t's keys 16 kb + 4 q + e) becomes the tile's probabilities up to the rows' running
-// maximum; m, l and the sums o are brought to it.
-template <int RT, bool MASKED, int NDT>
-__device__ __forceinline__ void softmax_step(const WinArgs& a, f32x4 (&s)[4][RT], int s0, int klen, const int (&pos)[RT], float (&m)[RT], float (&l)[RT],
+// maximum, packed in ph; m, l and the sums o are brought to it.
+template <typename T, int RT, bool MASKED, int NDT>
+__device__ __forceinline__ void softmax_step(const WinArgs& a, f32x4 (&s)[4][RT], typename Half2<T>::type (&ph)[4][RT], int s0, int klen, const int (&pos)[RT], float (&m)[RT], float (&l)[RT],
                                              f32x4 (&o)[RT][NDT], int q) {
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
     float mx = -INFINITY;
-    const int hi = min(klen - 1, pos[t] + a.right), lo = pos[t] - a.left;
+    const int hi = min(klen, pos[t] + a.right + 1) - s0;
+    const Meets meets(MASKED ? pos[t] - a.left - s0 : 0, hi, MASKED ? min(a.sinks - s0, hi) : 0, q);
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if constexpr (MASKED) {
-          const int key = s0 + 16 * kb + 4 * q + e;
-          if (key > hi || (key < lo && key >= a.sinks)) s[kb][t][e] = -INFINITY;
-        }
+        if constexpr (MASKED) s[kb][t][e] = meets.or_less(s[kb][t][e], kb, e);
         mx = fmaxf(mx, s[kb][t][e]);
       }
-    const float mnew = fmaxf(m[t], xor_max(mx) * a.c);                        // c > 0: the maximum commutes with it
-    const float ref = mnew == -INFINITY ? 0.f : mnew;                         // (a row that has seen nothing yet)
-    const float alpha = fast_exp2(m[t] - ref);
-    m[t] = mnew;
+    // The reference that the exponents are taken against is moved only when a row's maximum has outgrown it by 2^8: P then stays below 256, which
+    // costs no precision, and most tiles leave the sums as they are (moved at every new maximum, 60 % of a long window's tiles rescaled them).
+    mx = xor_max(mx) * a.c;                                                   // c > 0: the maximum commutes with it
+    if (__any(mx > m[t] + 8.f)) {
+      const float mnew = fmaxf(m[t], mx), alpha = fast_exp2(m[t] - (mnew == -INFINITY ? 0.f : mnew));
+      m[t] = mnew;
+      l[t] *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[t][dt][e] *= alpha;
+    }
+    const float ref = m[t] == -INFINITY ? 0.f : m[t];                         // (a row that has seen nothing yet)
     float rs = 0.f;
 #pragma unroll
-    for (int kb = 0; kb < 4; ++kb)
+    for (int kb = 0; kb < 4; ++kb) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float p = fast_exp2(fmaf(s[kb][t][e], a.c, -ref));
         rs += p;
         s[kb][t][e] = p;
       }
-    l[t] = l[t] * alpha + xor_sum(rs);
-    if (__any(alpha != 1.0f)) {                                               // (a maximum that did not move: times 2^0 in every lane)
-#pragma unroll
-      for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[t][dt][e] *= alpha;
+      ph[kb][t] = Half2<T>::pack(s[kb][t]);
     }
+    l[t] += xor_sum(rs);
   }
 }
 
@@ -234,11 +308,16 @@ __global__ void __launch_bounds__(256, NDT * RT * (int)sizeof(T) > 32 ? 1 : 2) w
     for (int ks = 0; ks < NK; ++ks) qf[t][ks] = gfrag<T>(qb + i * a.q_ts + (long)(h * a.G + g) * a.q_hs, row < a.rows, ks, lane, a.dh);
   }
   __syncthreads();
+#pragma unroll
+  for (int t = 0; t < RT; ++t)
+#pragma unroll
+    for (int ks = 0; ks < NK; ++ks) landed(qf[t][ks]);
   Mover<T, NDT, 256> mv;
-  mv.init(a.dh);
+  mv.init(a.dh, [&](int row, unsigned& x, unsigned& y) { x = row * (unsigned)a.k_ts; y = row * (unsigned)a.v_ts; });
   const int per = SPLIT ? (walk.n + a.nsplit - 1) / a.nsplit : walk.n;
   const int kt0 = split * per, kt1 = min(walk.n, kt0 + per);
   auto fetch = [&](int s0) {
+    if (s0 + 64 <= walk.hi && (s0 >= walk.lo || s0 + 64 <= a.sinks)) return mv.fetch_whole(kb_ + s0 * a.k_ts, vb_ + s0 * a.v_ts);
     mv.fetch([&](int row, const T*& x, const T*& y) {
       const int s = s0 + row;
       x = kb_ + s * a.k_ts;
@@ -271,9 +350,10 @@ __global__ void __launch_bounds__(256, NDT * RT * (int)sizeof(T) > 32 ? 1 : 2) w
         for (int t = 0; t < RT; ++t) s[kb][t] = mma<T>(f, qf[t][ks], s[kb][t]);
       }
     }
-    softmax_step<RT, MASKED>(a, s, s0, walk.klen, pos, m, l, o, q);
+    typename Half2<T>::type ph[4][RT];
+    softmax_step<T, RT, MASKED>(a, s, ph, s0, walk.klen, pos, m, l, o, q);
 #pragma unroll
-    for (int m2 = 0; m2 < 2; ++m2) wmma_transposed<T, NDT, RT>(Vs, m2, s[2 * m2], s[2 * m2 + 1], o, lane);
+    for (int m2 = 0; m2 < 2; ++m2) wmma_transposed<T, NDT, RT>(Vs, m2, ph[2 * m2], ph[2 * m2 + 1], o, lane);
   };
 
   if (kt0 < kt1) fetch(walk.key0(kt0));
@@ -352,6 +432,10 @@ __global__ void __launch_bounds__(256, NDT * TT * (int)sizeof(T) > 16 ? 1 : 2) w
 #pragma unroll
     for (int ks = 0; ks < NK; ++ks) qf[t][ks] = gfrag<T>(qb + i * a.q_ts + (long)(h * a.G + g) * a.q_hs, row < a.rows, ks, lane, a.dh);
   }
+#pragma unroll
+  for (int t = 0; t < TT; ++t)
+#pragma unroll
+    for (int ks = 0; ks < NK; ++ks) landed(qf[t][ks]);
   const int per = (walk.n + a.nsplit - 1) / a.nsplit, kt1 = min(walk.n, (split + 1) * per);
   auto fetch = [&](int s0) {
 #pragma unroll
@@ -396,13 +480,14 @@ __global__ void __launch_bounds__(256, NDT * TT * (int)sizeof(T) > 16 ? 1 : 2) w
       st16(tile + (at / CP) * W::RS + (at % CP) * 16, vf[j]);
     }
     if (kt + 4 < kt1) fetch(walk.key0(kt + 4));
-    if (tile_sight(a, walk.klen, s0, wp0, wp1) == 2) softmax_step<TT, false>(a, s, s0, walk.klen, pos, m, l, o, q);
-    else softmax_step<TT, true>(a, s, s0, walk.klen, pos, m, l, o, q);
+    typename Half2<T>::type ph[4][TT];
+    if (tile_sight(a, walk.klen, s0, wp0, wp1) == 2) softmax_step<T, TT, false>(a, s, ph, s0, walk.klen, pos, m, l, o, q);
+    else softmax_step<T, TT, true>(a, s, ph, s0, walk.klen, pos, m, l, o, q);
     // (a wave reads only what it wrote itself, and the LDS serves one wave's accesses in order: only the compiler has to be held back)
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int m2 = 0; m2 < 2; ++m2) wmma_transposed<T, NDT, TT>(tile, m2, s[2 * m2], s[2 * m2 + 1], o, lane);
+    for (int m2 = 0; m2 < 2; ++m2) wmma_transposed<T, NDT, TT>(tile, m2, ph[2 * m2], ph[2 * m2 + 1], o, lane);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
   }
@@ -540,9 +625,19 @@ __global__ void __launch_bounds__(256, 2) win_dq_kernel(const WinArgs a, const T
     if (live && q == 0) delta[orow] = dl[t];
   }
   __syncthreads();
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    landed(ls[t]);
+#pragma unroll
+    for (int ks = 0; ks < NK; ++ks) {
+      landed(qf[t][ks]);
+      landed(gf[t][ks]);
+    }
+  }
   Mover<T, NDT, 256> mv;
-  mv.init(a.dh);
+  mv.init(a.dh, [&](int row, unsigned& x, unsigned& y) { x = row * (unsigned)a.k_ts; y = row * (unsigned)a.v_ts; });
   auto fetch = [&](int s0) {
+    if (s0 + 64 <= walk.hi && (s0 >= walk.lo || s0 + 64 <= a.sinks)) return mv.fetch_whole(kb_ + s0 * a.k_ts, vb_ + s0 * a.v_ts);
     mv.fetch([&](int row, const T*& x, const T*& y) {
       const int s = s0 + row;
       x = kb_ + s * a.k_ts;
@@ -558,16 +653,23 @@ __global__ void __launch_bounds__(256, 2) win_dq_kernel(const WinArgs a, const T
   auto compute = [&](const unsigned char* Ks, int s0, auto masked_c) {
     constexpr bool MASKED = decltype(masked_c)::value;
     const unsigned char* Vs = Ks + W::TILE;
+    Meets meets[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+      if constexpr (MASKED) {
+        const int hi = min(walk.klen, pos[t] + a.right + 1) - s0;
+        meets[t] = Meets(pos[t] - a.left - s0, hi, min(a.sinks - s0, hi), q);
+      }
 #pragma unroll
     for (int m2 = 0; m2 < 2; ++m2) {
-      f32x4 s[2][RT];
+      typename Half2<T>::type dsh[2][RT];
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
         const int kb = 2 * m2 + kk;
-        f32x4 dp[RT];
+        f32x4 s[RT], dp[RT];
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-          s[kk][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+          s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
           dp[t] = f32x4{-dl[t], -dl[t], -dl[t], -dl[t]};   // dP - D out of the product itself
         }
 #pragma unroll
@@ -575,25 +677,22 @@ __global__ void __launch_bounds__(256, 2) win_dq_kernel(const WinArgs a, const T
           const typename W::frag f = wfrag<T, NDT>(Ks, 16 * kb + r, ks, lane), fv = wfrag<T, NDT>(Vs, 16 * kb + r, ks, lane);
 #pragma unroll
           for (int t = 0; t < RT; ++t) {
-            s[kk][t] = mma<T>(f, qf[t][ks], s[kk][t]);
+            s[t] = mma<T>(f, qf[t][ks], s[t]);
             dp[t] = mma<T>(fv, gf[t][ks], dp[t]);
           }
         }
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-          const int hi = min(walk.klen - 1, pos[t] + a.right), lo = pos[t] - a.left;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            float p = fast_exp2(fmaf(s[kk][t][e], a.c, -ls[t]));
-            if constexpr (MASKED) {
-              const int key = s0 + 16 * kb + 4 * q + e;
-              if (key > hi || (key < lo && key >= a.sinks)) p = 0.f;
-            }
-            s[kk][t][e] = p * dp[t][e];                     // dS / scale
+            float p = fast_exp2(fmaf(s[t][e], a.c, -ls[t]));
+            if constexpr (MASKED) p = meets[t].or_zero(p, kb, e);
+            s[t][e] = p * dp[t][e];                        // dS / scale
           }
+          dsh[kk][t] = Half2<T>::pack(s[t]);
         }
       }
-      wmma_transposed<T, NDT, RT>(Ks, m2, s[0], s[1], acc, lane);
+      wmma_transposed<T, NDT, RT>(Ks, m2, dsh[0], dsh[1], acc, lane);
     }
   };
   if (walk.n > 0) fetch(walk.key0(0));
@@ -626,33 +725,45 @@ __global__ void __launch_bounds__(256, 2) win_dq_kernel(const WinArgs a, const T
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dk, dv
-// A workgroup owns 64 KT keys (16 KT per wave) of one key head and walks the 64-row tiles that see them.  grid.x: nsink * nsplit workgroups for the
-// blocks that hold sinks (partial sums), then one per remaining block.
+// A workgroup owns 64 KT keys (16 KT per wave) of one key head and walks the 64-row tiles that see them: nkb blocks per head without sinks, and
+// nsplit workgroups (partial sums) for each of the nsink blocks that hold them.
 template <typename T, int NDT, int KT>
 __global__ void __launch_bounds__(256, NDT * (int)sizeof(T) > 24 ? 1 : 2) win_dkv_kernel(const WinArgs a, const T* __restrict__ q_, const T* __restrict__ k_, const T* __restrict__ v_,
                                                       const T* __restrict__ dout, const float* __restrict__ lse, const float* __restrict__ delta,
-                                                      T* __restrict__ dk, T* __restrict__ dv, float* __restrict__ part) {
+                                                      T* __restrict__ dk, T* __restrict__ dv, float* __restrict__ part, int nkb) {
   typedef WT<T, NDT> W;
   constexpr int NK = W::NK;
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
-  float* rowdata = reinterpret_cast<float*>(lds + 4 * W::TILE);   // two buffers of 64 x (lse | D | position)
+  float* rowdata = reinterpret_cast<float*>(lds + 4 * W::TILE);   // two buffers of 64 x (lse | -D)
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
-  int x, h, b;
-  win_block(x, h, b);
-  const bool shared = x < a.nsink * a.nsplit;
-  const int kb = shared ? x / a.nsplit : x - a.nsink * a.nsplit + a.nsink, split = shared ? x % a.nsplit : 0;
+  // one dimension: all blocks without sinks first (each XCD a contiguous range: neighbours read the same rows), then the sink blocks' shares, which are
+  // short and fill the CUs that the last round of the others leaves idle
+  const int heads = a.B * a.Hkv, whole = heads * nkb, lin = blockIdx.x;
+  const bool shared = lin >= whole;
+  int kb, split = 0, bh;
+  if (shared) {
+    const int n = lin - whole, s = n / heads;
+    bh = n - s * heads;
+    kb = s / a.nsplit;
+    split = s - kb * a.nsplit;
+  } else {
+    const int per = whole >> 3, rem = whole & 7, xcd = lin & 7, lg = (xcd < rem ? xcd * (per + 1) : rem * (per + 1) + (xcd - rem) * per) + (lin >> 3);
+    bh = lg / nkb;
+    kb = lg - bh * nkb + a.nsink;
+  }
+  const int b = bh / a.Hkv, h = bh - b * a.Hkv;
   const int base = a.q_start ? clip_pos(a.q_start[b]) : 0;
   const int klen = a.key_len ? max(0, min(a.key_len[b], a.Tk)) : a.Tk;
   const int s0 = kb * 64 * KT, k0 = s0 + wave * 16 * KT;                   // first key of the workgroup, of the wave
   const T* qb = q_ + b * a.q_bs;
   zero_lds<T>(lds, 4 * W::TILE);
   typename W::frag kf[KT][NK], vf[KT][NK];
-  int plo[KT], phi[KT];                                             // positions that see this lane's keys
+  int rlo[KT], rhi[KT];                                           // rows [rlo, rhi) see this lane's keys
 #pragma unroll
   for (int t = 0; t < KT; ++t) {
     const int s = k0 + 16 * t + r;
-    plo[t] = s - a.right;
-    phi[t] = s >= klen ? -2 * FAR : s < a.sinks ? 2 * FAR : s + a.left;
+    rlo[t] = max(0, min(a.Tq, s - a.right - base)) * a.G;
+    rhi[t] = s >= klen ? 0 : s < a.sinks ? a.rows : max(0, min(a.Tq, s + a.left - base + 1)) * a.G;
 #pragma unroll
     for (int ks = 0; ks < NK; ++ks) {
       kf[t][ks] = gfrag<T>(k_ + b * a.k_bs + h * a.k_hs + s * a.k_ts, s < klen, ks, lane, a.dh);
@@ -667,17 +778,35 @@ __global__ void __launch_bounds__(256, NDT * (int)sizeof(T) > 24 ? 1 : 2) win_dk
   const int nt = (row1 - row0 + 63) >> 6, per = shared ? (nt + a.nsplit - 1) / a.nsplit : nt;
   const int t0 = split * per, t1 = min(nt, t0 + per);
   __syncthreads();
+#pragma unroll
+  for (int t = 0; t < KT; ++t)
+#pragma unroll
+    for (int ks = 0; ks < NK; ++ks) {
+      landed(kf[t][ks]);
+      landed(vf[t][ks]);
+    }
   Mover<T, NDT, 256> mv;
-  mv.init(a.dh);
+  // (a tile's first row is a frame's first head where 64 rows are whole frames: then its rows lie at the same places in every tile)
+  mv.init(a.dh, [&](int row, unsigned& x, unsigned& y) {
+    const int i = a.frame(row), g = row - i * a.G;
+    x = i * (unsigned)a.q_ts + g * (unsigned)a.q_hs;
+    y = (i * (unsigned)a.Hq + g) * (unsigned)a.dh;
+  });
+  const bool even = 64 % a.G == 0;
   float pre_l = 0.f, pre_d = 0.f;
   auto fetch = [&](int rt) {
     const int first = row0 + rt * 64;
-    mv.fetch([&](int n, const T*& x, const T*& y) {
-      const int row = first + n, i = a.frame(row), g = row - i * a.G;
-      x = qb + i * a.q_ts + (long)(h * a.G + g) * a.q_hs;
-      y = dout + (((long)b * a.Tq + i) * a.Hq + h * a.G + g) * a.dh;
-      return row < row1;
-    });
+    if (even && first + 64 <= row1) {
+      const int i = a.frame(first);
+      mv.fetch_whole(qb + i * a.q_ts + (long)(h * a.G) * a.q_hs, dout + (((long)b * a.Tq + i) * a.Hq + h * a.G) * a.dh);
+    } else {
+      mv.fetch([&](int n, const T*& x, const T*& y) {
+        const int row = first + n, i = a.frame(row), g = row - i * a.G;
+        x = qb + i * a.q_ts + (long)(h * a.G + g) * a.q_hs;
+        y = dout + (((long)b * a.Tq + i) * a.Hq + h * a.G + g) * a.dh;
+        return row < row1;
+      });
+    }
     if (threadIdx.x < 64) {
       const int row = first + (int)threadIdx.x, i = a.frame(row), g = row - i * a.G;
       const long orow = ((long)b * a.Tq + i) * a.Hq + h * a.G + g;
@@ -690,66 +819,100 @@ __global__ void __launch_bounds__(256, NDT * (int)sizeof(T) > 24 ? 1 : 2) win_dk
   for (int t = 0; t < KT; ++t)
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) ak[t][dt] = av[t][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-  auto compute = [&](const unsigned char* Qs, const float* rd, auto masked_c) {
+  auto compute = [&](const unsigned char* Qs, const float* rd, int first_row, auto masked_c) {
     constexpr bool MASKED = decltype(masked_c)::value;
+    Meets meets[KT];
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+      if constexpr (MASKED) meets[t] = Meets(rlo[t] - first_row, rhi[t] - first_row, 0, q);
     const unsigned char* Gs = Qs + W::TILE;
+    // Three stages per 16 rows: the products S and dP - D, the probabilities and dS out of them, the products that sum dv and dk (32 rows at a
+    // time).  They are issued one behind the other's successor -- the first stage of rows n + 1 with the second of rows n --, so that the matrix
+    // pipe has work of this wave while its vector instructions run; two waves per SIMD alone leave both idle half of the time.
+    f32x4 p[2][KT], ds[2][KT];
+    typename Half2<T>::type ph[2][KT], dsh[2][KT];
+    typename W::frag fq[2][NK], fg[2][NK];
+    auto load = [&](int rb) {
 #pragma unroll
-    for (int m2 = 0; m2 < 2; ++m2) {
-      f32x4 p[2][KT], ds[2][KT];
+      for (int ks = 0; ks < NK; ++ks) {
+        fq[rb & 1][ks] = wfrag<T, NDT>(Qs, 16 * rb + r, ks, lane);
+        fg[rb & 1][ks] = wfrag<T, NDT>(Gs, 16 * rb + r, ks, lane);
+      }
+    };
+    auto first = [&](int rb) {
+      const f32x4 d4 = *reinterpret_cast<const f32x4*>(rd + 64 + 16 * rb + 4 * q);
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
-        const int rb = 2 * m2 + kk;
-        const f32x4 l4 = *reinterpret_cast<const f32x4*>(rd + 16 * rb + 4 * q);
-        const f32x4 d4 = *reinterpret_cast<const f32x4*>(rd + 64 + 16 * rb + 4 * q);
+      for (int t = 0; t < KT; ++t) {
+        p[rb & 1][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        ds[rb & 1][t] = d4;                                  // -D: dP - D out of the product itself
+      }
+#pragma unroll
+      for (int ks = 0; ks < NK; ++ks)
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
-          p[kk][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-          ds[kk][t] = d4;                                  // -D: dP - D out of the product itself
+          p[rb & 1][t] = mma<T>(fq[rb & 1][ks], kf[t][ks], p[rb & 1][t]);
+          ds[rb & 1][t] = mma<T>(fg[rb & 1][ks], vf[t][ks], ds[rb & 1][t]);
         }
+    };
+    auto soft = [&](int rb) {
+      const f32x4 l4 = *reinterpret_cast<const f32x4*>(rd + 16 * rb + 4 * q);
 #pragma unroll
-        for (int ks = 0; ks < NK; ++ks) {
-          const typename W::frag f = wfrag<T, NDT>(Qs, 16 * rb + r, ks, lane), fg = wfrag<T, NDT>(Gs, 16 * rb + r, ks, lane);
+      for (int t = 0; t < KT; ++t) {
 #pragma unroll
-          for (int t = 0; t < KT; ++t) {
-            p[kk][t] = mma<T>(f, kf[t][ks], p[kk][t]);
-            ds[kk][t] = mma<T>(fg, vf[t][ks], ds[kk][t]);
-          }
+        for (int e = 0; e < 4; ++e) {
+          float w = fast_exp2(fmaf(p[rb & 1][t][e], a.c, -l4[e]));
+          if constexpr (MASKED) w = meets[t].or_zero(w, rb, e);
+          p[rb & 1][t][e] = w;
+          ds[rb & 1][t][e] *= w;                             // dS / scale
         }
-        const int* p4 = reinterpret_cast<const int*>(rd + 128 + 16 * rb + 4 * q);
-#pragma unroll
-        for (int t = 0; t < KT; ++t)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float w = fast_exp2(fmaf(p[kk][t][e], a.c, -l4[e]));
-            if constexpr (MASKED) {
-              const int at = p4[e];
-              if (at < plo[t] || at > phi[t]) w = 0.f;
-            }
-            p[kk][t][e] = w;
-            ds[kk][t][e] *= w;                             // dS / scale
-          }
+        ph[rb & 1][t] = Half2<T>::pack(p[rb & 1][t]);
+        dsh[rb & 1][t] = Half2<T>::pack(ds[rb & 1][t]);
       }
-      wmma_transposed<T, NDT, KT>(Gs, m2, p[0], p[1], av, lane);
-      wmma_transposed<T, NDT, KT>(Qs, m2, ds[0], ds[1], ak, lane);
+    };
+#define FH_STAGE __builtin_amdgcn_sched_barrier(0);
+    if constexpr (sizeof(T) == 2) {
+      bf16x8 cg[NDT], cq[NDT];
+      load(0);
+      FH_STAGE load(1); first(0);
+      FH_STAGE load(2); first(1); soft(0);
+      FH_STAGE load(3); tile_columns<T, NDT>(Gs, 0, cg, lane); first(2); soft(1);
+      FH_STAGE tile_columns<T, NDT>(Qs, 0, cq, lane); mma_columns<T, NDT, KT>(cg, ph[0], ph[1], av); 
+      FH_STAGE tile_columns<T, NDT>(Gs, 1, cg, lane); mma_columns<T, NDT, KT>(cq, dsh[0], dsh[1], ak); soft(2);
+      FH_STAGE first(3); tile_columns<T, NDT>(Qs, 1, cq, lane);
+      FH_STAGE soft(3);
+      mma_columns<T, NDT, KT>(cg, ph[0], ph[1], av);
+      mma_columns<T, NDT, KT>(cq, dsh[0], dsh[1], ak);
+    } else {
+#pragma unroll
+      for (int m2 = 0; m2 < 2; ++m2) {
+        load(2 * m2);
+        first(2 * m2);
+        soft(2 * m2);
+        load(2 * m2 + 1);
+        first(2 * m2 + 1);
+        soft(2 * m2 + 1);
+        wmma_transposed<T, NDT, KT>(Gs, m2, ph[0], ph[1], av, lane);
+        wmma_transposed<T, NDT, KT>(Qs, m2, dsh[0], dsh[1], ak, lane);
+      }
     }
+#undef FH_STAGE
   };
   if (t0 < t1) fetch(t0);
   for (int rt = t0; rt < t1; ++rt) {
     unsigned char* Qs = lds + ((rt - t0) & 1) * 2 * W::TILE;
-    float* rd = rowdata + ((rt - t0) & 1) * 192;
+    float* rd = rowdata + ((rt - t0) & 1) * 128;
     mv.deposit(Qs);
     if (threadIdx.x < 64) {
       rd[threadIdx.x] = pre_l;
       rd[64 + threadIdx.x] = -pre_d;
-      reinterpret_cast<int*>(rd)[128 + threadIdx.x] = base + a.frame(row0 + rt * 64 + (int)threadIdx.x);
     }
     __syncthreads();
     if (rt + 1 < t1) fetch(rt + 1);
     // positions of the tile's rows against those that see the wave's keys
     const int p0 = base + a.frame(row0 + rt * 64), p1 = base + a.frame(min(row0 + rt * 64 + 63, row1 - 1)), ke = min(k0 + 16 * KT, klen) - 1;
     if (ke < k0 || p1 < k0 - a.right || (p0 > ke + a.left && k0 >= a.sinks)) continue;
-    if (k0 + 16 * KT - 1 < klen && p0 >= k0 + 16 * KT - 1 - a.right && (p1 <= k0 + a.left || k0 + 16 * KT - 1 < a.sinks)) compute(Qs, rd, std::false_type{});
-    else compute(Qs, rd, std::true_type{});
+    if (k0 + 16 * KT - 1 < klen && p0 >= k0 + 16 * KT - 1 - a.right && (p1 <= k0 + a.left || k0 + 16 * KT - 1 < a.sinks)) compute(Qs, rd, row0 + rt * 64, std::false_type{});
+    else compute(Qs, rd, row0 + rt * 64, std::true_type{});
   }
 #pragma unroll
   for (int t = 0; t < KT; ++t) {
@@ -853,11 +1016,13 @@ int run_dq(const WinArgs& a, const void* q, const void* k, const void* v, const 
 template <typename T, int NDT, int KT>
 int run_dkv(const WinArgs& a, const void* q, const void* k, const void* v, const void* dout, const float* lse, const float* delta, void* dk, void* dv, float* part,
             hipStream_t st) {
-  const size_t smem = 4 * WT<T, NDT>::TILE + 2 * 192 * 4;
+  const size_t smem = 4 * WT<T, NDT>::TILE + 2 * 128 * 4;
   if (int rc = set_lds(win_dkv_kernel<T, NDT, KT>, smem)) return rc;
-  const int nkb = (a.Tk + 64 * KT - 1) / (64 * KT);
-  hipLaunchKernelGGL((win_dkv_kernel<T, NDT, KT>), dim3(a.nsink * a.nsplit + nkb - a.nsink, a.Hkv, a.B), dim3(256), smem, st, a, (const T*)q, (const T*)k, (const T*)v,
-                     (const T*)dout, lse, delta, (T*)dk, (T*)dv, part);
+  const int nkb = (a.Tk + 64 * KT - 1) / (64 * KT) - a.nsink;
+  const long wgs = (long)a.B * a.Hkv * (nkb + a.nsink * a.nsplit);
+  if (wgs > 0x7fffffffL) return -930;
+  hipLaunchKernelGGL((win_dkv_kernel<T, NDT, KT>), dim3((unsigned)wgs), dim3(256), smem, st, a, (const T*)q, (const T*)k, (const T*)v, (const T*)dout, lse, delta, (T*)dk,
+                     (T*)dv, part, nkb);
   FH_CHECK_LAUNCH();
   return 0;
 }

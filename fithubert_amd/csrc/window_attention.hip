@@ -9,6 +9,11 @@ int check(int dtype, const fh_window_attention_desc* d) {
   if (d->dh < 8 || d->dh > 128 || d->dh % 8) return -923;
   if (d->B > 65535 || d->Hkv > 65535 || d->Tq >= FAR || d->Tk >= FAR || (long)d->Tq * (d->Hq / d->Hkv) >= FAR) return -924;
   if (!(d->scale > 0.f) || !(d->scale < INFINITY)) return -925;
+  // a 64-row tile's places are 32-bit byte offsets from its first row
+  const long far = 1 << 23, st[6] = {d->q_ts, d->q_hs, d->k_ts, d->k_hs, d->v_ts, d->v_hs};
+  for (long x : st)
+    if (x < 0 || x > far) return -929;
+  if (d->q_bs < 0 || d->k_bs < 0 || d->v_bs < 0 || (long)d->Hq * d->dh > far) return -929;
   const long vec = dtype == 0 ? 4 : 8;
   if ((d->q_bs | d->q_ts | d->q_hs | d->k_bs | d->k_ts | d->k_hs | d->v_bs | d->v_ts | d->v_hs) % vec) return -926;
   return 0;

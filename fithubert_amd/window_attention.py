@@ -19,10 +19,10 @@ _DT = {torch.float32: L.DT_F32, torch.bfloat16: L.DT_BF16, torch.float16: L.DT_F
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
-    """t itself where the kernels can read it in place: channels contiguous, address and strides multiples of 16 bytes (strides of axes of length 1 do
-    not count); a contiguous copy otherwise"""
+    """t itself where the kernels can read it in place: channels contiguous, address and strides multiples of 16 bytes, frames and heads at most 2^23 elements
+    apart (strides of axes of length 1 do not count); a contiguous copy otherwise"""
     vec = 16 // t.element_size()
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % vec == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1):
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % vec == 0 and (s <= 1 << 23 or not i) for i, (s, n) in enumerate(zip(t.stride()[:-1], t.shape[:-1])) if n > 1):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 

@@ -265,8 +265,8 @@ int fh_attention_backward_bias(int dtype, const void* qkv, const void* out, cons
  * Query i of entry b stands at position p = q_start[b] + i and sees key s when
  *     s < key_len[b]   and   s <= p + right   and   (s >= p - left  or  s < sinks).
  *   out = softmax(scale * q k^T over the keys it sees) v;   a row that sees none: out = 0, and it takes part in no gradient.
- * q [B][Tq][Hq][dh], k, v [B][Tk][Hkv][dh] by the strides below (elements; channels contiguous; addresses and strides multiples of 16
- * bytes), so a packed q|k|v projection or a longer cache is read in place; query head h reads key head h / (Hq / Hkv).
+ * q [B][Tq][Hq][dh], k, v [B][Tk][Hkv][dh] by the strides below (elements, not negative; channels contiguous; addresses and strides multiples
+ * of 16 bytes; frames and heads at most 2^23 elements apart), so a packed q|k|v projection or a longer cache is read in place; query head h reads key head h / (Hq / Hkv).
  * out, dout, dq [B][Tq][Hq][dh] and dk, dv [B][Tk][Hkv][dh] are contiguous; lse: B * Tq * Hq floats that the backward reads (forward: NULL
  * when there is none).  dq, dk, dv are written, not added to (keys that no row sees: 0).  dh <= 128, a multiple of 8; 16-bit modes round the
  * probabilities and dS to the element type before the second products, sums and softmax are fp32.  No atomics: results repeat bit for bit.
