@@ -25,14 +25,26 @@ namespace {
 template <typename T, int NDT> struct WT {
   static constexpr int KD = AT<T>::KD;
   static constexpr int NK = (NDT * 16 + KD - 1) / KD;   // fragments per row
-  static constexpr int RS = NK * 64 + 16;               // LDS row stride (bytes): 16 bytes of skew against bank conflicts
+  static constexpr int CP = NK <= 2 ? 8 : NK <= 4 ? 16 : 32;      // 16-byte pieces of a row's room, a power of two
+  static constexpr int RS = sizeof(T) == 2 ? CP * 16 : NK * 64 + 16; // LDS row stride (bytes)
   static constexpr int TILE = 64 * RS;
   static constexpr int VEC = ElemTraits<T>::VEC;
   typedef typename AT<T>::frag frag;
+  static constexpr int OCC = sizeof(T) == 4 && NDT >= 6 ? 1 : 2;   // waves per SIMD that the registers are cut for
+  // The 16-byte piece c of a row lies at place c ^ twist(row).  The LDS serves 256 bytes at a time: sixteen rows' fragments (one piece each), the column reads'
+  // two pieces of eight rows; the twists put each of these on 64 different banks (rows of 128 bytes: even and odd rows lie on different halves
+  // already).  fp32: no twist, 16 bytes of skew per row (its column reads are single floats; the twisted form took more registers and time).
+  static __device__ __forceinline__ int twist(int row) {
+    return sizeof(T) == 4 ? 0 : RS == 128 ? (row & 6) | ((row >> 3) & 1) : ((row & 7) << 1) | ((row >> 3) & 1);
+  }
+  static __device__ __forceinline__ int place(int row, int c) { return row * RS + ((c ^ twist(row)) << 4); }
 };
 
-template <typename T, int NDT> __device__ __forceinline__ typename AT<T>::frag wfrag(const unsigned char* lds, int row, int ks, int lane) {
-  return *reinterpret_cast<const typename AT<T>::frag*>(lds + row * WT<T, NDT>::RS + ks * 64 + (lane >> 4) * 16);
+// fragment ks of row 16 n + (lane & 15)
+template <typename T, int NDT> __device__ __forceinline__ typename AT<T>::frag wfrag(const unsigned char* lds, int n, int ks, int lane) {
+  typedef WT<T, NDT> W;
+  const int x = (lane >> 4) ^ W::twist(lane & 15);
+  return *reinterpret_cast<const typename W::frag*>(lds + (16 * n + (lane & 15)) * W::RS + ((x ^ ((ks & 3) << 2)) << 4) + (ks >> 2) * 256);
 }
 
 typedef __attribute__((ext_vector_type(2))) float f32x2;
@@ -65,10 +77,11 @@ template <> struct Half2<float> {
 // The columns of rows 32 m2 .. 32 m2 + 31 of an LDS tile as first operands (one per 16 channels): transposing reads (16-bit).
 template <typename T, int NDT> __device__ __forceinline__ void tile_columns(const unsigned char* tile, int m2, bf16x8 (&col)[NDT], int lane) {
   constexpr int RS = WT<T, NDT>::RS;
-  const int i = lane & 15, q = lane >> 4;
+  const int i = lane & 15, q = lane >> 4, row = 4 * q + (i >> 2), y = ((i >> 1) & 1) ^ WT<T, NDT>::twist(row);
+  const unsigned char* base = tile + (32 * m2 + row) * RS + (i & 1) * 8;
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt) {
-    const unsigned char* a0 = tile + (32 * m2 + 4 * q + (i >> 2)) * RS + (16 * dt + 4 * (i & 3)) * 2;
+    const unsigned char* a0 = base + ((y ^ (2 * dt)) << 4);
     union { struct { s16x4 lo, hi; } s; bf16x8 v; } u;
     u.s.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)a0);
     u.s.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a0 + 16 * RS));
@@ -97,7 +110,6 @@ __device__ __forceinline__ void wmma_transposed(const unsigned char* tile, int m
     tile_columns<T, NDT>(tile, m2, col, lane);
     mma_columns<T, NDT, RT>(col, P0, P1, acc);
   } else {
-    constexpr int RS = WT<T, NDT>::RS;
     const int i = lane & 15, q = lane >> 4;
 #pragma unroll
     for (int half = 0; half < 2; ++half)
@@ -106,7 +118,7 @@ __device__ __forceinline__ void wmma_transposed(const unsigned char* tile, int m
         const int row = 32 * m2 + 16 * half + 4 * q + e;
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) {
-          const float a = *reinterpret_cast<const float*>(tile + row * RS + (16 * dt + i) * 4);
+          const float a = *reinterpret_cast<const float*>(tile + WT<T, NDT>::place(row, 4 * dt + (i >> 2)) + (i & 3) * 4);
 #pragma unroll
           for (int t = 0; t < RT; ++t) acc[t][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, half ? P1[t][e] : P0[t][e], acc[t][dt], 0, 0, 0);
         }
@@ -123,25 +135,26 @@ template <typename F> __device__ __forceinline__ void landed(F& f) { asm volatil
 // its rows lie from the tile's first one is the same for every tile (x_of, y_of: 32-bit byte offsets), so a whole tile costs a load per
 // piece and no address arithmetic.
 template <typename T, int NDT, int NT> struct Mover {
+  typedef WT<T, NDT> W;
   static constexpr int VEC = WT<T, NDT>::VEC;
-  static constexpr int CP = NDT * 16 / VEC;        // columns at the widest head
+  static constexpr int CP = W::CP;                 // columns of a row's LDS room
   static constexpr int RP = NT / CP;               // rows per pass
-  static constexpr int NP = (64 + RP - 1) / RP;    // passes
+  static constexpr int NP = 64 / RP;               // passes
+  static_assert(NT % CP == 0 && 64 % RP == 0, "whole passes");
   V16 pre[2][NP];
   unsigned x_of[NP], y_of[NP];
-  int row, col, dst;
+  int row, col;
   bool live;
   // off(row, x, y): element offsets of a row from the tile's first row
   template <typename F> __device__ __forceinline__ void init(int dh, F&& off) {
     row = (int)threadIdx.x / CP;
     const int c = (int)threadIdx.x - row * CP;
     col = c * VEC;
-    live = row < RP && col < dh;
-    dst = row * WT<T, NDT>::RS + c * 16;
+    live = col < dh;
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
       unsigned x, y;
-      off(min(row + j * RP, 63), x, y);
+      off(row + j * RP, x, y);
       x_of[j] = (x + col) * sizeof(T);
       y_of[j] = (y + col) * sizeof(T);
     }
@@ -150,11 +163,10 @@ template <typename T, int NDT, int NT> struct Mover {
   __device__ __forceinline__ void fetch_whole(const T* x, const T* y) {
     if (live) {
 #pragma unroll
-      for (int j = 0; j < NP; ++j)
-        if (64 % RP == 0 || j < NP - 1 || row + j * RP < 64) {
-          pre[0][j] = ld16((const char*)x + x_of[j]);
-          pre[1][j] = ld16((const char*)y + y_of[j]);
-        }
+      for (int j = 0; j < NP; ++j) {
+        pre[0][j] = ld16((const char*)x + x_of[j]);
+        pre[1][j] = ld16((const char*)y + y_of[j]);
+      }
     }
   }
   // at(row, first, second): the addresses of a row's channels in the two tensors; false: zeros
@@ -163,7 +175,7 @@ template <typename T, int NDT, int NT> struct Mover {
     for (int j = 0; j < NP; ++j) {
       pre[0][j] = pre[1][j] = v16_zero();
       const T *x, *y;
-      if (live && row + j * RP < 64 && at(row + j * RP, x, y)) {
+      if (live && at(row + j * RP, x, y)) {
         pre[0][j] = ld16(x + col);
         pre[1][j] = ld16(y + col);
       }
@@ -172,11 +184,12 @@ template <typename T, int NDT, int NT> struct Mover {
   __device__ __forceinline__ void deposit(unsigned char* pair) const {
     if (live) {
 #pragma unroll
-      for (int j = 0; j < NP; ++j)
-        if (64 % RP == 0 || j < NP - 1 || row + j * RP < 64) {
-          st16(pair + dst + j * RP * WT<T, NDT>::RS, pre[0][j]);
-          st16(pair + WT<T, NDT>::TILE + dst + j * RP * WT<T, NDT>::RS, pre[1][j]);
-        }
+      for (int j = 0; j < NP; ++j) {
+        // (rows 16 apart share their twist)
+        const int at = sizeof(T) == 4 || RP % 16 == 0 ? W::place(row, col / VEC) + j * RP * W::RS : W::place(row + j * RP, col / VEC);
+        st16(pair + at, pre[0][j]);
+        st16(pair + W::TILE + at, pre[1][j]);
+      }
     }
   }
 };
@@ -280,7 +293,7 @@ __device__ __forceinline__ void softmax_step(const WinArgs& a, f32x4 (&s)[4][RT]
 }
 
 template <typename T, int NDT, int RT, bool SPLIT>
-__global__ void __launch_bounds__(256, NDT * RT * (int)sizeof(T) > 32 ? 1 : 2) win_fwd_kernel(const WinArgs a, const T* __restrict__ q_, const T* __restrict__ k_, const T* __restrict__ v_,
+__global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_fwd_kernel(const WinArgs a, const T* __restrict__ q_, const T* __restrict__ k_, const T* __restrict__ v_,
                                                           T* __restrict__ out, float* __restrict__ lse, float* __restrict__ part) {
   typedef WT<T, NDT> W;
   constexpr int NK = W::NK;
@@ -345,7 +358,7 @@ __global__ void __launch_bounds__(256, NDT * RT * (int)sizeof(T) > 32 ? 1 : 2) w
       for (int t = 0; t < RT; ++t) s[kb][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int ks = 0; ks < NK; ++ks) {
-        const typename W::frag f = wfrag<T, NDT>(Ks, 16 * kb + r, ks, lane);
+        const typename W::frag f = wfrag<T, NDT>(Ks, kb, ks, lane);
 #pragma unroll
         for (int t = 0; t < RT; ++t) s[kb][t] = mma<T>(f, qf[t][ks], s[kb][t]);
       }
@@ -407,7 +420,7 @@ __global__ void __launch_bounds__(256, NDT * RT * (int)sizeof(T) > 32 ? 1 : 2) w
 // time, so the four waves of a workgroup walk tiles of their own, without a barrier: keys go straight from memory into the first product's operand
 // registers, values through a tile of LDS that only this wave uses, and both are requested a tile ahead.  The waves' sums meet at the end.
 template <typename T, int NDT, int TT>
-__global__ void __launch_bounds__(256, NDT * TT * (int)sizeof(T) > 16 ? 1 : 2) win_few_kernel(const WinArgs a, const T* __restrict__ q_, const T* __restrict__ k_,
+__global__ void __launch_bounds__(256, NDT * TT * (int)sizeof(T) > 12 ? 1 : 2) win_few_kernel(const WinArgs a, const T* __restrict__ q_, const T* __restrict__ k_,
                                                                                     const T* __restrict__ v_, T* __restrict__ out, float* __restrict__ lse,
                                                                                     float* __restrict__ part) {
   typedef WT<T, NDT> W;
@@ -477,7 +490,7 @@ __global__ void __launch_bounds__(256, NDT * TT * (int)sizeof(T) > 16 ? 1 : 2) w
 #pragma unroll
     for (int j = 0; j < CP; ++j) {
       const int at = j * 64 + lane;
-      st16(tile + (at / CP) * W::RS + (at % CP) * 16, vf[j]);
+      st16(tile + W::place(at / CP, at % CP), vf[j]);
     }
     if (kt + 4 < kt1) fetch(walk.key0(kt + 4));
     typename Half2<T>::type ph[4][TT];
@@ -578,7 +591,7 @@ __global__ void __launch_bounds__(256) win_join_kernel(const WinArgs a, const fl
 
 // ------------------------------------------------------------------------------------------------ backward: dq, and D for the other pass
 template <typename T, int NDT, int RT>
-__global__ void __launch_bounds__(256, 2) win_dq_kernel(const WinArgs a, const T* __restrict__ q_, const T* __restrict__ k_, const T* __restrict__ v_,
+__global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_dq_kernel(const WinArgs a, const T* __restrict__ q_, const T* __restrict__ k_, const T* __restrict__ v_,
                                                          const T* __restrict__ out, const T* __restrict__ dout, const float* __restrict__ lse,
                                                          float* __restrict__ delta, T* __restrict__ dq) {
   typedef WT<T, NDT> W;
@@ -674,7 +687,7 @@ __global__ void __launch_bounds__(256, 2) win_dq_kernel(const WinArgs a, const T
         }
 #pragma unroll
         for (int ks = 0; ks < NK; ++ks) {
-          const typename W::frag f = wfrag<T, NDT>(Ks, 16 * kb + r, ks, lane), fv = wfrag<T, NDT>(Vs, 16 * kb + r, ks, lane);
+          const typename W::frag f = wfrag<T, NDT>(Ks, kb, ks, lane), fv = wfrag<T, NDT>(Vs, kb, ks, lane);
 #pragma unroll
           for (int t = 0; t < RT; ++t) {
             s[t] = mma<T>(f, qf[t][ks], s[t]);
@@ -728,7 +741,7 @@ __global__ void __launch_bounds__(256, 2) win_dq_kernel(const WinArgs a, const T
 // A workgroup owns 64 KT keys (16 KT per wave) of one key head and walks the 64-row tiles that see them: nkb blocks per head without sinks, and
 // nsplit workgroups (partial sums) for each of the nsink blocks that hold them.
 template <typename T, int NDT, int KT>
-__global__ void __launch_bounds__(256, NDT * (int)sizeof(T) > 24 ? 1 : 2) win_dkv_kernel(const WinArgs a, const T* __restrict__ q_, const T* __restrict__ k_, const T* __restrict__ v_,
+__global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_dkv_kernel(const WinArgs a, const T* __restrict__ q_, const T* __restrict__ k_, const T* __restrict__ v_,
                                                       const T* __restrict__ dout, const float* __restrict__ lse, const float* __restrict__ delta,
                                                       T* __restrict__ dk, T* __restrict__ dv, float* __restrict__ part, int nkb) {
   typedef WT<T, NDT> W;
@@ -835,8 +848,8 @@ __global__ void __launch_bounds__(256, NDT * (int)sizeof(T) > 24 ? 1 : 2) win_dk
     auto load = [&](int rb) {
 #pragma unroll
       for (int ks = 0; ks < NK; ++ks) {
-        fq[rb & 1][ks] = wfrag<T, NDT>(Qs, 16 * rb + r, ks, lane);
-        fg[rb & 1][ks] = wfrag<T, NDT>(Gs, 16 * rb + r, ks, lane);
+        fq[rb & 1][ks] = wfrag<T, NDT>(Qs, rb, ks, lane);
+        fg[rb & 1][ks] = wfrag<T, NDT>(Gs, rb, ks, lane);
       }
     };
     auto first = [&](int rb) {
@@ -897,22 +910,30 @@ __global__ void __launch_bounds__(256, NDT * (int)sizeof(T) > 24 ? 1 : 2) win_dk
     }
 #undef FH_STAGE
   };
-  if (t0 < t1) fetch(t0);
-  for (int rt = t0; rt < t1; ++rt) {
-    unsigned char* Qs = lds + ((rt - t0) & 1) * 2 * W::TILE;
-    float* rd = rowdata + ((rt - t0) & 1) * 128;
+  // Neighbouring blocks see mostly the same rows, one block's worth further on.  Each begins its walk where the tile's place among all rows is a multiple of the
+  // walk's length (and wraps): the workgroups of an XCD then read the same few tiles at the same time instead of as many as they are, which their
+  // L2 does not hold (ten minutes of audio: 403 -> 387 us).
+  const int n = t1 - t0;
+  int rt = t0 + (n > 0 ? (n - ((row0 >> 6) + t0) % n) % n : 0);
+  if (n > 0) fetch(rt);
+  for (int k = 0; k < n; ++k) {
+    const int next = rt + 1 < t1 ? rt + 1 : t0;
+    unsigned char* Qs = lds + (k & 1) * 2 * W::TILE;
+    float* rd = rowdata + (k & 1) * 128;
     mv.deposit(Qs);
     if (threadIdx.x < 64) {
       rd[threadIdx.x] = pre_l;
       rd[64 + threadIdx.x] = -pre_d;
     }
     __syncthreads();
-    if (rt + 1 < t1) fetch(rt + 1);
+    if (k + 1 < n) fetch(next);
+    const int at = row0 + rt * 64;
+    rt = next;
     // positions of the tile's rows against those that see the wave's keys
-    const int p0 = base + a.frame(row0 + rt * 64), p1 = base + a.frame(min(row0 + rt * 64 + 63, row1 - 1)), ke = min(k0 + 16 * KT, klen) - 1;
+    const int p0 = base + a.frame(at), p1 = base + a.frame(min(at + 63, row1 - 1)), ke = min(k0 + 16 * KT, klen) - 1;
     if (ke < k0 || p1 < k0 - a.right || (p0 > ke + a.left && k0 >= a.sinks)) continue;
-    if (k0 + 16 * KT - 1 < klen && p0 >= k0 + 16 * KT - 1 - a.right && (p1 <= k0 + a.left || k0 + 16 * KT - 1 < a.sinks)) compute(Qs, rd, row0 + rt * 64, std::false_type{});
-    else compute(Qs, rd, row0 + rt * 64, std::true_type{});
+    if (k0 + 16 * KT - 1 < klen && p0 >= k0 + 16 * KT - 1 - a.right && (p1 <= k0 + a.left || k0 + 16 * KT - 1 < a.sinks)) compute(Qs, rd, at, std::false_type{});
+    else compute(Qs, rd, at, std::true_type{});
   }
 #pragma unroll
   for (int t = 0; t < KT; ++t) {
@@ -1034,7 +1055,7 @@ int bwd_t(WinArgs a, const void* q, const void* k, const void* v, const void* ou
   float* part = (float*)(scratch + al16((size_t)a.B * a.Tq * a.Hq * 4));
   if (a.rows > 0) {
     int rc;
-    if constexpr (NDT <= (DT == 0 ? 4 : 6)) {
+    if constexpr (DT != 0 && NDT <= 6) {
       rc = bwd_tiles(a, DT, (long)a.B * a.Hkv * ((a.rows + 127) / 128), false) == 2 ? run_dq<T, NDT, 2>(a, q, k, v, out, dout, lse, delta, dq, st)
                                                                                      : run_dq<T, NDT, 1>(a, q, k, v, out, dout, lse, delta, dq, st);
     } else {
@@ -1046,7 +1067,7 @@ int bwd_t(WinArgs a, const void* q, const void* k, const void* v, const void* ou
     const int keys = dkv_keys(a, DT);
     bwd_sinks(a, keys);
     int rc;
-    if constexpr (NDT <= (DT == 0 ? 3 : 4)) {
+    if constexpr (DT != 0 && NDT <= 4) {
       rc = keys == 128 ? run_dkv<T, NDT, 2>(a, q, k, v, dout, lse, delta, dk, dv, part, st) : run_dkv<T, NDT, 1>(a, q, k, v, dout, lse, delta, dk, dv, part, st);
     } else {
       rc = run_dkv<T, NDT, 1>(a, q, k, v, dout, lse, delta, dk, dv, part, st);

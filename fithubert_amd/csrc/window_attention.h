@@ -48,8 +48,7 @@ static inline void bwd_sinks(WinArgs& a, int keys) {
 }
 // 16-key (16-row) tiles per wave of the backward passes: two where that still gives every CU two workgroups, and where the accumulators fit
 static inline int bwd_tiles(const WinArgs& a, int dtype, long blocks128, bool dkv) {
-  const int widest = dkv ? (dtype == 0 ? 48 : 64) : (dtype == 0 ? 64 : 96);
-  return a.dh <= widest && blocks128 >= 512 ? 2 : 1;
+  return dtype != 0 && a.dh <= (dkv ? 64 : 96) && blocks128 >= 512 ? 2 : 1;
 }
 static inline int dkv_keys(const WinArgs& a, int dtype) { return 64 * bwd_tiles(a, dtype, (long)a.B * a.Hkv * ((a.Tk + 127) / 128), true); }
 static inline size_t al16(size_t n) { return (n + 15) & ~(size_t)15; }
