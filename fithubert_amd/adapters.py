@@ -73,13 +73,13 @@ class _AdapterLinear(torch.autograd.Function):
         dy = _dense(dy)
         need = ctx.needs_input_grad
         dx = torch.empty_like(x) if need[0] else None
-        da = torch.empty(a.shape, dtype=torch.float32, device=dev) if need[3] else None
-        db = torch.empty(b.shape, dtype=torch.float32, device=dev) if need[4] else None
+        da = torch.empty_like(a) if need[3] else None
+        db = torch.empty_like(b) if need[4] else None
         with torch.cuda.device(dev):
             scratch = _scratch(dt, d, 1, dev)
             L.check(L.lib().fh_adapter_linear_backward(dt, C.byref(d), x.data_ptr(), weight.data_ptr(), a.data_ptr(), b.data_ptr(), h.data_ptr(), dy.data_ptr(),
                                                        _ptr(dx), _ptr(da), _ptr(db), _ptr(scratch), torch.cuda.current_stream(dev).cuda_stream), "fh_adapter_linear_backward")
-        return dx, None, None, da.to(a.dtype) if da is not None else None, db.to(b.dtype) if db is not None else None, None, None, None
+        return dx, None, None, da, db, None, None, None
 
 
 def adapter_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], lora_a: torch.Tensor, lora_b: torch.Tensor, scaling: torch.Tensor,

@@ -6,10 +6,10 @@
 // down:   h and G.  A workgroup owns 16 rows, its four waves split the long reduction (K or N) and join in LDS: one pass over x (dy), many
 //         short workgroups, so that a handful of rows is as quick as its longest load chain.  Rows of several segments: one trip per segment
 //         that the tile touches, dealt over grid.y where requests are short.
-// up:     the products with B_a (A_a), added to the shared projection's GEMM as its residual operand.
+// up:     the products with B_a (A_a), added to the accumulators of the shared projection's GEMM (fp32, small backward: its residual operand).
 // outer:  dA and dB: a workgroup owns 64 columns of one adapter's factor and walks that adapter's rows, whichever segments they lie in, 32
 //         at a time per wave; long walks are dealt over several workgroups whose partial sums are added in order (no atomics).
-#include "gemm.h"
+#include "gemm_loops.cuh"
 #include "kernels.h"
 #include "attn_frag.cuh"
 
@@ -22,35 +22,48 @@ struct Segs {
   int n, adapters, M;
   __device__ __forceinline__ int begin(int s) const { return max(0, min(M, start[s])); }
   __device__ __forceinline__ int adapter(int s) const { const int a = which[s]; return a >= 0 && a < adapters ? a : -1; }
-  // number of segments that end at or before `row`: the first one that may hold it
-  __device__ __forceinline__ int first_at(int row) const {
-    int lo = 0, hi = n;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (start[mid + 1] <= row) lo = mid + 1; else hi = mid;
+  // number of segments that end at or before `row`: the first one that may hold it.  The 64 lanes look at 64 places at a time.
+  __device__ __forceinline__ int first_at(int row, int lane) const {
+    int lo = 0, len = n;
+    while (len > 0) {
+      const int step = (len + 63) >> 6, at = lo + lane * step + step - 1;
+      const int passed = __popcll(__ballot(at < lo + len && start[min(at, n - 1) + 1] <= row));
+      lo += passed * step;
+      len = step > 1 ? min(step - 1, lo + step - 1 > n ? n - lo : step - 1) : 0;
     }
-    return lo;
+    return __builtin_amdgcn_readfirstlane(min(lo, n));
   }
 };
 
-// eight (16-bit) or four (fp32) consecutive reduction elements k0 + .. of column `col` of a row-major [k][ld] matrix
-template <typename T> __device__ __forceinline__ typename AT<T>::frag column_frag(const T* w, int k0, int kend, long ld, bool live) {
-  constexpr int VEC = ElemTraits<T>::VEC;
-  union { T e[VEC]; typename AT<T>::frag f; } u;
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) u.e[e] = live && k0 + e < kend ? w[(long)(k0 + e) * ld] : from_f<T>(0.f);
-  return u.f;
+// The factors the other way round, for the backward pass: At[a][k][r] = A_a[r][k] and Bt[a][r][n] = B_a[n][r], 64 x 64 elements per workgroup.  (Gathered in place the
+// products' fragments are eight loads each: down's product with dy took 47 us of them at 16384 x 4096, 16 adapter columns, against 30.)
+template <typename T>
+__global__ void __launch_bounds__(256) adapter_turn_kernel(const T* __restrict__ fa, const T* __restrict__ fb, T* __restrict__ ta, T* __restrict__ tb, int K, int N, int R) {
+  __shared__ T tile[64][65];
+  const int rt = (R + 63) / 64, na = rt * ((K + 63) / 64);
+  const bool is_a = (int)blockIdx.x < na;
+  const int n = is_a ? blockIdx.x : blockIdx.x - na, rows = is_a ? R : N, cols = is_a ? K : R;
+  const int ct = (cols + 63) / 64, r0 = n / ct * 64, c0 = n % ct * 64;
+  const long off = (long)blockIdx.y * rows * cols;
+  const T* src = (is_a ? fa : fb) + off;
+  T* dst = (is_a ? ta : tb) + off;
+  const int c = threadIdx.x & 63;
+  for (int r = threadIdx.x >> 6; r < 64; r += 4)
+    if (r0 + r < rows && c0 + c < cols) tile[r][c] = src[(long)(r0 + r) * cols + c0 + c];
+  __syncthreads();
+  for (int r = threadIdx.x >> 6; r < 64; r += 4)
+    if (c0 + r < cols && r0 + c < rows) dst[(long)(c0 + r) * rows + r0 + c] = tile[c][r];
 }
 
-// out[row][r] = scaling[a] * sum_k x[row][k] f_a(r, k);   COLS: f_a(r, k) = f[a][k][r] (B_a), else f[a][r][k] (A_a)
-template <typename T, int NR, bool COLS>
+// out[row][r] = scaling[a] * sum_k x[row][k] f[a][r][k]   (h: f = A; G: f = Bt)
+template <typename T, int NR>
 __global__ void __launch_bounds__(256) adapter_down_kernel(const Segs g, const T* __restrict__ x, const T* __restrict__ f, T* __restrict__ out, int K, int R) {
   constexpr int KD = AT<T>::KD, VEC = ElemTraits<T>::VEC;
   typedef typename AT<T>::frag frag;
   __shared__ f32x4 part[4][NR][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
   const int i0 = blockIdx.x * 16, i1 = min(i0 + 16, g.M);
-  const int s0 = g.first_at(i0);
+  const int s0 = g.first_at(i0, threadIdx.x & 63);
   if (blockIdx.y == 0 && threadIdx.x < 16 * NR) {
     // rows that no adapter's segment holds: zero (their own store below never comes)
     const int row = i0 + (threadIdx.x & 15), c = (threadIdx.x >> 4) * 16;
@@ -84,15 +97,11 @@ __global__ void __launch_bounds__(256) adapter_down_kernel(const Segs g, const T
       for (int n = 0; n < NR; ++n) {
         const int col = 16 * n + r;
         frag ff;
-        if constexpr (COLS) {
-          ff = column_frag<T>(fa + min(col, R - 1), k0, K, R, col < R);
-        } else {
-          ff = zero_frag((frag*)nullptr);
-          if (col < R && k0 < K) {
-            union { V16 v; frag f; } u;
-            u.v = ld16(fa + (long)col * K + k0);
-            ff = u.f;
-          }
+        ff = zero_frag((frag*)nullptr);
+        if (col < R && k0 < K) {
+          union { V16 v; frag f; } u;
+          u.v = ld16(fa + (long)col * K + k0);
+          ff = u.f;
         }
         acc[n] = mma<T>(fx, ff, acc[n]);
       }
@@ -118,8 +127,8 @@ __global__ void __launch_bounds__(256) adapter_down_kernel(const Segs g, const T
   }
 }
 
-// out[i][j] = sum_r h[i][r] f_a(r, j) (0 for rows without an adapter);   COLS: f_a(r, j) = f[a][r][j] (A_a), else f[a][j][r] (B_a)
-template <typename T, bool COLS>
+// out[i][j] = sum_r h[i][r] f[a][j][r], 0 for rows without an adapter   (y's part: f = B; dx's: f = At)
+template <typename T>
 __global__ void __launch_bounds__(256) adapter_up_kernel(const Segs g, const T* __restrict__ h, const T* __restrict__ f, T* __restrict__ out, int N, int R) {
   constexpr int KD = AT<T>::KD, VEC = ElemTraits<T>::VEC;
   typedef typename AT<T>::frag frag;
@@ -129,7 +138,7 @@ __global__ void __launch_bounds__(256) adapter_up_kernel(const Segs g, const T* 
   f32x4 acc[4];
 #pragma unroll
   for (int n = 0; n < 4; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int s = g.first_at(i0); s < g.n; ++s) {
+  for (int s = g.first_at(i0, threadIdx.x & 63); s < g.n; ++s) {
     const int b = max(g.begin(s), i0), e = min(g.begin(s + 1), i1);
     if (g.begin(s) >= i1) break;
     const int a = g.adapter(s);
@@ -148,15 +157,11 @@ __global__ void __launch_bounds__(256) adapter_up_kernel(const Segs g, const T* 
       for (int n = 0; n < 4; ++n) {
         const int col = j0 + 16 * n + r;
         frag ff;
-        if constexpr (COLS) {
-          ff = column_frag<T>(fa + min(col, N - 1), k0, R, N, col < N);
-        } else {
-          ff = zero_frag((frag*)nullptr);
-          if (col < N && k0 < R) {
-            union { V16 v; frag f; } u;
-            u.v = ld16(fa + (long)col * R + k0);
-            ff = u.f;
-          }
+        ff = zero_frag((frag*)nullptr);
+        if (col < N && k0 < R) {
+          union { V16 v; frag f; } u;
+          u.v = ld16(fa + (long)col * R + k0);
+          ff = u.f;
         }
         acc[n] = mma<T>(ff, fh, acc[n]);   // transposed: a lane holds four neighbouring columns of one row
       }
@@ -173,10 +178,119 @@ __global__ void __launch_bounds__(256) adapter_up_kernel(const Segs g, const T* 
   }
 }
 
+// The same products added to a wave's accumulators of the projection's GEMM, between its main loop and its epilogue: one rounding for the whole of y (dx), and
+// no pass over it.
+template <typename T> struct AdapterExtend {
+  static constexpr bool STORES = true;
+  Segs g;
+  const T* h;
+  const T* f;
+  int N, R;
+  // C = acc + bias, 32 rows at a time through LDS so that a row of 64 columns leaves as whole 128-byte lines.  The lanes exchange their values without a barrier of
+  // the workgroup; the wave barriers keep the compiler from letting lanes whose columns lie past N run ahead (that condition is the same in every
+  // pass, and threaded through them it had half of the lanes write all passes before the others read the first).
+  __device__ __forceinline__ void store(const GemmParams& p, const f32x4 (&acc)[4][8], unsigned char* my, int row0, int col0, int lane) const {
+    constexpr int ROW = 64 * 2 + 16;
+    static_assert(32 * ROW <= EPI_WAVE, "a pass fits the wave's room");
+    const int r = lane & 15, q = lane >> 4, col = col0 + 8 * (lane & 7);
+    float b4[4][4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const int j = col0 + 16 * n + 4 * q;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) b4[n][e] = 0.f;
+      if (p.ep.bias && j < p.N) ld4(p.ep.bias + j, b4[n]);
+    }
+    unsigned char* wp = my + r * ROW + 8 * q;
+    const unsigned char* lp = my + (lane >> 3) * ROW + (lane & 7) * 16;
+#pragma unroll
+    for (int h2 = 0; h2 < 4; ++h2) {
+#pragma unroll
+      for (int mm = 0; mm < 2; ++mm)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const f32x4& a = acc[n][2 * h2 + mm];
+          uint2 pk;
+          pk.x = pack2<T>(a[0] + b4[n][0], a[1] + b4[n][1]);
+          pk.y = pack2<T>(a[2] + b4[n][2], a[3] + b4[n][3]);
+          *reinterpret_cast<uint2*>(wp + mm * 16 * ROW + n * 32) = pk;
+        }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      V16 v[4];
+#pragma unroll
+      for (int it = 0; it < 4; ++it) v[it] = ld16(lp + it * 8 * ROW);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int it = 0; it < 4; ++it) {
+        const int row = row0 + 32 * h2 + 8 * it + (lane >> 3);
+        if (row < p.M && col < p.N) st16(reinterpret_cast<T*>(p.C) + (long)row * p.ldc + col, v[it]);
+      }
+    }
+  }
+  __device__ __forceinline__ bf16x8 row_frag(int row, int b, int e, int k0) const {
+    bf16x8 fh = zero_frag((bf16x8*)nullptr);
+    if (row >= b && row < e && k0 < R) fh = *reinterpret_cast<const bf16x8*>(h + (long)row * R + k0);
+    return fh;
+  }
+  template <int NN, int NM> __device__ __forceinline__ void operator()(f32x4 (&acc)[NN][NM], int row0, int col0, int lane) const {
+    // nothing below may be computed in front of the main loop and held across it: that loop counts its vector-memory operations, so it may not spill
+    asm volatile("" : "+v"(lane));
+    row0 = __builtin_amdgcn_readfirstlane(row0);
+    col0 = __builtin_amdgcn_readfirstlane(col0);
+    asm volatile("" : "+s"(row0), "+s"(col0));
+    const int r = lane & 15, q = lane >> 4, row1 = min(row0 + 16 * NM, g.M);
+    if (row0 >= g.M || col0 >= N) return;
+    for (int s = g.first_at(row0, lane); s < g.n; ++s) {
+      const int b = max(g.begin(s), row0), e = min(g.begin(s + 1), row1);
+      if (g.begin(s) >= row1) break;
+      const int a = g.adapter(s);
+      if (b >= e || a < 0) continue;
+      const T* fa = f + (long)a * N * R;
+      for (int k = 0; k < R; k += 32) {
+        const int k0 = k + 8 * q;
+        bf16x8 ff[NN];
+#pragma unroll
+        for (int n = 0; n < NN; ++n) {
+          const int col = col0 + 16 * n + r;
+          ff[n] = zero_frag((bf16x8*)nullptr);
+          if (col < N && k0 < R) ff[n] = *reinterpret_cast<const bf16x8*>(fa + (long)col * R + k0);
+        }
+#pragma unroll
+        for (int m = 0; m < NM; ++m) {
+          if (b >= row0 + 16 * m + 16 || e <= row0 + 16 * m) continue;
+          const bf16x8 fh = row_frag(row0 + 16 * m + r, b, e, k0);
+#pragma unroll
+          for (int n = 0; n < NN; ++n) acc[n][m] = mfma16<T>(ff[n], fh, acc[n][m]);
+        }
+      }
+    }
+  }
+};
+// The launch's parameters with everything that a plain X W^T + bias leaves unused as constants: the loops' epilogues fold to what is left.
+__device__ __forceinline__ GemmParams plain_product(const GemmParams& a) {
+  GemmParams p = a;
+  GemmEpilogue& e = p.ep;
+  e.alpha = 1.f; e.bias_gstride = 0; e.bias_mod = 0; e.preact = nullptr; e.act = FH_ACT_NONE; e.drop.p = 0.f; e.gelu_aux = nullptr; e.residual = nullptr;
+  e.row_len = nullptr; e.out_f32 = 0; e.atomic = 0; e.idiv = e.jdiv = 0; e.si1 = e.si0 = e.sj1 = e.sj0 = 0; e.tail_cols = 0; e.aux_factor = 0;
+  e.kd_teacher = nullptr; e.c0_wpart = nullptr;
+  return p;
+}
+template <typename T, int YL> __global__ void __launch_bounds__(512) adapter_gemm_kernel(const GemmParams a, const AdapterExtend<T> ext) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  gemm_8ph_tile<T, FH_R_CONTIG, YL, false, AdapterExtend<T>>(a, lds, logical_block(1), 1, 0, ext);
+}
+template <typename T> __global__ void __launch_bounds__(256) adapter_gemm_small_kernel(const GemmParams a, const AdapterExtend<T> ext) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  const GemmParams p = plain_product(a);
+  gemm_small_tile<T, AdapterExtend<T>>(p, lds, ext);
+}
+
 // dst[a][r][c] (BY_ROW) or dst[a][c][r] = sum over the rows of adapter a of u[row][r] v[row][c];  with several splits: partial sums
 // [split][a] .. in the same layout
-template <typename T, int NR, bool BY_ROW>
-__global__ void __launch_bounds__(256) adapter_outer_kernel(const Segs g, const T* __restrict__ u, const T* __restrict__ v, float* __restrict__ dst, int C, int R) {
+template <typename T, int NR, bool BY_ROW, typename O>
+__global__ void __launch_bounds__(256) adapter_outer_kernel(const Segs g, const T* __restrict__ u, const T* __restrict__ v, O* __restrict__ dst, int C, int R) {
   constexpr int VEC = ElemTraits<T>::VEC, ES = sizeof(T);
   constexpr int RU = NR * 16 * ES + 16, RV = 64 * ES + 16;           // LDS row strides
   constexpr int PER = 32 * (RU + RV), SUM = NR * 4 * 64 * 16;        // a wave's tiles; one wave's sums at the end
@@ -292,7 +406,7 @@ __global__ void __launch_bounds__(256) adapter_outer_kernel(const Segs g, const 
     }
   }
   __syncthreads();
-  float* d = dst + ((long)split * g.adapters + a) * C * R;
+  O* d = dst + ((long)split * g.adapters + a) * C * R;
   for (int t = wave; t < NR * 4; t += 4) {
     const int n = t >> 2, m = t & 3;
     const f32x4 o = sum[t * 64 + lane];
@@ -307,10 +421,11 @@ __global__ void __launch_bounds__(256) adapter_outer_kernel(const Segs g, const 
   }
 }
 
-__global__ void __launch_bounds__(256) adapter_join_kernel(const float* __restrict__ part, float* __restrict__ dst, long n4, int splits) {
+template <typename T> __global__ void __launch_bounds__(256) adapter_join_kernel(const float* __restrict__ part, T* __restrict__ dst, long n4, int splits) {
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
   if (i >= n4) return;
   float s[4] = {0.f, 0.f, 0.f, 0.f}, f[4];
+#pragma unroll 4
   for (int k = 0; k < splits; ++k) {
     ld4(part + ((long)k * n4 + i) * 4, f);
 #pragma unroll
@@ -347,12 +462,17 @@ size_t outer_bytes(const fh_adapter_desc* d, int C) {
   return n > 1 ? al16((size_t)n * d->n_adapters * C * d->R * 4) : 0;
 }
 
-template <typename T, bool COLS> int down(const Segs& g, const void* x, const void* f, void* out, int K, int R, hipStream_t st) {
+size_t partial_bytes(const fh_adapter_desc* d) {
+  const size_t pa = outer_bytes(d, d->K), pb = outer_bytes(d, d->N);
+  return pa > pb ? pa : pb;
+}
+
+template <typename T> int down(const Segs& g, const void* x, const void* f, void* out, int K, int R, hipStream_t st) {
   if (g.M == 0) return 0;
   const int tiles = (g.M + 15) / 16;
   const long per = 1 + ((long)16 * g.n + g.M - 1) / g.M;   // segments that a tile touches
   const dim3 grid(tiles, per > 16 ? 16 : (int)per), block(256);
-#define FH_DOWN(NR) hipLaunchKernelGGL((adapter_down_kernel<T, NR, COLS>), grid, block, 0, st, g, (const T*)x, (const T*)f, (T*)out, K, R)
+#define FH_DOWN(NR) hipLaunchKernelGGL((adapter_down_kernel<T, NR>), grid, block, 0, st, g, (const T*)x, (const T*)f, (T*)out, K, R)
   if (R <= 16) FH_DOWN(1);
   else if (R <= 32) FH_DOWN(2);
   else if (R <= 64) FH_DOWN(4);
@@ -361,62 +481,91 @@ template <typename T, bool COLS> int down(const Segs& g, const void* x, const vo
   FH_CHECK_LAUNCH();
   return 0;
 }
-template <typename T, bool COLS> int up(const Segs& g, const void* h, const void* f, void* out, int N, int R, hipStream_t st) {
-  hipLaunchKernelGGL((adapter_up_kernel<T, COLS>), dim3((g.M + 15) / 16, (N + 255) / 256), dim3(256), 0, st, g, (const T*)h, (const T*)f, (T*)out, N, R);
+template <typename T> int up(const Segs& g, const void* h, const void* f, void* out, int N, int R, hipStream_t st) {
+  hipLaunchKernelGGL((adapter_up_kernel<T>), dim3((g.M + 15) / 16, (N + 255) / 256), dim3(256), 0, st, g, (const T*)h, (const T*)f, (T*)out, N, R);
   FH_CHECK_LAUNCH();
   return 0;
 }
-template <typename T, bool BY_ROW> int outer(const fh_adapter_desc* d, const void* u, const void* v, float* dst, int C, float* part, hipStream_t st) {
+template <typename T, bool BY_ROW> int outer(const fh_adapter_desc* d, const void* u, const void* v, void* dst, int C, float* part, hipStream_t st) {
   const Segs g = segs_of(d);
   const int n = outer_splits(d, C), R = d->R;
-  float* to = n > 1 ? part : dst;
   const dim3 grid((C + 63) / 64, d->n_adapters, n), block(256);
-#define FH_OUTER(NR) hipLaunchKernelGGL((adapter_outer_kernel<T, NR, BY_ROW>), grid, block, 0, st, g, (const T*)u, (const T*)v, to, C, R)
-  if (R <= 16) FH_OUTER(1);
-  else if (R <= 32) FH_OUTER(2);
-  else if (R <= 64) FH_OUTER(4);
-  else FH_OUTER(8);
+#define FH_OUTER(NR)                                                                                                                                \
+  {                                                                                                                                                 \
+    if (n > 1) hipLaunchKernelGGL((adapter_outer_kernel<T, NR, BY_ROW, float>), grid, block, 0, st, g, (const T*)u, (const T*)v, part, C, R);        \
+    else hipLaunchKernelGGL((adapter_outer_kernel<T, NR, BY_ROW, T>), grid, block, 0, st, g, (const T*)u, (const T*)v, (T*)dst, C, R);               \
+  }
+  if (R <= 16) FH_OUTER(1) else if (R <= 32) FH_OUTER(2) else if (R <= 64) FH_OUTER(4) else FH_OUTER(8)
 #undef FH_OUTER
   FH_CHECK_LAUNCH();
   if (n > 1) {
     const long n4 = (long)d->n_adapters * C * R / 4;
-    hipLaunchKernelGGL(adapter_join_kernel, dim3((unsigned)((n4 + 255) / 256)), dim3(256), 0, st, part, dst, n4, n);
+    hipLaunchKernelGGL((adapter_join_kernel<T>), dim3((unsigned)((n4 + 255) / 256)), dim3(256), 0, st, part, (T*)dst, n4, n);
     FH_CHECK_LAUNCH();
   }
   return 0;
 }
 
+// The projection's product with the adapters' part.  16-bit: inside the GEMM, on the 256 x 256 8-phase loop where its tiles give work to a good part of the CUs, on
+// the 64 x 64 one-trip loop otherwise (forward only: it takes W by its rows); else, and in fp32, the part goes first and is the GEMM's residual.
+template <typename T, int YL>
+int project(int dtype, const fh_adapter_desc* d, GemmParams& p, const void* h, const void* f, hipStream_t st) {
+  const Segs g = segs_of(d);
+  if constexpr (sizeof(T) == 2) {
+    const AdapterExtend<T> ext{g, (const T*)h, (const T*)f, p.N, d->R};
+    const int tiles = ((p.M + 255) / 256) * ((p.N + 255) / 256);
+    if (tiles >= 96 && p.Kseg >= 128) {
+      const size_t smem = 131072;
+      if (int rc = (int)hipFuncSetAttribute((const void*)adapter_gemm_kernel<T, YL>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return rc;
+      hipLaunchKernelGGL((adapter_gemm_kernel<T, YL>), dim3(tiles), dim3(512), smem, st, p, ext);
+      FH_CHECK_LAUNCH();
+      return 0;
+    }
+    if constexpr (YL == FH_R_CONTIG) {
+      const size_t smem = 2 * (size_t)64 * 512 * 2;
+      if (int rc = (int)hipFuncSetAttribute((const void*)adapter_gemm_small_kernel<T>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return rc;
+      hipLaunchKernelGGL((adapter_gemm_small_kernel<T>), dim3(((p.M + 63) / 64) * ((p.N + 63) / 64)), dim3(256), smem, st, p, ext);
+      FH_CHECK_LAUNCH();
+      return 0;
+    }
+  }
+  if (int rc = up<T>(g, h, f, p.C, p.N, d->R, st)) return rc;
+  p.ep.residual = p.C;
+  return fh_gemm_launch(p, dtype, st);
+}
+
 template <typename T>
 int forward_t(int dtype, const fh_adapter_desc* d, const void* x, const void* w, const float* bias, const void* a, const void* b, void* h, void* y, hipStream_t st) {
-  const Segs g = segs_of(d);
-  if (int rc = down<T, false>(g, x, a, h, d->K, d->R, st)) return rc;
-  if (int rc = up<T, false>(g, h, b, y, d->N, d->R, st)) return rc;
+  if (int rc = down<T>(segs_of(d), x, a, h, d->K, d->R, st)) return rc;
   GemmParams p = fh_gemm_params();
   p.X = fh_operand(x, FH_R_CONTIG, d->K);
   p.Y = fh_operand(w, FH_R_CONTIG, d->K);
   p.C = y;
   p.M = d->M; p.N = d->N; p.Kseg = d->K; p.ldc = d->N;
   p.ep.bias = bias;
-  p.ep.residual = y;
-  return fh_gemm_launch(p, dtype, st);
+  return project<T, FH_R_CONTIG>(dtype, d, p, h, b, st);
 }
 template <typename T>
 int backward_t(int dtype, const fh_adapter_desc* d, const void* x, const void* w, const void* a, const void* b, const void* h, const void* dy, void* dx,
-               float* da, float* db, char* scratch, hipStream_t st) {
-  const Segs g = segs_of(d);
+               void* da, void* db, char* scratch, hipStream_t st) {
   T* G = (T*)scratch;
   float* part = (float*)(scratch + al16((size_t)d->M * d->R * sizeof(T)));
-  if (dx || da)
-    if (int rc = down<T, true>(g, dy, b, G, d->N, d->R, st)) return rc;
+  T* at = (T*)((char*)part + partial_bytes(d));
+  T* bt = at + (long)d->n_adapters * d->K * d->R;
+  if ((dx || da) && d->M > 0) {
+    const int rt = (d->R + 63) / 64;
+    hipLaunchKernelGGL((adapter_turn_kernel<T>), dim3(rt * ((d->K + 63) / 64 + (d->N + 63) / 64), d->n_adapters), dim3(256), 0, st, (const T*)a, (const T*)b, at, bt, d->K,
+                       d->N, d->R);
+    FH_CHECK_LAUNCH();
+    if (int rc = down<T>(segs_of(d), dy, bt, G, d->N, d->R, st)) return rc;
+  }
   if (dx && d->M > 0) {
-    if (int rc = up<T, true>(g, G, a, dx, d->K, d->R, st)) return rc;
     GemmParams p = fh_gemm_params();
     p.X = fh_operand(dy, FH_R_CONTIG, d->N);
     p.Y = fh_operand(w, FH_R_STRIDED, d->K);
     p.C = dx;
     p.M = d->M; p.N = d->K; p.Kseg = d->N; p.ldc = d->K;
-    p.ep.residual = dx;
-    if (int rc = fh_gemm_launch(p, dtype, st)) return rc;
+    if (int rc = project<T, FH_R_STRIDED>(dtype, d, p, G, at, st)) return rc;
   }
   if (da)
     if (int rc = outer<T, true>(d, G, x, da, d->K, part, st)) return rc;
@@ -432,8 +581,7 @@ extern "C" {
 long fh_adapter_scratch_bytes(int dtype, const fh_adapter_desc* d, int backward) {
   if (check(dtype, d)) return -1;
   if (!backward) return 0;
-  const size_t pa = outer_bytes(d, d->K), pb = outer_bytes(d, d->N);
-  return (long)(al16((size_t)d->M * d->R * fh_esize(dtype)) + (pa > pb ? pa : pb));
+  return (long)(al16((size_t)d->M * d->R * fh_esize(dtype)) + partial_bytes(d) + (size_t)d->n_adapters * d->R * ((size_t)d->K + d->N) * fh_esize(dtype));
 }
 
 int fh_adapter_linear_forward(int dtype, const fh_adapter_desc* d, const void* x, const void* w, const float* bias, const void* a, const void* b,
@@ -450,10 +598,10 @@ int fh_adapter_linear_forward(int dtype, const fh_adapter_desc* d, const void* x
 }
 
 int fh_adapter_linear_backward(int dtype, const fh_adapter_desc* d, const void* x, const void* w, const void* a, const void* b, const void* h,
-                               const void* dy, void* dx, float* da, float* db, void* scratch, fh_stream_t stream) {
+                               const void* dy, void* dx, void* da, void* db, void* scratch, fh_stream_t stream) {
   if (int rc = check(dtype, d)) return rc;
   if (!dx && !da && !db) return 0;
-  if (d->M > 0 && (!dy || ((dx || da) && !b) || (dx && (!w || !a)) || (da && !x) || (db && !h) || !scratch)) return -946;
+  if (d->M > 0 && (!dy || ((dx || da) && (!a || !b)) || (dx && !w) || (da && !x) || (db && !h) || !scratch)) return -946;
   if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)a | (uintptr_t)b | (uintptr_t)h | (uintptr_t)dy | (uintptr_t)dx | (uintptr_t)da | (uintptr_t)db | (uintptr_t)scratch) & 15)
     return -947;
   const hipStream_t st = (hipStream_t)stream;

@@ -1485,6 +1485,14 @@ __global__ void __launch_bounds__(WM* WN * 64, WM * WN == 4 ? 2 : 1) gemm_ring_k
   }
 }
 
+// What may still be added to a wave's accumulators behind the main loop: ext(acc [n tiles][m tiles], first row, first column, lane), called by every wave with all
+// its lanes (adapters.hip: the low-rank products of the rows' adapters).  On the 256-tile loop such a launch stores its tile itself:
+// ext.store(p, acc, EPI_WAVE bytes of LDS for this wave, first row, first column, lane).
+struct NoExtend {
+  static constexpr bool STORES = false;
+  template <typename ACC> __device__ __forceinline__ void operator()(ACC&, int, int, int) const {}
+};
+
 // ------------------------------------------------------------------ small-M loop (R_CONTIG x R_CONTIG): the whole reduction in one trip
 // At the reference's own batch (3 utterances per GPU: M = 747 rows per layer GEMM) a launch has a few dozen tiles and its time
 // is the LATENCY of its K loop: 7.5 dependent load -> LDS -> MFMA steps of ~2.5 us each = 22-27 us for 30 MFLOP, 110 such launches
@@ -1492,10 +1500,9 @@ __global__ void __launch_bounds__(WM* WN * 64, WM * WN == 4 ? 2 : 1) gemm_ring_k
 // operand) into LDS with one burst of LDS-DMA -- one memory round trip --, then runs all its MFMAs back to back; wave w owns the
 // 16-column strip w (4 accumulators), the operand image and fragment reads are the ring loaders'.  ~4x more tiles than the
 // 128-tile loops (so the few rows spread over the CUs) and ~3x shorter per launch.
-template <typename H>
-__global__ void __launch_bounds__(256) gemm_small_kernel(const GemmParams p) {
+template <typename H, typename EXT = NoExtend>
+__device__ __forceinline__ void gemm_small_tile(const GemmParams& p, unsigned char* lds, const EXT& ext = EXT()) {
   typedef RingLoader<FH_R_CONTIG, 64, 512, 4> LD;
-  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int g = blockIdx.z;
   const int tiles_j = (p.N + 63) / 64;
@@ -1528,7 +1535,13 @@ __global__ void __launch_bounds__(256) gemm_small_kernel(const GemmParams p) {
       }
       __syncthreads();  // the tiles are rewritten by the next pass
     }
+  ext(acc, i0, j0 + 16 * wave, lane);
   gemm_epilogue<H, 1, 4>(p, acc, i0, j0, 0, 16 * wave, lane, g);
+}
+template <typename H>
+__global__ void __launch_bounds__(256) gemm_small_kernel(const GemmParams p) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  gemm_small_tile<H>(p, lds);
 }
 bool small_ok(const GemmParams& p) {
   return p.X.layout == FH_R_CONTIG && p.Y.layout == FH_R_CONTIG && !p.ep.atomic && (p.splitk & 0xffff) <= 1;
@@ -1958,8 +1971,8 @@ template <> struct QuarterLoader<FH_R_STRIDED> {
 
 
 // one 256 x 256 output tile (logical tile lb, reduction split lblk.split of nsplit) of the 8-phase loop
-template <typename H, int XL, int YL, bool KD = false>
-__device__ __forceinline__ void gemm_8ph_tile(const GemmParams& p, unsigned char* lds, const LogicalBlock lblk, int nsplit, int g) {
+template <typename H, int XL, int YL, bool KD = false, typename EXT = NoExtend>
+__device__ __forceinline__ void gemm_8ph_tile(const GemmParams& p, unsigned char* lds, const LogicalBlock lblk, int nsplit, int g, const EXT& ext = EXT()) {
   constexpr int BK_ = 64, XT = 256 * 64 * 2, STAGE = 2 * XT;
   constexpr int RA = XL == FH_R_STRIDED ? 16 : 8, RB = YL == FH_R_STRIDED ? 8 : 4;  // LDS reads of an A / B fragment phase
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -2077,6 +2090,11 @@ __device__ __forceinline__ void gemm_8ph_tile(const GemmParams& p, unsigned char
   if (!late) __builtin_amdgcn_s_barrier();
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
   unsigned char* my = lds + wave * EPI_WAVE;
+  if constexpr (EXT::STORES) {
+    ext(acc, i0 + xi0, j0 + yj0, lane);
+    ext.store(p, acc, my, i0 + xi0, j0 + yj0, lane);
+    return;
+  }
   const int r = lane & 15, q = lane >> 4;
   if (epilogue_bf16<H, 8, KD>(p, acc, 0, my, i0, j0, xi0, yj0, lane, g)) return;
   float bv[8];

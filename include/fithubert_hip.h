@@ -296,8 +296,8 @@ int fh_window_attention_backward(int dtype, const fh_window_attention_desc* d, c
  * Segment s is the rows [seg_start[s], seg_start[s + 1]) (device, n_segments + 1 values, ascending; clipped to [0, M]); seg_adapter[s] outside
  * [0, n_adapters), rows in front of the first and behind the last segment: the shared projection alone.  Several segments may name one
  * adapter.  h [M][R] (dtype) receives scaling[a] x A_a^T, 0 on rows without an adapter: what the backward reads.
- * Backward (W and bias are frozen): dx = dy W + G A_a with G = scaling[a] dy B_a; da = sum G^T x; db = sum dy^T h -- da, db fp32, written, 0
- * for an adapter without rows.  dx, da or db may be NULL.  16-bit modes round h and G to the element type, sums are fp32; no atomics.
+ * Backward (W and bias are frozen): dx = dy W + G A_a with G = scaling[a] dy B_a; da = sum G^T x; db = sum dy^T h -- in the element type,
+ * written, 0 for an adapter without rows.  dx, da or db may be NULL.  16-bit modes round h and G to the element type, sums are fp32; no atomics.
  * K, N, R multiples of 8, R <= 128; every tensor contiguous and 16-byte aligned.
  * scratch: fh_adapter_scratch_bytes(dtype, d, 0 forward | 1 backward) bytes, 16-byte aligned (0: NULL will do).
  * ------------------------------------------------------------------------------------------ */
@@ -311,7 +311,7 @@ long fh_adapter_scratch_bytes(int dtype, const fh_adapter_desc* d, int backward)
 int fh_adapter_linear_forward(int dtype, const fh_adapter_desc* d, const void* x, const void* w, const float* bias, const void* a, const void* b,
                               void* h, void* y, void* scratch, fh_stream_t stream);
 int fh_adapter_linear_backward(int dtype, const fh_adapter_desc* d, const void* x, const void* w, const void* a, const void* b, const void* h,
-                               const void* dy, void* dx, float* da, float* db, void* scratch, fh_stream_t stream);
+                               const void* dy, void* dx, void* da, void* db, void* scratch, fh_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------
  * Layer-wise KD loss + gradient (train.py:250-293,372-378):  out[l] = mean_{b,t,d} f(pred_l - teacher_{tl[l]}),

@@ -87,7 +87,11 @@ def check(s):
     (515, 136, 1000, 32, 5, [0, 250, 515], [7, 1]),                                     # a number that is no adapter's
     (700, 96, 104, 40, 70, [10 * i for i in range(71)], list(range(70))),
     (2100, 480, 480, 16, 2, [0, 1500, 2100], [0, 1]),
-    (1000, 1024, 256, 8, 1, [0], [])])                                                   # no request at all
+    (1000, 1024, 256, 8, 1, [0], []),
+    # the 256-tile loop: rows and columns that end inside a tile, a wave's rows, 64 columns
+    (9973, 480, 1440, 8, 12, [0, 82, 327, 736, 4900, 9900], [1, 6, -1, 11, 4]),
+    (2561, 136, 2568, 24, 3, [100, 1000, 2000, 2550], [0, 2, 1]),
+    (6200, 1448, 1096, 40, 2, [0, 3100, 6200], [1, 0])])                                                   # no request at all
 def test_forward_and_backward(dtype, M, K, N, R, n, start, which):
     check(make(M + K, dtype, M, K, N, R, n, start, which, bias=M % 2 == 0))
 
