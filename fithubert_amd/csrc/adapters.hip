@@ -48,78 +48,92 @@ __global__ void __launch_bounds__(256) adapter_turn_kernel(const T* __restrict__
   const T* src = (is_a ? fa : fb) + off;
   T* dst = (is_a ? ta : tb) + off;
   const int c = threadIdx.x & 63;
-  for (int r = threadIdx.x >> 6; r < 64; r += 4)
-    if (r0 + r < rows && c0 + c < cols) tile[r][c] = src[(long)(r0 + r) * cols + c0 + c];
+  T v[16];   // (all loads in flight at once; those past the edge repeat the last row or column and are not stored)
+  const T* at = src + min(c0 + c, cols - 1);
+#pragma unroll
+  for (int u = 0; u < 16; ++u) v[u] = at[(long)min(r0 + (int)(threadIdx.x >> 6) + 4 * u, rows - 1) * cols];
+#pragma unroll
+  for (int u = 0; u < 16; ++u) tile[(threadIdx.x >> 6) + 4 * u][c] = v[u];
   __syncthreads();
   for (int r = threadIdx.x >> 6; r < 64; r += 4)
     if (c0 + r < cols && r0 + c < rows) dst[(long)(c0 + r) * rows + r0 + c] = tile[c][r];
 }
 
-// out[row][r] = scaling[a] * sum_k x[row][k] f[a][r][k]   (h: f = A; G: f = Bt)
-template <typename T, int NR>
+// out[row][r] = scaling[a] * sum_k x[row][k] f[a][r][k]   (h: f = A; G: f = Bt).  RT 16-row tiles per workgroup share the reads of f; a wave takes 128 bytes of
+// every row at a time.
+template <typename T, int NR, int RT>
 __global__ void __launch_bounds__(256) adapter_down_kernel(const Segs g, const T* __restrict__ x, const T* __restrict__ f, T* __restrict__ out, int K, int R) {
   constexpr int KD = AT<T>::KD, VEC = ElemTraits<T>::VEC;
   typedef typename AT<T>::frag frag;
-  __shared__ f32x4 part[4][NR][64];
+  __shared__ f32x4 part[4][NR * RT][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
-  const int i0 = blockIdx.x * 16, i1 = min(i0 + 16, g.M);
-  const int s0 = g.first_at(i0, threadIdx.x & 63);
-  if (blockIdx.y == 0 && threadIdx.x < 16 * NR) {
+  const int i0 = blockIdx.x * 16 * RT, i1 = min(i0 + 16 * RT, g.M);
+  const int s0 = g.first_at(i0, lane);
+  if (blockIdx.y == 0) {
     // rows that no adapter's segment holds: zero (their own store below never comes)
-    const int row = i0 + (threadIdx.x & 15), c = (threadIdx.x >> 4) * 16;
-    if (row < i1) {
+    for (int n = threadIdx.x; n < 16 * RT * NR; n += 256) {
+      const int row = i0 + n % (16 * RT), c = n / (16 * RT) * 16;
+      if (row >= i1) continue;
       int s = s0;
       while (s < g.n && g.start[s + 1] <= row) ++s;
       if (s >= g.n || g.start[s] > row || g.adapter(s) < 0)
         for (int j = c; j < min(c + 16, R); ++j) out[(long)row * R + j] = from_f<T>(0.f);
     }
   }
+  auto piece = [](const T* p, bool live) {
+    union { V16 v; frag f; } u;
+    u.v = v16_zero();
+    if (live) u.v = ld16(p);
+    return u.f;
+  };
   for (int s = s0 + (int)blockIdx.y; s < g.n; s += (int)gridDim.y) {
     const int b = max(g.begin(s), i0), e = min(g.begin(s + 1), i1);
     if (g.begin(s) >= i1) break;
     const int a = g.adapter(s);
     if (b >= e || a < 0) continue;
     const T* fa = f + (long)a * K * R;
-    const T* xr = x + (long)min(i0 + r, g.M - 1) * K;
-    f32x4 acc[NR];
+    const T* xr[RT];
 #pragma unroll
-    for (int n = 0; n < NR; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < RT; ++t) xr[t] = x + (long)min(i0 + 16 * t + r, g.M - 1) * K;
+    f32x4 acc[NR][RT];
+#pragma unroll
+    for (int n = 0; n < NR; ++n)
+#pragma unroll
+      for (int t = 0; t < RT; ++t) acc[n][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 2
-    for (int k = wave * KD; k < K; k += 4 * KD) {
-      const int k0 = k + VEC * q;
-      frag fx = zero_frag((frag*)nullptr);
-      if (k0 < K) {
-        union { V16 v; frag f; } u;
-        u.v = ld16(xr + k0);
-        fx = u.f;
+    for (int k = wave * 2 * KD; k < K; k += 8 * KD) {
+      frag fx[2][RT], ff[2][NR];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int k0 = k + u * KD + VEC * q;
+#pragma unroll
+        for (int t = 0; t < RT; ++t) fx[u][t] = piece(xr[t] + k0, k0 < K);
+#pragma unroll
+        for (int n = 0; n < NR; ++n) ff[u][n] = piece(fa + (long)(16 * n + r) * K + k0, 16 * n + r < R && k0 < K);
       }
 #pragma unroll
-      for (int n = 0; n < NR; ++n) {
-        const int col = 16 * n + r;
-        frag ff;
-        ff = zero_frag((frag*)nullptr);
-        if (col < R && k0 < K) {
-          union { V16 v; frag f; } u;
-          u.v = ld16(fa + (long)col * K + k0);
-          ff = u.f;
-        }
-        acc[n] = mma<T>(fx, ff, acc[n]);
-      }
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+          for (int t = 0; t < RT; ++t) acc[n][t] = mma<T>(fx[u][t], ff[u][n], acc[n][t]);
     }
 #pragma unroll
-    for (int n = 0; n < NR; ++n) part[wave][n][lane] = acc[n];
+    for (int n = 0; n < NR; ++n)
+#pragma unroll
+      for (int t = 0; t < RT; ++t) part[wave][n * RT + t][lane] = acc[n][t];
     __syncthreads();
     const float sc = g.scaling[a];
-    for (int n = wave; n < NR; n += 4) {
-      f32x4 v = part[0][n][lane];
+    for (int m = wave; m < NR * RT; m += 4) {
+      f32x4 v = part[0][m][lane];
 #pragma unroll
       for (int w = 1; w < 4; ++w)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) v[c] += part[w][n][lane][c];
-      const int col = 16 * n + r;
+        for (int c = 0; c < 4; ++c) v[c] += part[w][m][lane][c];
+      const int col = 16 * (m / RT) + r;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const int row = i0 + 4 * q + c;
+        const int row = i0 + 16 * (m % RT) + 4 * q + c;
         if (row >= b && row < e && col < R) out[(long)row * R + col] = from_f<T>(v[c] * sc);   // rounded to the element type: the next product's operand
       }
     }
@@ -163,7 +177,10 @@ __global__ void __launch_bounds__(256) adapter_up_kernel(const Segs g, const T* 
           u.v = ld16(fa + (long)col * R + k0);
           ff = u.f;
         }
-        acc[n] = mma<T>(ff, fh, acc[n]);   // transposed: a lane holds four neighbouring columns of one row
+        // transposed: a lane holds four neighbouring columns of one row; rows of other requests keep their sum (a zero times this adapter's infinity would reach them)
+        const f32x4 t = mma<T>(ff, fh, acc[n]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[n][c] = mine ? t[c] : acc[n][c];
       }
     }
   }
@@ -229,9 +246,10 @@ template <typename T> struct AdapterExtend {
       }
     }
   }
-  __device__ __forceinline__ bf16x8 row_frag(int row, int b, int e, int k0) const {
-    bf16x8 fh = zero_frag((bf16x8*)nullptr);
-    if (row >= b && row < e && k0 < R) fh = *reinterpret_cast<const bf16x8*>(h + (long)row * R + k0);
+  typedef typename AT<T>::frag frag;
+  __device__ __forceinline__ frag row_frag(int row, int b, int e, int k0) const {
+    frag fh = zero_frag((frag*)nullptr);
+    if (row >= b && row < e && k0 < R) fh = *reinterpret_cast<const frag*>(h + (long)row * R + k0);
     return fh;
   }
   template <int NN, int NM> __device__ __forceinline__ void operator()(f32x4 (&acc)[NN][NM], int row0, int col0, int lane) const {
@@ -248,21 +266,27 @@ template <typename T> struct AdapterExtend {
       const int a = g.adapter(s);
       if (b >= e || a < 0) continue;
       const T* fa = f + (long)a * N * R;
-      for (int k = 0; k < R; k += 32) {
-        const int k0 = k + 8 * q;
-        bf16x8 ff[NN];
+      for (int k = 0; k < R; k += AT<T>::KD) {
+        const int k0 = k + ElemTraits<T>::VEC * q;
+        frag ff[NN];
 #pragma unroll
         for (int n = 0; n < NN; ++n) {
           const int col = col0 + 16 * n + r;
-          ff[n] = zero_frag((bf16x8*)nullptr);
-          if (col < N && k0 < R) ff[n] = *reinterpret_cast<const bf16x8*>(fa + (long)col * R + k0);
+          ff[n] = zero_frag((frag*)nullptr);
+          if (col < N && k0 < R) ff[n] = *reinterpret_cast<const frag*>(fa + (long)col * R + k0);
         }
 #pragma unroll
         for (int m = 0; m < NM; ++m) {
           if (b >= row0 + 16 * m + 16 || e <= row0 + 16 * m) continue;
-          const bf16x8 fh = row_frag(row0 + 16 * m + r, b, e, k0);
+          const int row = row0 + 16 * m + r;
+          const bool mine = row >= b && row < e;   // rows of other requests keep their sum (a zero times this adapter's infinity would reach them)
+          const frag fh = row_frag(row, b, e, k0);
 #pragma unroll
-          for (int n = 0; n < NN; ++n) acc[n][m] = mfma16<T>(ff[n], fh, acc[n][m]);
+          for (int n = 0; n < NN; ++n) {
+            const f32x4 t = mma<T>(ff[n], fh, acc[n][m]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[n][m][c] = mine ? t[c] : acc[n][m][c];
+          }
         }
       }
     }
@@ -285,6 +309,175 @@ template <typename T> __global__ void __launch_bounds__(256) adapter_gemm_small_
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   const GemmParams p = plain_product(a);
   gemm_small_tile<T, AdapterExtend<T>>(p, lds, ext);
+}
+
+// Few rows (a frame of each of some live requests): y whole, in one kernel behind `down`.  A workgroup owns 16 columns of 64 rows; its four waves split K straight from
+// memory into the products' operands -- W is read once, by as many workgroups as N has 16s --, then a thread holds four columns of one row and adds
+// that row's own adapter, whatever the other rows use: a tile of one-row requests costs no walk over them.
+template <typename T>
+__global__ void __launch_bounds__(256) adapter_few_kernel(const Segs g, const T* __restrict__ x, const T* __restrict__ w, const float* __restrict__ bias,
+                                                          const T* __restrict__ h, const T* __restrict__ f, T* __restrict__ y, int K, int N, int R) {
+  constexpr int KD = AT<T>::KD, VEC = ElemTraits<T>::VEC;
+  typedef typename AT<T>::frag frag;
+  __shared__ f32x4 part[4][4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+  const int i0 = blockIdx.y * 64, j0 = blockIdx.x * 16, mt = min(4, (g.M - i0 + 15) >> 4);
+  // the adapter of this thread's row in the end (row tile `wave`, row r): the segments' ends 64 at a time, one count per row
+  const int row = i0 + 16 * wave + r, seg0 = g.first_at(min(i0 + 16 * wave, g.M), lane);
+  int mine = seg0;
+  for (int s = seg0; s < g.n; s += 64) {
+    const int end = s + lane < g.n ? g.start[s + lane + 1] : 0x7fffffff;
+    bool more = false;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const int passed = __popcll(__ballot(end <= i0 + 16 * wave + k));
+      if (k == r) mine += passed;
+      more = passed == 64;
+    }
+    if (!more) break;
+  }
+  const int a = row < g.M && mine < g.n && g.start[mine] <= row ? g.adapter(mine) : -1;
+  f32x4 acc[4];
+#pragma unroll
+  for (int m = 0; m < 4; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const T* wr = w + (long)min(j0 + r, N - 1) * K;
+  const T* xr[4];
+#pragma unroll
+  for (int m = 0; m < 4; ++m) xr[m] = x + (long)min(i0 + 16 * m + r, g.M - 1) * K;
+#pragma unroll 2
+  for (int k = wave * 2 * KD; k < K; k += 8 * KD) {
+    frag fw[2], fx[2][4];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int k0 = k + u * KD + VEC * q;
+      fw[u] = zero_frag((frag*)nullptr);
+      if (k0 < K) fw[u] = *reinterpret_cast<const frag*>(wr + k0);
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        fx[u][m] = zero_frag((frag*)nullptr);
+        if (m < mt && k0 < K) fx[u][m] = *reinterpret_cast<const frag*>(xr[m] + k0);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int m = 0; m < 4; ++m)
+        if (m < mt) acc[m] = mma<T>(fw[u], fx[u][m], acc[m]);
+  }
+#pragma unroll
+  for (int m = 0; m < 4; ++m) part[wave][m][lane] = acc[m];
+  __syncthreads();
+  const int j = j0 + 4 * q;
+  if (row >= g.M || j >= N) return;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] += part[k][wave][lane][e];
+  if (bias) {
+    float b4[4];
+    ld4(bias + j, b4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] += b4[e];
+  }
+  if (a >= 0) {
+    const T* fa = f + ((long)a * N + j) * R;
+    const T* hr = h + (long)row * R;
+    for (int k = 0; k < R; k += VEC) {
+      float hv[VEC], fv[VEC];
+      unpack16<T>(ld16(hr + k), hv);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        unpack16<T>(ld16(fa + (long)e * R + k), fv);
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) v[e] = fmaf(hv[c], fv[c], v[e]);
+      }
+    }
+  }
+  st4(y + (long)row * N + j, v);
+}
+
+// fp32: C = X Y^T (+ bias) with the adapters' part, 64 x 64 per workgroup, 32 of the reduction at a time through two LDS buffers; a wave owns 32 x 32.  YL = FH_R_STRIDED: Y is read by
+// its columns (dx: W[n][k] with the reduction over n) and turned on its way into LDS.  (The library's 128 x 128 fp32 loop with the part as residual: a
+// 1497 x 480 x 480 product is 48 workgroups of it and took 52 us.)
+template <int YL>
+__global__ void __launch_bounds__(256) adapter_gemm_f32_kernel(const float* __restrict__ X, const float* __restrict__ Y, const float* __restrict__ bias, float* __restrict__ C,
+                                                               int M, int N, int K, long ldy, const AdapterExtend<float> ext) {
+  constexpr int BK = 32, ROW = BK + 4;
+  __shared__ __attribute__((aligned(16))) float lds[2][2][64 * ROW];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, q = lane >> 4;
+  const int tj_n = (N + 63) / 64, lb = xcd_remap(blockIdx.x, gridDim.x), ti = lb / tj_n, i0 = ti * 64, j0 = (lb - ti * tj_n) * 64;
+  const int wi = (wave >> 1) * 32, wj = (wave & 1) * 32;
+  f32x4 px[2], py[2];
+  auto fetch = [&](int k0) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int n = tid + 256 * u, row = n >> 3, k = k0 + (n & 7) * 4;
+      px[u] = py[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (i0 + row < M && k < K) px[u] = *reinterpret_cast<const f32x4*>(X + (long)(i0 + row) * K + k);
+      if constexpr (YL == FH_R_CONTIG) {
+        if (j0 + row < N && k < K) py[u] = *reinterpret_cast<const f32x4*>(Y + (long)(j0 + row) * ldy + k);
+      } else {
+        const int kr = k0 + (n >> 4), j = j0 + (n & 15) * 4;
+        if (kr < K && j < N) py[u] = *reinterpret_cast<const f32x4*>(Y + (long)kr * ldy + j);
+      }
+    }
+  };
+  auto deposit = [&](int buf) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int n = tid + 256 * u;
+      *reinterpret_cast<f32x4*>(&lds[buf][0][(n >> 3) * ROW + (n & 7) * 4]) = px[u];
+      if constexpr (YL == FH_R_CONTIG) {
+        *reinterpret_cast<f32x4*>(&lds[buf][1][(n >> 3) * ROW + (n & 7) * 4]) = py[u];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) lds[buf][1][((n & 15) * 4 + e) * ROW + (n >> 4)] = py[u][e];
+      }
+    }
+  };
+  f32x4 acc[2][2];
+#pragma unroll
+  for (int n = 0; n < 2; ++n)
+#pragma unroll
+    for (int m = 0; m < 2; ++m) acc[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  fetch(0);
+  int buf = 0;
+  for (int k0 = 0; k0 < K; k0 += BK, buf ^= 1) {
+    deposit(buf);   // (its readers of two steps ago have passed the barrier of the step in between)
+    __syncthreads();
+    if (k0 + BK < K) fetch(k0 + BK);
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      f32x4 fx[2], fy[2];
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        fx[m] = *reinterpret_cast<const f32x4*>(&lds[buf][0][(wi + 16 * m + r) * ROW + ks * 16 + 4 * q]);
+        fy[m] = *reinterpret_cast<const f32x4*>(&lds[buf][1][(wj + 16 * m + r) * ROW + ks * 16 + 4 * q]);
+      }
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int m = 0; m < 2; ++m) acc[n][m] = mma<float>(fy[n], fx[m], acc[n][m]);
+    }
+  }
+  ext(acc, i0 + wi, j0 + wj, lane);
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    const int j = j0 + wj + 16 * n + 4 * q;
+    if (j >= N) continue;
+    float b4[4] = {0.f, 0.f, 0.f, 0.f};
+    if (bias) ld4(bias + j, b4);
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      const int row = i0 + wi + 16 * m + r;
+      if (row >= M) continue;
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = acc[n][m][e] + b4[e];
+      st4(C + (long)row * N + j, v);
+    }
+  }
 }
 
 // dst[a][r][c] (BY_ROW) or dst[a][c][r] = sum over the rows of adapter a of u[row][r] v[row][c];  with several splits: partial sums
@@ -469,14 +662,16 @@ size_t partial_bytes(const fh_adapter_desc* d) {
 
 template <typename T> int down(const Segs& g, const void* x, const void* f, void* out, int K, int R, hipStream_t st) {
   if (g.M == 0) return 0;
-  const int tiles = (g.M + 15) / 16;
-  const long per = 1 + ((long)16 * g.n + g.M - 1) / g.M;   // segments that a tile touches
+  // 32-row tiles where they still fill the chip twice over and requests are long enough to share them (16384 x 4096, rank 16: 50 -> 36 us)
+  const bool wide = g.M >= 16384 && R <= 64 && (long)g.n * 64 <= g.M;
+  const int tile = wide ? 32 : 16, tiles = (g.M + tile - 1) / tile;
+  const long per = 1 + ((long)tile * g.n + g.M - 1) / g.M;   // segments that a tile touches
   const dim3 grid(tiles, per > 16 ? 16 : (int)per), block(256);
-#define FH_DOWN(NR) hipLaunchKernelGGL((adapter_down_kernel<T, NR>), grid, block, 0, st, g, (const T*)x, (const T*)f, (T*)out, K, R)
-  if (R <= 16) FH_DOWN(1);
-  else if (R <= 32) FH_DOWN(2);
-  else if (R <= 64) FH_DOWN(4);
-  else FH_DOWN(8);
+#define FH_DOWN(NR, RT) hipLaunchKernelGGL((adapter_down_kernel<T, NR, RT>), grid, block, 0, st, g, (const T*)x, (const T*)f, (T*)out, K, R)
+  if (R <= 16) { if (wide) FH_DOWN(1, 2); else FH_DOWN(1, 1); }
+  else if (R <= 32) { if (wide) FH_DOWN(2, 2); else FH_DOWN(2, 1); }
+  else if (R <= 64) { if (wide) FH_DOWN(4, 2); else FH_DOWN(4, 1); }
+  else FH_DOWN(8, 1);
 #undef FH_DOWN
   FH_CHECK_LAUNCH();
   return 0;
@@ -506,27 +701,51 @@ template <typename T, bool BY_ROW> int outer(const fh_adapter_desc* d, const voi
   return 0;
 }
 
-// The projection's product with the adapters' part.  16-bit: inside the GEMM, on the 256 x 256 8-phase loop where its tiles give work to a good part of the CUs, on
-// the 64 x 64 one-trip loop otherwise (forward only: it takes W by its rows); else, and in fp32, the part goes first and is the GEMM's residual.
+// The projection's product with the adapters' part:
+//   few rows (forward)        adapter_few_kernel, by its number of workgroups: with the whole of h's kernel, bf16 and rank 16, us against the next line's:
+//                             1 x 480 -> 1440 7.2 | 18, 256 x 4096 -> 1024 35 | 44 (256 workgroups), 512 x 480 -> 1440 12.7 | 12.4 (720), 512 x 1024 -> 4096 48 | 35
+//                             (2048), but 56 | 56 with one-row requests; fp32: 512 x 4096 -> 1024 98 | 131 (512), 1024 x 768 -> 768 36 | 33 (768)
+//   requests under 16 rows    the part on its own first (16-row tiles, many of them), then the GEMM's residual operand: a large tile would walk its requests one by one
+//   fp32                      adapter_gemm_f32_kernel
+//   16-bit                    inside the GEMM: the 256 x 256 8-phase loop where its tiles give work to a good part of the CUs, else the 64 x 64 one-trip loop (it takes W by
+//                             its rows: forward only; a small backward goes as short requests do)
 template <typename T, int YL>
 int project(int dtype, const fh_adapter_desc* d, GemmParams& p, const void* h, const void* f, hipStream_t st) {
   const Segs g = segs_of(d);
-  if constexpr (sizeof(T) == 2) {
-    const AdapterExtend<T> ext{g, (const T*)h, (const T*)f, p.N, d->R};
-    const int tiles = ((p.M + 255) / 256) * ((p.N + 255) / 256);
-    if (tiles >= 96 && p.Kseg >= 128) {
-      const size_t smem = 131072;
-      if (int rc = (int)hipFuncSetAttribute((const void*)adapter_gemm_kernel<T, YL>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return rc;
-      hipLaunchKernelGGL((adapter_gemm_kernel<T, YL>), dim3(tiles), dim3(512), smem, st, p, ext);
-      FH_CHECK_LAUNCH();
-      return 0;
-    }
-    if constexpr (YL == FH_R_CONTIG) {
-      const size_t smem = 2 * (size_t)64 * 512 * 2;
-      if (int rc = (int)hipFuncSetAttribute((const void*)adapter_gemm_small_kernel<T>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return rc;
-      hipLaunchKernelGGL((adapter_gemm_small_kernel<T>), dim3(((p.M + 63) / 64) * ((p.N + 63) / 64)), dim3(256), smem, st, p, ext);
-      FH_CHECK_LAUNCH();
-      return 0;
+  const AdapterExtend<T> ext{g, (const T*)h, (const T*)f, p.N, d->R};
+  const bool brief = (long)d->n_segments * 16 > p.M;
+  const long few = (long)((p.M + 63) / 64) * ((p.N + 15) / 16);
+  if (YL == FH_R_CONTIG && few <= (brief ? 2048 : sizeof(T) == 4 ? 512 : 400)) {
+    hipLaunchKernelGGL((adapter_few_kernel<T>), dim3((p.N + 15) / 16, (p.M + 63) / 64), dim3(256), 0, st, g, (const T*)p.X.p, (const T*)p.Y.p, p.ep.bias, (const T*)h, (const T*)f,
+                       (T*)p.C, p.Kseg, p.N, d->R);
+    FH_CHECK_LAUNCH();
+    return 0;
+  }
+  if (!brief) {
+    if constexpr (sizeof(T) == 4) {
+      const long tiles = (long)((p.M + 63) / 64) * ((p.N + 63) / 64);
+      if (tiles <= 0x7fffffffL) {
+        hipLaunchKernelGGL((adapter_gemm_f32_kernel<YL>), dim3((unsigned)tiles), dim3(256), 0, st, (const float*)p.X.p, (const float*)p.Y.p, p.ep.bias, (float*)p.C, p.M, p.N,
+                           p.Kseg, p.Y.ld, ext);
+        FH_CHECK_LAUNCH();
+        return 0;
+      }
+    } else {
+      const long tiles = (long)((p.M + 255) / 256) * ((p.N + 255) / 256);
+      if (tiles >= 96 && tiles <= 0x7fffffffL && p.Kseg >= 128) {
+        const size_t smem = 131072;
+        if (int rc = (int)hipFuncSetAttribute((const void*)adapter_gemm_kernel<T, YL>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return rc;
+        hipLaunchKernelGGL((adapter_gemm_kernel<T, YL>), dim3((unsigned)tiles), dim3(512), smem, st, p, ext);
+        FH_CHECK_LAUNCH();
+        return 0;
+      }
+      if constexpr (YL == FH_R_CONTIG) {
+        const size_t smem = 2 * (size_t)64 * 512 * 2;
+        if (int rc = (int)hipFuncSetAttribute((const void*)adapter_gemm_small_kernel<T>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return rc;
+        hipLaunchKernelGGL((adapter_gemm_small_kernel<T>), dim3(((p.M + 63) / 64) * ((p.N + 63) / 64)), dim3(256), smem, st, p, ext);
+        FH_CHECK_LAUNCH();
+        return 0;
+      }
     }
   }
   if (int rc = up<T>(g, h, f, p.C, p.N, d->R, st)) return rc;

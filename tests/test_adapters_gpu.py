@@ -3,7 +3,7 @@
 Tolerances are elementwise (u = eps / 2 of the element type; a sum of n products in fp32 is off by at most n 2^-24 of the sum of their magnitudes):
   h, G   (K or N) 2^-24 of their magnitude sums + u |h|, and the scaling's own rounding 2^-24
   y, dx  n 2^-24 of the magnitude sum of both products + the error of h (G) times |B| (|A|) + u |y|; the adapter's part may be rounded once on its
-         way to the sum: + u |part|
+         way to the sum (short requests): + u |part|
   da, db rows 2^-24 of the magnitude sum + the error of G (h) times |x| (|dy|); rounded once to the factor's type: + u
 fp16 adds half its smallest spacing, 2^-25, to every rounded value."""
 import pytest
@@ -88,6 +88,9 @@ def check(s):
     (700, 96, 104, 40, 70, [10 * i for i in range(71)], list(range(70))),
     (2100, 480, 480, 16, 2, [0, 1500, 2100], [0, 1]),
     (1000, 1024, 256, 8, 1, [0], []),
+    (513, 72, 200, 16, 4, [0, 300, 513], [3, 0]),                                        # behind the few-row kernel's last row
+    (511, 200, 72, 8, 70, [7 * i for i in range(74)], list(range(73))),                  # more than 64 requests in it
+    (17000, 72, 40, 56, 3, [0, 5000, 5001, 16990], [1, 0, 2]),                          # 32-row tiles
     # the 256-tile loop: rows and columns that end inside a tile, a wave's rows, 64 columns
     (9973, 480, 1440, 8, 12, [0, 82, 327, 736, 4900, 9900], [1, 6, -1, 11, 4]),
     (2561, 136, 2568, 24, 3, [100, 1000, 2000, 2550], [0, 2, 1]),
@@ -142,6 +145,23 @@ def test_padding_rows_may_be_anything():
         assert torch.equal(got["y"][:30], want["y"][:30]) and torch.equal(got["da"], want["da"]) and torch.equal(got["db"], want["db"])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K,N,start", [(90, 64, 96, [0, 37, 80]), (900, 64, 96, [0, 437, 880]), (900, 64, 96, [10 * i for i in range(91)]), (9000, 136, 1096, [0, 4437, 8880])])
+def test_an_adapter_of_infinities_stays_with_its_own_rows(dtype, M, K, N, start):
+    s = make(11, dtype, M, K, N, 16, 2, start, [i % 2 for i in range(len(start) - 1)])
+    want = run(s)
+    theirs = torch.ones(M, dtype=torch.bool, device=DEV)
+    for i, (b, e) in enumerate(zip(start, start[1:])):
+        theirs[b:e] = i % 2 == 0
+    for n in ("a", "b"):
+        for bad in (float("nan"), float("inf")):
+            t = dict(s, **{n: s[n].clone()})
+            t[n][1] = bad
+            got = run(t)
+            assert torch.equal(got["y"][theirs], want["y"][theirs]) and torch.equal(got["dx"][theirs], want["dx"][theirs])
+            assert torch.equal(got["da"][0], want["da"][0]) and torch.equal(got["db"][0], want["db"][0])
+
+
 def test_gradients_against_differences():
     s = make(9, torch.float32, 50, 48, 56, 8, 2, [0, 21, 50], [0, 1])
     got = run(s)
@@ -182,3 +202,4 @@ def test_equal_calls_give_equal_bits_on_any_stream_and_captured():
     g.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(run(s)[n], t) for n, t in zip(("y", "dx", "da", "db"), (y,) + grads))
+
