@@ -69,8 +69,9 @@ class _AdapterLinear(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, a, b, scaling, start, which, h = ctx.saved_tensors
         dt, dev = _DT[x.dtype], x.device
+        x, weight, a, b, h, dy = (_dense(t) for t in (x, weight, a, b, h, dy))   # (saved-tensor hooks may give back other strides)
+        scaling, start, which = scaling.contiguous(), start.contiguous(), which.contiguous()
         d = _desc(x, a, weight.shape[0], scaling, start, which)
-        dy = _dense(dy)
         need = ctx.needs_input_grad
         dx = torch.empty_like(x) if need[0] else None
         da = torch.empty_like(a) if need[3] else None

@@ -21,10 +21,17 @@ _DT = {torch.float32: L.DT_F32, torch.bfloat16: L.DT_BF16, torch.float16: L.DT_F
 def _aligned(t: torch.Tensor) -> torch.Tensor:
     """t itself where the kernels can read it in place: channels contiguous, address and strides multiples of 16 bytes, frames and heads at most 2^23 elements
     apart (strides of axes of length 1 do not count); a contiguous copy otherwise"""
+    if t.is_contiguous() and t.data_ptr() % 16 == 0 and t.shape[2] * t.shape[3] <= 1 << 23:
+        return t
     vec = 16 // t.element_size()
     if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % vec == 0 and (s <= 1 << 23 or not i) for i, (s, n) in enumerate(zip(t.stride()[:-1], t.shape[:-1])) if n > 1):
         return t
     return t.clone(memory_format=torch.contiguous_format)
+
+
+def _dense(t: torch.Tensor) -> torch.Tensor:
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def _per_entry(x, B: int, dev: torch.device, name: str) -> Optional[torch.Tensor]:
@@ -34,7 +41,9 @@ def _per_entry(x, B: int, dev: torch.device, name: str) -> Optional[torch.Tensor
         return torch.full((B,), int(x), dtype=torch.int32, device=dev)
     if x.dim() != 1 or x.shape[0] != B or x.dtype.is_floating_point or x.dtype == torch.bool:
         raise ValueError(f"{name}: one integer per entry ({B}), got {tuple(x.shape)} {x.dtype}")
-    return x if x.dtype == torch.int32 and x.device == dev and x.is_contiguous() else x.to(device=dev, dtype=torch.int32).contiguous()
+    if x.dtype == torch.int32 and x.device == dev and x.is_contiguous():
+        return x
+    return x.to(device=dev).clamp(-(1 << 31), (1 << 31) - 1).to(torch.int32).contiguous() if x.dtype == torch.int64 else x.to(device=dev, dtype=torch.int32).contiguous()
 
 
 def _desc(q, k, v, left, right, sinks, scale, key_len, q_start) -> L.WindowAttentionC:
@@ -71,18 +80,17 @@ class _WindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, key_len, q_start, d):
         out, lse = _forward(q, k, v, d, True)
-        ctx.save_for_backward(q, k, v, out, lse, key_len, q_start)   # (d holds addresses: what they belong to lives as long)
-        ctx.d = d
+        ctx.save_for_backward(q, k, v, out, lse, key_len, q_start)
+        ctx.limits = d.left, d.right, d.sinks, d.scale   # (not d: what saved-tensor hooks give back has addresses and strides of its own)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse, _, _ = ctx.saved_tensors
-        dt, dev, d = _DT[q.dtype], q.device, ctx.d
-        dout = dout.contiguous()
-        if dout.data_ptr() % 16:
-            dout = dout.clone()
+        q, k, v, out, lse, key_len, q_start = ctx.saved_tensors
+        dt, dev = _DT[q.dtype], q.device
+        q, k, v, out, lse, dout = _aligned(q), _aligned(k), _aligned(v), _dense(out), _dense(lse), _dense(dout)
+        d = _desc(q, k, v, *ctx.limits, key_len, q_start)
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
         with torch.cuda.device(dev):
             scratch = _scratch(dt, d, 1, dev)

@@ -203,3 +203,15 @@ def test_equal_calls_give_equal_bits_on_any_stream_and_captured():
     torch.cuda.synchronize()
     assert all(torch.equal(run(s)[n], t) for n, t in zip(("y", "dx", "da", "db"), (y,) + grads))
 
+
+def test_saved_tensors_that_come_back_elsewhere():
+    """Activations parked in host memory between the passes, and hooks that give back other strides."""
+    s = make(12, torch.bfloat16, 90, 64, 96, 16, 2, [0, 37, 80], [1, 0])
+    want = run(s)
+    other = lambda t: torch.empty((2,) + t.shape, dtype=t.dtype, device=t.device).permute(*range(1, t.dim() + 1), 0)[..., 0].copy_(t)  # noqa: E731
+    for hooks in (torch.autograd.graph.save_on_cpu(), torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), other)):
+        x, a, b = (s[n].detach().requires_grad_(True) for n in ("x", "a", "b"))
+        with hooks:
+            y = adapter_linear(x, s["weight"], s["bias"], a, b, s["scaling"], s["start"].clone(), s["which"].clone())
+        got = torch.autograd.grad(y, (x, a, b), s["dy"])
+        assert all(torch.equal(want[n], t) for n, t in zip(("dx", "da", "db"), got))

@@ -264,3 +264,24 @@ def test_a_cache_past_32_bit_offsets():
     value, bound = reference(q[2:], tail, tail, None, torch.ones(1, 1, 512, dtype=torch.bool, device=DEV), dh ** -0.5)["out"]
     near("out", got[2:], value, bound)
     assert (got[:2] == 0).all()
+
+
+def test_saved_tensors_that_come_back_elsewhere():
+    """Activations parked in host memory between the passes, and hooks that give back other strides."""
+    q, k, v, dout = inputs(21, torch.bfloat16, 2, 70, 70, 4, 2, 64, packed=True)
+    at = dict(left=9, right=3, sinks=2)
+    want = run(q, k, v, dout, key_len=torch.tensor([70, 31], device=DEV), q_start=torch.tensor([0, 2], device=DEV), **at)
+    other = lambda t: torch.empty((2,) + t.shape, dtype=t.dtype, device=t.device).permute(*range(1, t.dim() + 1), 0)[..., 0].copy_(t)  # noqa: E731
+    for hooks in (torch.autograd.graph.save_on_cpu(), torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), other)):
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        with hooks:
+            out = window_attention(*leaves, key_len=torch.tensor([70, 31], device=DEV), q_start=torch.tensor([0, 2], device=DEV), **at)
+        torch.empty(1000, device=DEV, dtype=torch.int32).fill_(-1)
+        got = torch.autograd.grad(out, leaves, dout)
+        assert all(torch.equal(want[n], t) for n, t in zip(("dq", "dk", "dv"), got))
+
+
+def test_wide_integers_are_limited_not_wrapped():
+    q, k, v, _ = inputs(22, torch.float32, 2, 20, 20, 2, 2, 32)
+    a = window_attention(q, k, v, left=5, right=0, key_len=torch.tensor([2 ** 32 + 7, 20], device=DEV), q_start=torch.tensor([0, 2 ** 32], device=DEV))
+    assert torch.equal(a[0], window_attention(q, k, v, left=5, right=0)[0]) and (a[1] == 0).all()
