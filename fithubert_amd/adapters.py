@@ -45,16 +45,33 @@ def _scratch(dt, d, backward, dev):
     return torch.empty(n, dtype=torch.uint8, device=dev) if n else None
 
 
+_stream = torch._C._cuda_getCurrentRawStream   # (what torch.cuda.current_stream(..).cuda_stream gives, without an object on the way: a call of a few rows is the host's time)
+
+
 def _forward(x, weight, bias, a, b, scaling, start, which):
     dt, dev = _DT[x.dtype], x.device
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return _forward(x, weight, bias, a, b, scaling, start, which)
     d = _desc(x, a, weight.shape[0], scaling, start, which)
-    h = torch.empty(x.shape[0], a.shape[1], dtype=x.dtype, device=dev)
-    y = torch.empty(x.shape[0], weight.shape[0], dtype=x.dtype, device=dev)
-    with torch.cuda.device(dev):
-        scratch = _scratch(dt, d, 0, dev)
-        L.check(L.lib().fh_adapter_linear_forward(dt, C.byref(d), x.data_ptr(), weight.data_ptr(), _ptr(bias), a.data_ptr(), b.data_ptr(), h.data_ptr(), y.data_ptr(),
-                                                  _ptr(scratch), torch.cuda.current_stream(dev).cuda_stream), "fh_adapter_linear_forward")
+    h, y = x.new_empty((d.M, d.R)), x.new_empty((d.M, d.N))
+    scratch = _scratch(dt, d, 0, dev)
+    L.check(L.lib().fh_adapter_linear_forward(dt, C.byref(d), x.data_ptr(), weight.data_ptr(), _ptr(bias), a.data_ptr(), b.data_ptr(), h.data_ptr(), y.data_ptr(),
+                                              _ptr(scratch), _stream(dev.index)), "fh_adapter_linear_forward")
     return y, h
+
+
+def _backward(x, weight, a, b, scaling, start, which, h, dy, need):
+    dt, dev = _DT[x.dtype], x.device
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return _backward(x, weight, a, b, scaling, start, which, h, dy, need)
+    d = _desc(x, a, weight.shape[0], scaling, start, which)
+    dx, da, db = (t.new_empty(t.shape) if n else None for t, n in zip((x, a, b), need))
+    scratch = _scratch(dt, d, 1, dev)
+    L.check(L.lib().fh_adapter_linear_backward(dt, C.byref(d), x.data_ptr(), weight.data_ptr(), a.data_ptr(), b.data_ptr(), h.data_ptr(), dy.data_ptr(),
+                                               _ptr(dx), _ptr(da), _ptr(db), _ptr(scratch), _stream(dev.index)), "fh_adapter_linear_backward")
+    return dx, da, db
 
 
 class _AdapterLinear(torch.autograd.Function):
@@ -68,18 +85,10 @@ class _AdapterLinear(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, weight, a, b, scaling, start, which, h = ctx.saved_tensors
-        dt, dev = _DT[x.dtype], x.device
-        x, weight, a, b, h, dy = (_dense(t) for t in (x, weight, a, b, h, dy))   # (saved-tensor hooks may give back other strides)
-        scaling, start, which = scaling.contiguous(), start.contiguous(), which.contiguous()
-        d = _desc(x, a, weight.shape[0], scaling, start, which)
         need = ctx.needs_input_grad
-        dx = torch.empty_like(x) if need[0] else None
-        da = torch.empty_like(a) if need[3] else None
-        db = torch.empty_like(b) if need[4] else None
-        with torch.cuda.device(dev):
-            scratch = _scratch(dt, d, 1, dev)
-            L.check(L.lib().fh_adapter_linear_backward(dt, C.byref(d), x.data_ptr(), weight.data_ptr(), a.data_ptr(), b.data_ptr(), h.data_ptr(), dy.data_ptr(),
-                                                       _ptr(dx), _ptr(da), _ptr(db), _ptr(scratch), torch.cuda.current_stream(dev).cuda_stream), "fh_adapter_linear_backward")
+        # (saved-tensor hooks may give back other strides)
+        dx, da, db = _backward(_dense(x), _dense(weight), _dense(a), _dense(b), scaling.contiguous(), start.contiguous(), which.contiguous(), _dense(h), _dense(dy),
+                               (need[0], need[3], need[4]))
         return dx, None, None, da, db, None, None, None
 
 

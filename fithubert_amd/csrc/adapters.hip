@@ -480,16 +480,25 @@ __global__ void __launch_bounds__(256) adapter_gemm_f32_kernel(const float* __re
   }
 }
 
-// dst[a][r][c] (BY_ROW) or dst[a][c][r] = sum over the rows of adapter a of u[row][r] v[row][c];  with several splits: partial sums
-// [split][a] .. in the same layout
-template <typename T, int NR, bool BY_ROW, typename O>
-__global__ void __launch_bounds__(256) adapter_outer_kernel(const Segs g, const T* __restrict__ u, const T* __restrict__ v, O* __restrict__ dst, int C, int R) {
+// One gradient's sums: dst[a][r][c] (dA: by row) or dst[a][c][r] (dB) = sum over the rows of adapter a of u[row][r] v[row][c], in `wgs` workgroups per adapter: `splits`
+// of the rows for every 64 columns.  With several splits: partial sums part[split][a] .. in the same layout.
+template <typename T> struct Outer {
+  const T* u;
+  const T* v;
+  T* dst;
+  float* part;
+  int C, splits, wgs;
+};
+template <typename T, int NR, bool BY_ROW>
+__device__ __forceinline__ void outer_sums(const Segs& g, const Outer<T>& o, int wg, int R, unsigned char* lds) {
+  const T* __restrict__ u = o.u;
+  const T* __restrict__ v = o.v;
+  const int C = o.C;
   constexpr int VEC = ElemTraits<T>::VEC, ES = sizeof(T);
   constexpr int RU = NR * 16 * ES + 16, RV = 64 * ES + 16;           // LDS row strides
-  constexpr int PER = 32 * (RU + RV), SUM = NR * 4 * 64 * 16;        // a wave's tiles; one wave's sums at the end
-  __shared__ __attribute__((aligned(16))) unsigned char lds[4 * PER > SUM ? 4 * PER : SUM];
+  constexpr int PER = 32 * (RU + RV);                                // a wave's tiles
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
-  const int c0 = blockIdx.x * 64, a = blockIdx.y, split = blockIdx.z, ways = 4 * (int)gridDim.z;
+  const int split = wg % o.splits, c0 = wg / o.splits * 64, a = blockIdx.y, ways = 4 * o.splits;
   unsigned char* tu = lds + wave * PER;
   unsigned char* tv = tu + 32 * RU;
   f32x4 acc[NR][4];
@@ -599,32 +608,48 @@ __global__ void __launch_bounds__(256) adapter_outer_kernel(const Segs g, const 
     }
   }
   __syncthreads();
-  O* d = dst + ((long)split * g.adapters + a) * C * R;
+  const long at = ((long)split * g.adapters + a) * C * R;
+  auto put = [&](long n, const float* w) {
+    if (o.splits > 1) st4(o.part + at + n, w);
+    else st4(o.dst + at + n, w);
+  };
   for (int t = wave; t < NR * 4; t += 4) {
     const int n = t >> 2, m = t & 3;
-    const f32x4 o = sum[t * 64 + lane];
-    float w[4] = {o[0], o[1], o[2], o[3]};
+    const f32x4 f = sum[t * 64 + lane];
+    const float w[4] = {f[0], f[1], f[2], f[3]};
     if constexpr (BY_ROW) {   // tile rows: columns c, tile columns: r
       const int c = c0 + 16 * m + 4 * q, rr = 16 * n + i;
-      if (c < C && rr < R) st4(d + (long)rr * C + c, w);
+      if (c < C && rr < R) put((long)rr * C + c, w);
     } else {
       const int rr = 16 * n + 4 * q, c = c0 + 16 * m + i;
-      if (c < C && rr < R) st4(d + (long)c * R + rr, w);
+      if (c < C && rr < R) put((long)c * R + rr, w);
     }
   }
 }
 
-template <typename T> __global__ void __launch_bounds__(256) adapter_join_kernel(const float* __restrict__ part, T* __restrict__ dst, long n4, int splits) {
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+// dA's workgroups first, dB's behind them: one launch, so that neither waits for the other's last rows
+template <typename T, int NR>
+__global__ void __launch_bounds__(256) adapter_outer_kernel(const Segs g, const Outer<T> da, const Outer<T> db, int R) {
+  constexpr int PER = 32 * ((NR * 16 + 64) * (int)sizeof(T) + 32), SUM = NR * 4 * 64 * 16;   // (one wave's sums at the end)
+  __shared__ __attribute__((aligned(16))) unsigned char lds[4 * PER > SUM ? 4 * PER : SUM];
+  if ((int)blockIdx.x < da.wgs) outer_sums<T, NR, true>(g, da, blockIdx.x, R, lds);
+  else outer_sums<T, NR, false>(g, db, blockIdx.x - da.wgs, R, lds);
+}
+
+// the splits' sums in their order: na x 256 x 4 elements of dA first, dB behind them
+template <typename T> __global__ void __launch_bounds__(256) adapter_join_kernel(const Outer<T> da, const Outer<T> db, int na, long a4, long b4) {
+  const bool is_a = (int)blockIdx.x < na;
+  const Outer<T>& o = is_a ? da : db;
+  const long n4 = is_a ? a4 : b4, i = (long)((int)blockIdx.x - (is_a ? 0 : na)) * 256 + threadIdx.x;
   if (i >= n4) return;
   float s[4] = {0.f, 0.f, 0.f, 0.f}, f[4];
 #pragma unroll 4
-  for (int k = 0; k < splits; ++k) {
-    ld4(part + ((long)k * n4 + i) * 4, f);
+  for (int k = 0; k < o.splits; ++k) {
+    ld4(o.part + ((long)k * n4 + i) * 4, f);
 #pragma unroll
     for (int e = 0; e < 4; ++e) s[e] += f[e];
   }
-  st4(dst + i * 4, s);
+  st4(o.dst + i * 4, s);
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -655,10 +680,7 @@ size_t outer_bytes(const fh_adapter_desc* d, int C) {
   return n > 1 ? al16((size_t)n * d->n_adapters * C * d->R * 4) : 0;
 }
 
-size_t partial_bytes(const fh_adapter_desc* d) {
-  const size_t pa = outer_bytes(d, d->K), pb = outer_bytes(d, d->N);
-  return pa > pb ? pa : pb;
-}
+size_t partial_bytes(const fh_adapter_desc* d) { return outer_bytes(d, d->K) + outer_bytes(d, d->N); }
 
 template <typename T> int down(const Segs& g, const void* x, const void* f, void* out, int K, int R, hipStream_t st) {
   if (g.M == 0) return 0;
@@ -681,21 +703,24 @@ template <typename T> int up(const Segs& g, const void* h, const void* f, void* 
   FH_CHECK_LAUNCH();
   return 0;
 }
-template <typename T, bool BY_ROW> int outer(const fh_adapter_desc* d, const void* u, const void* v, void* dst, int C, float* part, hipStream_t st) {
+template <typename T> int outer(const fh_adapter_desc* d, const void* G, const void* x, void* da, const void* h, const void* dy, void* db, float* part, hipStream_t st) {
   const Segs g = segs_of(d);
-  const int n = outer_splits(d, C), R = d->R;
-  const dim3 grid((C + 63) / 64, d->n_adapters, n), block(256);
-#define FH_OUTER(NR)                                                                                                                                \
-  {                                                                                                                                                 \
-    if (n > 1) hipLaunchKernelGGL((adapter_outer_kernel<T, NR, BY_ROW, float>), grid, block, 0, st, g, (const T*)u, (const T*)v, part, C, R);        \
-    else hipLaunchKernelGGL((adapter_outer_kernel<T, NR, BY_ROW, T>), grid, block, 0, st, g, (const T*)u, (const T*)v, (T*)dst, C, R);               \
-  }
-  if (R <= 16) FH_OUTER(1) else if (R <= 32) FH_OUTER(2) else if (R <= 64) FH_OUTER(4) else FH_OUTER(8)
-#undef FH_OUTER
+  const int R = d->R;
+  auto side = [&](const void* u, const void* v, void* dst, int C, float* p) {
+    const int n = outer_splits(d, C);
+    return Outer<T>{(const T*)u, (const T*)v, (T*)dst, p, C, n, dst ? (C + 63) / 64 * n : 0};
+  };
+  const Outer<T> a = side(G, x, da, d->K, part), b = side(h, dy, db, d->N, part + outer_bytes(d, d->K) / 4);
+  const dim3 grid(a.wgs + b.wgs, d->n_adapters), block(256);
+  if (R <= 16) hipLaunchKernelGGL((adapter_outer_kernel<T, 1>), grid, block, 0, st, g, a, b, R);
+  else if (R <= 32) hipLaunchKernelGGL((adapter_outer_kernel<T, 2>), grid, block, 0, st, g, a, b, R);
+  else if (R <= 64) hipLaunchKernelGGL((adapter_outer_kernel<T, 4>), grid, block, 0, st, g, a, b, R);
+  else hipLaunchKernelGGL((adapter_outer_kernel<T, 8>), grid, block, 0, st, g, a, b, R);
   FH_CHECK_LAUNCH();
-  if (n > 1) {
-    const long n4 = (long)d->n_adapters * C * R / 4;
-    hipLaunchKernelGGL((adapter_join_kernel<T>), dim3((unsigned)((n4 + 255) / 256)), dim3(256), 0, st, part, (T*)dst, n4, n);
+  auto quads = [&](const Outer<T>& o) { return o.wgs && o.splits > 1 ? (long)d->n_adapters * o.C * R / 4 : 0; };
+  const long a4 = quads(a), b4 = quads(b), na = (a4 + 255) / 256, nb = (b4 + 255) / 256;
+  if (na + nb > 0) {
+    hipLaunchKernelGGL((adapter_join_kernel<T>), dim3((unsigned)(na + nb)), dim3(256), 0, st, a, b, (int)na, a4, b4);
     FH_CHECK_LAUNCH();
   }
   return 0;
@@ -786,10 +811,7 @@ int backward_t(int dtype, const fh_adapter_desc* d, const void* x, const void* w
     p.M = d->M; p.N = d->K; p.Kseg = d->N; p.ldc = d->K;
     if (int rc = project<T, FH_R_STRIDED>(dtype, d, p, G, at, st)) return rc;
   }
-  if (da)
-    if (int rc = outer<T, true>(d, G, x, da, d->K, part, st)) return rc;
-  if (db)
-    if (int rc = outer<T, false>(d, h, dy, db, d->N, part, st)) return rc;
+  if (da || db) return outer<T>(d, G, x, da, h, dy, db, part, st);
   return 0;
 }
 

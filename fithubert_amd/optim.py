@@ -29,7 +29,7 @@ _DT = {torch.float32: L.DT_F32, torch.bfloat16: L.DT_BF16, torch.float16: L.DT_F
 
 def moment_blocks(sizes: Sequence[int]) -> int:
     """blocks of 256 elements that tensors of these sizes take in the flat moments"""
-    return sum((n + BLOCK - 1) // BLOCK for n in sizes)
+    return sum([(n + BLOCK - 1) // BLOCK for n in sizes])
 
 
 def adamw_moments(params: Sequence[torch.Tensor], bits: int = 32) -> List[torch.Tensor]:

@@ -65,15 +65,32 @@ def _ptr(t):
     return t.data_ptr() if t is not None else None
 
 
+_stream = torch._C._cuda_getCurrentRawStream   # (what torch.cuda.current_stream(..).cuda_stream gives, without an object on the way: a call of a few frames is the host's time)
+
+
 def _forward(q, k, v, d, want_lse):
     dt, dev = _DT[q.dtype], q.device
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev) if want_lse else None
-    with torch.cuda.device(dev):
-        scratch = _scratch(dt, d, 0, dev)
-        L.check(L.lib().fh_window_attention_forward(dt, C.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(scratch),
-                                                    torch.cuda.current_stream(dev).cuda_stream), "fh_window_attention_forward")
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return _forward(q, k, v, d, want_lse)
+    out = q.new_empty(q.shape)
+    lse = q.new_empty(q.shape[:3], dtype=torch.float32) if want_lse else None
+    scratch = _scratch(dt, d, 0, dev)
+    L.check(L.lib().fh_window_attention_forward(dt, C.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(scratch), _stream(dev.index)),
+            "fh_window_attention_forward")
     return out, lse
+
+
+def _backward(q, k, v, out, lse, dout, d):
+    dt, dev = _DT[q.dtype], q.device
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return _backward(q, k, v, out, lse, dout, d)
+    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+    scratch = _scratch(dt, d, 1, dev)
+    L.check(L.lib().fh_window_attention_backward(dt, C.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(), lse.data_ptr(), dq.data_ptr(),
+                                                 dk.data_ptr(), dv.data_ptr(), _ptr(scratch), _stream(dev.index)), "fh_window_attention_backward")
+    return dq, dk, dv
 
 
 class _WindowAttention(torch.autograd.Function):
@@ -81,23 +98,19 @@ class _WindowAttention(torch.autograd.Function):
     def forward(ctx, q, k, v, key_len, q_start, d):
         out, lse = _forward(q, k, v, d, True)
         ctx.save_for_backward(q, k, v, out, lse, key_len, q_start)
-        ctx.limits = d.left, d.right, d.sinks, d.scale   # (not d: what saved-tensor hooks give back has addresses and strides of its own)
+        ctx.d, ctx.strides = d, (q.stride(), k.stride(), v.stride())
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse, key_len, q_start = ctx.saved_tensors
-        dt, dev = _DT[q.dtype], q.device
-        q, k, v, out, lse, dout = _aligned(q), _aligned(k), _aligned(v), _dense(out), _dense(lse), _dense(dout)
-        d = _desc(q, k, v, *ctx.limits, key_len, q_start)
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
-        with torch.cuda.device(dev):
-            scratch = _scratch(dt, d, 1, dev)
-            L.check(L.lib().fh_window_attention_backward(dt, C.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(), lse.data_ptr(),
-                                                         dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(scratch), torch.cuda.current_stream(dev).cuda_stream),
-                    "fh_window_attention_backward")
-        return dq, dk, dv, None, None, None
+        q, k, v, d = _aligned(q), _aligned(k), _aligned(v), ctx.d
+        if ctx.strides == (q.stride(), k.stride(), v.stride()):
+            d.key_len, d.q_start = _ptr(key_len), _ptr(q_start)
+        else:   # (saved-tensor hooks may give back tensors with addresses and strides of their own)
+            d = _desc(q, k, v, d.left, d.right, d.sinks, d.scale, key_len, q_start)
+        return _backward(q, k, v, _dense(out), _dense(lse), _dense(dout), d) + (None, None, None)
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, left: int = -1, right: int = -1, sinks: int = 0,
