@@ -292,6 +292,12 @@ __device__ __forceinline__ void softmax_step(const WinArgs& a, f32x4 (&s)[4][RT]
   }
 }
 
+// Where several workgroups share a row block's keys: part[entry][head][share][row][dh] sums, behind them [entry][head][share][row] maximum and sum.
+__device__ __forceinline__ long share_row(const WinArgs& a, int b, int h, int split, int row) { return (((long)b * a.Hkv + h) * a.nsplit + split) * a.rows + row; }
+__device__ __forceinline__ float2* share_stat(const WinArgs& a, float* part, long n) {
+  return reinterpret_cast<float2*>(part + (long)a.B * a.Hkv * a.nsplit * a.rows * a.dh) + n;
+}
+
 template <typename T, int NDT, int RT, bool SPLIT>
 __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_fwd_kernel(const WinArgs a, const T* __restrict__ q_, const T* __restrict__ k_, const T* __restrict__ v_,
                                                           T* __restrict__ out, float* __restrict__ lse, float* __restrict__ part) {
@@ -387,17 +393,13 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_fwd_kernel(const W
     if (row >= a.rows) continue;
     const int i = a.frame(row), g = row - i * a.G;
     if constexpr (SPLIT) {
-      // partial sums of this workgroup's keys: [entry][head][split][row][dh + 2] with the maximum and the sum behind the channels
-      float* dst = part + ((((long)b * a.Hkv + h) * a.nsplit + split) * a.rows + row) * (a.dh + 2);
+      float* dst = part + share_row(a, b, h, split, row) * a.dh;
 #pragma unroll
       for (int dt = 0; dt < NDT; ++dt) {
         const int d = 16 * dt + 4 * q;
-        if (d < a.dh) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) dst[d + e] = o[t][dt][e];
-        }
+        if (d < a.dh) *reinterpret_cast<f32x4*>(dst + d) = o[t][dt];
       }
-      if (q == 0) { dst[a.dh] = m[t]; dst[a.dh + 1] = l[t]; }
+      if (q == 0) *share_stat(a, part, share_row(a, b, h, split, row)) = make_float2(m[t], l[t]);
     } else {
       const float inv = l[t] > 0.f ? 1.0f / l[t] : (l[t] == 0.f ? 0.f : l[t]);   // (NaN stays NaN)
       const long orow = ((long)b * a.Tq + i) * a.Hq + h * a.G + g;
@@ -535,10 +537,9 @@ __global__ void __launch_bounds__(256, NDT * TT * (int)sizeof(T) > 12 ? 1 : 2) w
     }
     if (d >= a.dh) continue;
     if (a.nsplit > 1) {
-      float* dst = part + ((((long)b * a.Hkv + h) * a.nsplit + split) * a.rows + row) * (a.dh + 2);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) dst[d + e] = v[e];
-      if (d == 0) { dst[a.dh] = top; dst[a.dh + 1] = sum; }
+      const long n2 = share_row(a, b, h, split, row);
+      *reinterpret_cast<f32x4*>(part + n2 * a.dh + d) = f32x4{v[0], v[1], v[2], v[3]};
+      if (d == 0) *share_stat(a, part, n2) = make_float2(top, sum);
     } else {
       const float inv = sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);
       const int i = a.frame(row), g = row - i * a.G;
@@ -551,42 +552,46 @@ __global__ void __launch_bounds__(256, NDT * TT * (int)sizeof(T) > 12 ? 1 : 2) w
   }
 }
 
-// joins the partial sums of a row: a workgroup per row, its four waves take every fourth share, a lane two channels
+// Joins the shares of a row (at most 256), a workgroup per row: a thread per share for the weights, then 16 bytes of a share per thread, added over the groups of
+// threads in their order.
 template <typename T>
-__global__ void __launch_bounds__(256) win_join_kernel(const WinArgs a, const float* __restrict__ part, T* __restrict__ out, float* __restrict__ lse) {
-  __shared__ float acc[4][132];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+__global__ void __launch_bounds__(256) win_join_kernel(const WinArgs a, float* __restrict__ part, T* __restrict__ out, float* __restrict__ lse) {
+  __shared__ float weight[256], acc[1024], top[4], total[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const long n = blockIdx.x;                                     // row of [entry][head][row]
   const int row = (int)(n % a.rows);
   const long bh = n / a.rows;
-  const int h = (int)(bh % a.Hkv), b = (int)(bh / a.Hkv), W = a.dh + 2;
-  const float* src = part + (bh * a.nsplit * a.rows + row) * W;
-  const long step = (long)a.rows * W;
-  float m = -INFINITY;
-  for (int s = lane; s < a.nsplit; s += 64) m = fmaxf(m, src[s * step + a.dh]);
-  m = wave_max(m);
-  const float ref = m == -INFINITY ? 0.f : m;
-  const int c = min(2 * lane, a.dh - 2);
-  float l = 0.f, o0 = 0.f, o1 = 0.f;
-#pragma unroll 4
-  for (int s = wave; s < a.nsplit; s += 4) {
-    const float* p = src + s * step;
-    const float w = fast_exp2(p[a.dh] - ref);
-    l += w * p[a.dh + 1];
-    o0 += w * p[c];
-    o1 += w * p[c + 1];
+  const int h = (int)(bh % a.Hkv), b = (int)(bh / a.Hkv), per = a.dh > 64 ? 32 : 16, c = tid % per * 4, first = tid / per, groups = 256 / per;
+  const long at = share_row(a, b, h, 0, row);
+  const float2 st = tid < a.nsplit ? *share_stat(a, part, at + (long)tid * a.rows) : make_float2(-INFINITY, 0.f);
+  const float wm = wave_max(st.x);
+  if (lane == 0) top[wave] = wm;
+  __syncthreads();
+  const float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), ref = m == -INFINITY ? 0.f : m, w = fast_exp2(st.x - ref);
+  weight[tid] = w;
+  const float ws = wave_sum(w * st.y);
+  if (lane == 0) total[wave] = ws;
+  __syncthreads();
+  float o[4] = {0.f, 0.f, 0.f, 0.f};
+  if (c < a.dh) {
+#pragma unroll 8
+    for (int s = first; s < a.nsplit; s += groups) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(part + (at + (long)s * a.rows) * a.dh + c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += weight[s] * x[e];
+    }
   }
-  acc[wave][2 * lane] = o0;
-  acc[wave][2 * lane + 1] = o1;
-  if (lane == 0) acc[wave][128] = l;
+  *reinterpret_cast<f32x4*>(acc + tid * 4) = f32x4{o[0], o[1], o[2], o[3]};
   __syncthreads();
   const int i = a.frame(row), g = row - i * a.G;
   const long orow = ((long)b * a.Tq + i) * a.Hq + h * a.G + g;
-  l = acc[0][128] + acc[1][128] + acc[2][128] + acc[3][128];
-  const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
-  if (threadIdx.x == 0 && lse) lse[orow] = l == 0.f ? INFINITY : m + log2f(l);
-  const int d = threadIdx.x;
-  if (d < a.dh) out[orow * a.dh + d] = from_f<T>((acc[0][d] + acc[1][d] + acc[2][d] + acc[3][d]) * inv);
+  const float l = total[0] + total[1] + total[2] + total[3], inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
+  if (tid == 0 && lse) lse[orow] = l == 0.f ? INFINITY : m + log2f(l);
+  if (tid < a.dh) {
+    float v = 0.f;
+    for (int k = 0; k < groups; ++k) v += acc[k * per * 4 + tid];
+    out[orow * a.dh + tid] = from_f<T>(v * inv);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dq, and D for the other pass
