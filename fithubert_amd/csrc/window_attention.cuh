@@ -735,7 +735,7 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_dq_kernel(const Wi
       if (d < a.dh) {
         float w[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = acc[t][dt][e] * a.scale;
+        for (int e = 0; e < 4; ++e) w[e] = ls[t] == INFINITY ? 0.f : acc[t][dt][e] * a.scale;   // (a row without keys: whatever its gradient holds)
         st4(dq + orow * a.dh + d, w);
       }
     }

@@ -124,7 +124,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, left:
     Query i of entry b stands at position p = ``q_start[b]`` + i (default 0; required as soon as Tq != Tk) and sees key s when s < ``key_len[b]``
     (default Tk), s <= p + ``right`` and (s >= p - ``left`` or s < ``sinks``); a negative ``left`` or ``right`` is no limit.  A row that sees no key
     gives zeros and takes part in no gradient.  Keys that no row of the call sees may hold anything; an infinity or NaN in a key that some rows see
-    may reach rows near them that do not (0 x inf).  ``scale`` > 0, default dh ** -0.5.
+    may reach rows near them that do not (0 x inf), one in a row's query or gradient the gradients of keys near those it sees.  ``scale`` > 0, default dh ** -0.5.
 
     16-bit modes round the probabilities (backward: and dS) to the element type in front of the second products; softmax and sums are fp32.  Nothing
     depends on the order of atomics: equal calls give equal bits."""

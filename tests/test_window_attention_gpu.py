@@ -129,6 +129,23 @@ def test_ragged_lengths_leave_rows_without_keys(dtype, left, right, sinks):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("left,right,sinks", [(20, 0, 0), (3, 9, 0), (-1, 0, 4)])
+def test_rows_without_keys_may_hold_anything(dtype, left, right, sinks):
+    T = 150
+    q, k, v, dout = inputs(8, dtype, 4, T, T, 4, 2, 48)
+    kw = dict(left=left, right=right, sinks=sinks, key_len=torch.tensor([100, 0, 1, 64], device=DEV, dtype=torch.int32), q_start=torch.tensor([0, 3, 0, -20], device=DEV, dtype=torch.int32))
+    empty = ~seen(T, T, kw["key_len"], kw["q_start"], left, right, sinks).any(-1)
+    assert empty[1].all() and empty.sum() > T
+    clean = run(q, k, v, dout, **kw)
+    for bad in (math.nan, math.inf):
+        q2, d2 = q.clone(), dout.clone()
+        q2[empty], d2[empty] = bad, bad
+        dirty = run(q2, k, v, d2, **kw)
+        assert (dirty["out"][empty] == 0).all() and (dirty["dq"][empty] == 0).all()
+        assert all(torch.equal(clean[n], dirty[n]) for n in clean), bad
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_what_no_row_sees_may_be_anything(dtype):
     T = 200
     q, k, v, dout = inputs(3, dtype, 2, T, T, 4, 2, 64)
