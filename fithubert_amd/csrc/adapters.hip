@@ -13,6 +13,9 @@
 #include "kernels.h"
 #include "attn_frag.cuh"
 
+int fh_gemm_path_bf16(const GemmParams& p, int path, hipStream_t stream);  // gemm_bf16.hip
+int fh_gemm_path_f16(const GemmParams& p, int path, hipStream_t stream);   // gemm_f16.hip
+
 namespace {
 
 struct Segs {
@@ -775,7 +778,11 @@ int project(int dtype, const fh_adapter_desc* d, GemmParams& p, const void* h, c
   }
   if (int rc = up<T>(g, h, f, p.C, p.N, d->R, st)) return rc;
   p.ep.residual = p.C;
-  return fh_gemm_launch(p, dtype, st);
+  if constexpr (sizeof(T) == 4) return fh_gemm_launch(p, dtype, st);
+  // The loop that an unmeasured shape takes, without the per-shape table: a measurement would run the launch several times, each on top of the last one's sum, and
+  // the table is not for two threads (a backward pass runs on autograd's).
+  const int loop = p.M >= 4096 && p.N >= 128 && p.Kseg >= 128 ? 8 : 2;
+  return dtype == 2 ? fh_gemm_path_f16(p, loop, st) : fh_gemm_path_bf16(p, loop, st);
 }
 
 template <typename T>

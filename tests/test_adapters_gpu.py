@@ -215,3 +215,16 @@ def test_saved_tensors_that_come_back_elsewhere():
             y = adapter_linear(x, s["weight"], s["bias"], a, b, s["scaling"], s["start"].clone(), s["which"].clone())
         got = torch.autograd.grad(y, (x, a, b), s["dy"])
         assert all(torch.equal(want[n], t) for n, t in zip(("dx", "da", "db"), got))
+
+
+def test_under_the_gemm_tuner():
+    """The tuner runs a launch several times: the sum that lies in the output already must not be taken again."""
+    from fithubert_amd import _lib as L
+    s = make(13, torch.bfloat16, 900, 256, 320, 16, 3, [10 * i for i in range(91)], [i % 3 for i in range(90)])
+    want = run(s)
+    L.lib().fh_gemm_tune(1)
+    try:
+        got = run(s)
+    finally:
+        L.lib().fh_gemm_tune(0)
+    assert all(torch.equal(want[n], got[n]) for n in want)
