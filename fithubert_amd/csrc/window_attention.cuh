@@ -983,6 +983,7 @@ __global__ void __launch_bounds__(256) win_dkv_join_kernel(const WinArgs a, cons
   if (s >= a.Tk) return;
   const float* src = part + (((((long)b * a.Hkv + h) * a.nsink + kb) * a.nsplit * 2 + which) * keys + key) * a.dh + c * 4;
   float sum[4] = {0.f, 0.f, 0.f, 0.f}, f[4];
+#pragma unroll 8
   for (int i = 0; i < a.nsplit; ++i) {
     ld4(src + (long)i * 2 * keys * a.dh, f);
 #pragma unroll
