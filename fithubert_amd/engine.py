@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
-from typing import Dict, List, Optional, Tuple
+from typing import Dict, List, Optional, Tuple, Union
 
 import torch
 
@@ -271,7 +271,7 @@ class StudentEngine:
         """The KD loss can ride in the merged heads' GEMM epilogue (fh_student_forward_kd): layer-wise heads with time reduction."""
         return self.c.n_tasks == 0 and self.c.tr_factor > 0 and bool(heads_on)
 
-    def forward(self, wave: torch.Tensor, sample_lengths=None, training: bool = False, heads_on: bool = True,
+    def forward(self, wave: torch.Tensor, sample_lengths=None, training: Union[bool, int] = False, heads_on: bool = True,
                 seed: int = 0, kd: Optional[dict] = None, keep_fc2_out: bool = True) -> Workspace:
         """``kd`` (training only): dict(teacher=[Lt][B][Tt][P] tensor, layer_w, teacher_layer, loss_type=0, grad_scale=1.0) -- the
         layer-wise KD loss is then computed inside the projection heads' GEMM epilogue: ``ws.kd_out`` holds the fp64 loss vector
@@ -279,9 +279,11 @@ class StudentEngine:
         predictions themselves are never written."""
         assert wave.is_cuda and wave.dtype == torch.float32 and wave.dim() == 2 and wave.is_contiguous()
         B, S = wave.shape
+        # keep_fc2_out=False or training=2 (as fh_student_call.training): the `f2` copies -- layer_results[i][2] of the module API, read by no loss -- are
+        # not stored
+        keep_fc2_out = keep_fc2_out and training != 2
         if training and self.auto_tune and (self._shape_class(B, S) + (bool(heads_on), bool(keep_fc2_out))) not in self._tuned:
             self.autotune(B, S, bool(heads_on), bool(keep_fc2_out))
-        # keep_fc2_out=False (training only): the `f2` copies -- layer_results[i][2] of the module API, read by no loss -- are not stored
         call = StudentCallC(B, S, (1 if keep_fc2_out else 2) if training else 0, int(heads_on), seed & 0xFFFFFFFF)
         nbytes = self.lib.fh_student_ws_bytes(C.byref(self.c), C.byref(call))
         if nbytes <= 0:
