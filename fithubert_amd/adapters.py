@@ -111,7 +111,7 @@ def adapter_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.T
         raise ValueError(f"x [..][K], weight [N][K], lora_a [n][R][K], lora_b [n][N][R]: got {tuple(x.shape)}, {tuple(weight.shape)}, {tuple(lora_a.shape)}, {tuple(lora_b.shape)}")
     if x.dtype not in _DT or any(t.dtype != x.dtype for t in (weight, lora_a, lora_b)):
         raise ValueError(f"x, weight and the factors are fp32, bf16 or fp16, all of one type: got {x.dtype}, {weight.dtype}, {lora_a.dtype}, {lora_b.dtype}")
-    if K % 8 or N % 8 or not 1 <= R <= 128:
+    if K < 8 or N < 8 or K % 8 or N % 8 or not 1 <= R <= 128:
         raise ValueError(f"K {K} and N {N} are multiples of 8, the rank {R} lies in 1 .. 128")
     if scaling.shape != (n,) or scaling.dtype != torch.float32 or (bias is not None and (bias.shape != (N,) or bias.dtype != torch.float32)):
         raise ValueError("scaling [n] and bias [N] are fp32")

@@ -136,3 +136,24 @@ def test_adamw_refuses():
     for bad in (dict(lr=-1.0), dict(betas=(0.9, 1.0)), dict(eps=-1e-8), dict(weight_decay=-0.1)):
         with pytest.raises(ValueError):
             ManyAdamW([torch.zeros(3, requires_grad=True)], **bad)
+
+
+@pytest.mark.parametrize("bad", [dict(q_ts=(1 << 23) + 8), dict(k_hs=(1 << 23) + 8), dict(k_ts=-64), dict(q_bs=-512), dict(Hq=1 << 18, dh=64)])
+def test_window_attention_entries_refuse_strides(bad):
+    lib, d = L.lib(), _win(**bad)
+    assert lib.fh_window_attention_scratch_bytes(1, C.byref(d), 1) == -1
+    assert lib.fh_window_attention_forward(1, C.byref(d), P, P, P, P, None, P, None) < 0
+    assert lib.fh_window_attention_backward(1, C.byref(d), P, P, P, P, P, P, P, P, P, P, None) < 0
+
+
+@pytest.mark.parametrize("K,N", [(0, 24), (16, 0)])
+def test_adapter_linear_refuses_no_channels(K, N):
+    with pytest.raises(ValueError, match="multiples of 8"):
+        adapter_linear(torch.zeros(4, K), torch.zeros(N, K), None, torch.zeros(2, 8, K), torch.zeros(2, N, 8), torch.ones(2), torch.tensor([0, 4], dtype=torch.int32), torch.tensor([0], dtype=torch.int32))
+
+
+def test_window_attention_refuses_limits():
+    q = torch.zeros(2, 5, 4, 16)
+    for kw in (dict(scale=0.0), dict(scale=float("inf")), dict(scale=float("nan"))):
+        with pytest.raises(ValueError):
+            window_attention(q, q, q, **kw)

@@ -228,3 +228,35 @@ def test_under_the_gemm_tuner():
     finally:
         L.lib().fh_gemm_tune(0)
     assert all(torch.equal(want[n], got[n]) for n in want)
+
+
+def test_refusals_on_the_gpu():
+    s = make(14, torch.bfloat16, 20, 64, 64, 8, 2, [0, 20], [1])
+    args = [s[n] for n in ("x", "weight", "bias", "a", "b", "scaling", "start", "which")]
+    for i in (1, 2, 5):                                      # the projection and the scalings are frozen
+        bad = list(args)
+        bad[i] = bad[i].clone().requires_grad_(True)
+        with pytest.raises(ValueError):
+            adapter_linear(*bad)
+        with torch.no_grad():
+            assert torch.equal(adapter_linear(*bad), adapter_linear(*args))
+    for i in (2, 6, 7):                                      # not on the GPU
+        bad = list(args)
+        bad[i] = bad[i].cpu()
+        with pytest.raises(ValueError):
+            adapter_linear(*bad)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_broadcast_inputs_and_one_leaf_twice(dtype):
+    """A row that stands for many, and both factors out of one tensor: the gradients are the sums."""
+    s = make(15, dtype, 40, 64, 64, 8, 2, [0, 20, 40], [1, 0])
+    s["x"] = s["x"][:1].expand(40, -1)
+    s["b"] = s["a"].transpose(1, 2)
+    check(s)
+    row = s["x"][:1].clone().requires_grad_(True)
+    one = s["a"].clone().requires_grad_(True)
+    y = adapter_linear(row.expand(40, -1), s["weight"], s["bias"], one, one.transpose(1, 2), s["scaling"], s["start"], s["which"])
+    dx, da = torch.autograd.grad(y, (row, one), s["dy"])
+    want = run(s)
+    assert torch.equal(dx, want["dx"].sum(0, keepdim=True)) and torch.equal(da, want["da"] + want["db"].transpose(1, 2))

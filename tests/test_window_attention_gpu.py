@@ -303,3 +303,27 @@ def test_wide_integers_are_limited_not_wrapped():
     q, k, v, _ = inputs(22, torch.float32, 2, 20, 20, 2, 2, 32)
     a = window_attention(q, k, v, left=5, right=0, key_len=torch.tensor([2 ** 32 + 7, 20], device=DEV), q_start=torch.tensor([0, 2 ** 32], device=DEV))
     assert torch.equal(a[0], window_attention(q, k, v, left=5, right=0)[0]) and (a[1] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,Tq,Tk", [(0, 7, 7), (2, 0, 9), (2, 70, 0), (2, 3, 0), (0, 0, 0)])
+def test_no_frames(dtype, B, Tq, Tk):
+    q, k, v, dout = inputs(23, dtype, B, Tq, Tk, 4, 2, 32)
+    got = run(q, k, v, dout, left=3, right=0, sinks=2, q_start=0)
+    assert [got[n].shape for n in ("out", "dq", "dk", "dv")] == [q.shape, q.shape, k.shape, v.shape]
+    assert all((got[n] == 0).all() for n in got)
+
+
+def test_refusals_on_the_gpu():
+    q, k, v, _ = inputs(24, torch.bfloat16, 2, 9, 9, 4, 2, 32)
+    for kw in (dict(key_len=torch.tensor([1], device=DEV)), dict(key_len=torch.tensor([1.0, 2.0], device=DEV)), dict(q_start=torch.tensor([[1, 2]], device=DEV))):
+        with pytest.raises(ValueError):
+            window_attention(q, k, v, **kw)
+    with pytest.raises(ValueError):
+        window_attention(q[:, :3], k, v)                     # where do three queries stand among nine keys?
+    with pytest.raises(ValueError):
+        window_attention(q, k.cpu(), v)
+    y = window_attention(q.requires_grad_(True), k, v)
+    g = torch.autograd.grad(y, q, torch.ones_like(y), create_graph=True)[0]
+    with pytest.raises(RuntimeError):                        # no second derivatives
+        torch.autograd.grad(g.sum(), q)
