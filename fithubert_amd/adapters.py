@@ -31,11 +31,8 @@ def _dense(t: torch.Tensor) -> torch.Tensor:
 
 
 def _desc(x, a, N, scaling, start, which) -> L.AdapterC:
-    d = L.AdapterC()
-    d.M, d.K = x.shape
-    d.N, d.R, d.n_adapters, d.n_segments = N, a.shape[1], a.shape[0], which.shape[0]
-    d.seg_start, d.seg_adapter, d.scaling = start.data_ptr(), which.data_ptr(), scaling.data_ptr()
-    return d
+    (M, K), (n, R, _) = x.shape, a.shape
+    return L.AdapterC(M, K, N, R, n, which.shape[0], start.data_ptr(), which.data_ptr(), scaling.data_ptr())
 
 
 def _scratch(dt, d, backward, dev):
@@ -109,7 +106,8 @@ def adapter_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.T
     (N, K), (n, R) = weight.shape, lora_a.shape[:2]
     if x.shape[-1] != K or lora_a.shape != (n, R, K) or lora_b.shape != (n, N, R) or n < 1:
         raise ValueError(f"x [..][K], weight [N][K], lora_a [n][R][K], lora_b [n][N][R]: got {tuple(x.shape)}, {tuple(weight.shape)}, {tuple(lora_a.shape)}, {tuple(lora_b.shape)}")
-    if x.dtype not in _DT or any(t.dtype != x.dtype for t in (weight, lora_a, lora_b)):
+    dt = x.dtype
+    if dt not in _DT or weight.dtype != dt or lora_a.dtype != dt or lora_b.dtype != dt:
         raise ValueError(f"x, weight and the factors are fp32, bf16 or fp16, all of one type: got {x.dtype}, {weight.dtype}, {lora_a.dtype}, {lora_b.dtype}")
     if K < 8 or N < 8 or K % 8 or N % 8 or not 1 <= R <= 128:
         raise ValueError(f"K {K} and N {N} are multiples of 8, the rank {R} lies in 1 .. 128")
@@ -117,17 +115,19 @@ def adapter_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.T
         raise ValueError("scaling [n] and bias [N] are fp32")
     if seg_adapter.dim() != 1 or seg_start.shape != (seg_adapter.shape[0] + 1,) or seg_start.dtype != torch.int32 or seg_adapter.dtype != torch.int32:
         raise ValueError(f"seg_start [requests + 1] and seg_adapter [requests] are int32: got {tuple(seg_start.shape)} {seg_start.dtype}, {tuple(seg_adapter.shape)} {seg_adapter.dtype}")
-    if x.device.type != "cuda" or any(t is not None and t.device != x.device for t in (weight, bias, lora_a, lora_b, scaling, seg_start, seg_adapter)):
+    gpu = x.get_device()   # (-1: not on one)
+    if gpu < 0 or not (weight.get_device() == lora_a.get_device() == lora_b.get_device() == scaling.get_device() == seg_start.get_device() == seg_adapter.get_device() == gpu) \
+            or (bias is not None and bias.get_device() != gpu):
         raise ValueError(f"all tensors live on one GPU (x: {x.device})")
     grad = torch.is_grad_enabled()
-    if grad and any(t is not None and t.requires_grad for t in (weight, bias, scaling)):
+    if grad and (weight.requires_grad or scaling.requires_grad or (bias is not None and bias.requires_grad)):
         raise ValueError("the shared projection and the scalings are frozen: detach weight, bias and scaling")
     if R % 8:
         lora_a, lora_b = F.pad(lora_a, (0, 0, 0, -R % 8)), F.pad(lora_b, (0, -R % 8))
-    flat = _dense(x.reshape(-1, K))
+    flat = _dense(x if x.dim() == 2 else x.reshape(-1, K))
     args = (flat, _dense(weight), _dense(bias) if bias is not None else None, _dense(lora_a), _dense(lora_b), scaling.contiguous(), seg_start.contiguous(), seg_adapter.contiguous())
-    if grad and any(t.requires_grad for t in (x, lora_a, lora_b)):
+    if grad and (x.requires_grad or lora_a.requires_grad or lora_b.requires_grad):
         y = _AdapterLinear.apply(*args)
     else:
         y = _forward(*args)[0]
-    return y.view(*x.shape[:-1], N)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
