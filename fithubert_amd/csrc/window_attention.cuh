@@ -201,6 +201,65 @@ template <typename T, int NDT, int NT> struct Mover {
   }
 };
 
+// The same pair of tiles loaded straight into LDS (16-bit modes: rows without padding), 1 KiB of neighbouring places per wave and load: no registers in between, so that two
+// tiles can be on their way.  Lane i of a load fills the i-th 16 bytes behind the wave's; the twist is in WHICH piece of its row it asks for.
+// (Issued from an asm statement: the compiler neither counts these loads nor drains them in front of LDS reads, `dma_wait` and the barrier order them.)
+typedef __attribute__((address_space(3))) const unsigned char* lds_ptr_t;
+template <typename T, int NDT, int NT> struct Dma {
+  typedef WT<T, NDT> W;
+  static constexpr int CP = W::CP, RP = NT / CP, NP = 64 / RP, LOADS = 2 * NP;
+  static_assert(sizeof(T) == 2 && NT % CP == 0 && RP % 16 == 0 && 64 % RP == 0, "whole passes, one twist per thread");
+  unsigned x_of[NP], y_of[NP], wave0;
+  int row, col;
+  bool live;
+  template <typename F> __device__ __forceinline__ void init(int dh, F&& off) {
+    row = (int)threadIdx.x / CP;
+    col = (((int)threadIdx.x - row * CP) ^ W::twist(row)) * W::VEC;
+    live = col < dh;
+    wave0 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024;
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+      unsigned x, y;
+      off(row + j * RP, x, y);
+      x_of[j] = (x + col) * sizeof(T);
+      y_of[j] = (y + col) * sizeof(T);
+    }
+  }
+  static __device__ __forceinline__ void load(const char* src, unsigned dst) {
+    unsigned keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0" : "=&s"(keep) : "v"(src), "s"(dst) : "memory");
+  }
+  // four bytes per lane
+  static __device__ __forceinline__ void word(const float* src, unsigned dst) {
+    unsigned keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, off\n\ts_mov_b32 m0, %0" : "=&s"(keep) : "v"(src), "s"(dst) : "memory");
+  }
+  // the whole tile whose first rows are x, y to the pair of tiles at `pair`
+  __device__ __forceinline__ void whole(const T* x, const T* y, unsigned pair) const {
+    if (live) {
+#pragma unroll
+      for (int j = 0; j < NP; ++j) {
+        load((const char*)x + x_of[j], pair + wave0 + j * RP * W::RS);
+        load((const char*)y + y_of[j], pair + wave0 + j * RP * W::RS + W::TILE);
+      }
+    }
+  }
+  // at(row, first, second): the addresses of a row's channels in the two tensors
+  template <typename F> __device__ __forceinline__ void rows(F&& at, unsigned pair) const {
+    if (live) {
+#pragma unroll
+      for (int j = 0; j < NP; ++j) {
+        const T *x, *y;
+        at(row + j * RP, x, y);
+        load((const char*)(x + col), pair + wave0 + j * RP * W::RS);
+        load((const char*)(y + col), pair + wave0 + j * RP * W::RS + W::TILE);
+      }
+    }
+  }
+};
+// all of this wave's loads but the N newest are there, and so is what every wave wrote; then the others' too
+template <int N> __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory"); }
+
 __device__ __forceinline__ int clip_pos(int p) { return max(-FAR, min(FAR, p)); }
 
 // (x, y, z) of the grid in an order that keeps neighbouring x on one XCD: they read the same keys
@@ -647,7 +706,7 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_dq_kernel(const Wi
       for (int e = 0; e < W::VEC; ++e) d = fmaf(fx[e], fy[e], d);
     }
     dl[t] = xor_sum(d);
-    if (live && q == 0) delta[orow] = dl[t];
+    if (live && q == 0) delta[orow] = -dl[t];   // (as the other pass wants it)
   }
   __syncthreads();
 #pragma unroll
@@ -752,6 +811,7 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_dq_kernel(const Wi
 // ------------------------------------------------------------------------------------------------ backward: dk, dv
 // A workgroup owns 64 KT keys (16 KT per wave) of one key head and walks the 64-row tiles that see them: nkb blocks per head without sinks, and
 // nsplit workgroups (partial sums) for each of the nsink blocks that hold them.
+template <typename T, int NDT> constexpr int dkv_bufs() { return sizeof(T) == 2 && NDT <= 4 ? 3 : 2; }   // (three of wide heads: one workgroup per CU)
 template <typename T, int NDT, int KT>
 __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_dkv_kernel(const WinArgs a, const T* __restrict__ q_, const T* __restrict__ k_, const T* __restrict__ v_,
                                                       const T* __restrict__ dout, const float* __restrict__ lse, const float* __restrict__ delta,
@@ -759,7 +819,9 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_dkv_kernel(const W
   typedef WT<T, NDT> W;
   constexpr int NK = W::NK;
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
-  float* rowdata = reinterpret_cast<float*>(lds + 4 * W::TILE);   // two buffers of 64 x (lse | -D)
+  constexpr bool DMA = sizeof(T) == 2;
+  constexpr int BUFS = dkv_bufs<T, NDT>();                        // tiles of rows in LDS: the one in use and those on their way
+  float* rowdata = reinterpret_cast<float*>(lds + 2 * BUFS * W::TILE);   // as many buffers of 64 x (lse | -D)
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
   // one dimension: all blocks without sinks first (each XCD a contiguous range: neighbours read the same rows), then the sink blocks' shares, which are
   // short and fill the CUs that the last round of the others leaves idle
@@ -781,7 +843,7 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_dkv_kernel(const W
   const int klen = a.key_len ? max(0, min(a.key_len[b], a.Tk)) : a.Tk;
   const int s0 = kb * 64 * KT, k0 = s0 + wave * 16 * KT;                   // first key of the workgroup, of the wave
   const T* qb = q_ + b * a.q_bs;
-  zero_lds<T>(lds, 4 * W::TILE);
+  zero_lds<T>(lds, 2 * BUFS * W::TILE);
   typename W::frag kf[KT][NK], vf[KT][NK];
   int rlo[KT], rhi[KT];                                           // rows [rlo, rhi) see this lane's keys
 #pragma unroll
@@ -810,34 +872,21 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_dkv_kernel(const W
       landed(kf[t][ks]);
       landed(vf[t][ks]);
     }
-  Mover<T, NDT, 256> mv;
   // (a tile's first row is a frame's first head where 64 rows are whole frames: then its rows lie at the same places in every tile)
-  mv.init(a.dh, [&](int row, unsigned& x, unsigned& y) {
+  const auto places = [&](int row, unsigned& x, unsigned& y) {
     const int i = a.frame(row), g = row - i * a.G;
     x = i * (unsigned)a.q_ts + g * (unsigned)a.q_hs;
     y = (i * (unsigned)a.Hq + g) * (unsigned)a.dh;
-  });
+  };
+  const auto address = [&](int row, const T*& x, const T*& y) {
+    const int i = a.frame(row), g = row - i * a.G;
+    x = qb + i * a.q_ts + (long)(h * a.G + g) * a.q_hs;
+    y = dout + (((long)b * a.Tq + i) * a.Hq + h * a.G + g) * a.dh;
+  };
   const bool even = 64 % a.G == 0;
-  float pre_l = 0.f, pre_d = 0.f;
-  auto fetch = [&](int rt) {
-    const int first = row0 + rt * 64;
-    if (even && first + 64 <= row1) {
-      const int i = a.frame(first);
-      mv.fetch_whole(qb + i * a.q_ts + (long)(h * a.G) * a.q_hs, dout + (((long)b * a.Tq + i) * a.Hq + h * a.G) * a.dh);
-    } else {
-      mv.fetch([&](int n, const T*& x, const T*& y) {
-        const int row = first + n, i = a.frame(row), g = row - i * a.G;
-        x = qb + i * a.q_ts + (long)(h * a.G + g) * a.q_hs;
-        y = dout + (((long)b * a.Tq + i) * a.Hq + h * a.G + g) * a.dh;
-        return row < row1;
-      });
-    }
-    if (threadIdx.x < 64) {
-      const int row = first + (int)threadIdx.x, i = a.frame(row), g = row - i * a.G;
-      const long orow = ((long)b * a.Tq + i) * a.Hq + h * a.G + g;
-      pre_l = row < row1 ? lse[orow] : INFINITY;                  // +inf: the row's probabilities are 0
-      pre_d = row < row1 ? delta[orow] : 0.f;
-    }
+  const auto stat = [&](int row) {   // a row's place in lse and delta
+    const int i = a.frame(row), g = row - i * a.G;
+    return ((long)b * a.Tq + i) * a.Hq + h * a.G + g;
   };
   f32x4 ak[KT][NDT], av[KT][NDT];
 #pragma unroll
@@ -927,25 +976,94 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_dkv_kernel(const W
   // L2 does not hold (ten minutes of audio: 403 -> 387 us).
   const int n = t1 - t0;
   int rt = t0 + (n > 0 ? (n - ((row0 >> 6) + t0) % n) % n : 0);
-  if (n > 0) fetch(rt);
-  for (int k = 0; k < n; ++k) {
-    const int next = rt + 1 < t1 ? rt + 1 : t0;
-    unsigned char* Qs = lds + (k & 1) * 2 * W::TILE;
-    float* rd = rowdata + (k & 1) * 128;
-    mv.deposit(Qs);
-    if (threadIdx.x < 64) {
-      rd[threadIdx.x] = pre_l;
-      rd[64 + threadIdx.x] = -pre_d;
-    }
-    __syncthreads();
-    if (k + 1 < n) fetch(next);
-    const int at = row0 + rt * 64;
-    rt = next;
+  const auto after = [&](int tile) { return tile + 1 < t1 ? tile + 1 : t0; };
+  auto work = [&](int buf, int tile) {
+    const unsigned char* Qs = lds + buf * 2 * W::TILE;
+    const float* rd = rowdata + buf * 128;
+    const int at = row0 + tile * 64;
     // positions of the tile's rows against those that see the wave's keys
     const int p0 = base + a.frame(at), p1 = base + a.frame(min(at + 63, row1 - 1)), ke = min(k0 + 16 * KT, klen) - 1;
-    if (ke < k0 || p1 < k0 - a.right || (p0 > ke + a.left && k0 >= a.sinks)) continue;
+    if (ke < k0 || p1 < k0 - a.right || (p0 > ke + a.left && k0 >= a.sinks)) return;
     if (k0 + 16 * KT - 1 < klen && p0 >= k0 + 16 * KT - 1 - a.right && (p1 <= k0 + a.left || k0 + 16 * KT - 1 < a.sinks)) compute(Qs, rd, at, std::false_type{});
     else compute(Qs, rd, at, std::true_type{});
+  };
+  if constexpr (DMA) {
+    Dma<T, NDT, 256> dma;
+    dma.init(a.dh, places);
+    const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(size_t)((lds_ptr_t)lds));
+    constexpr int AHEAD = BUFS - 1, LOADS = Dma<T, NDT, 256>::LOADS;
+    auto send = [&](int tile, int buf) {
+      const int first = row0 + tile * 64;
+      const unsigned pair = lds0 + buf * 2 * W::TILE;
+      if (first + 64 <= row1) {
+        if (wave == (tile & 3)) {   // in front of the tile's own loads: `dma_wait` counts the newest
+          const long at = stat(first + lane);
+          const unsigned dst = lds0 + 2 * BUFS * W::TILE + buf * 512;
+          dma.word(lse + at, dst);
+          dma.word(delta + at, dst + 256);
+        }
+      } else if (wave == (tile & 3)) {
+        const bool there = first + lane < row1;
+        const long at = stat(min(first + lane, row1 - 1));
+        rowdata[buf * 128 + lane] = there ? lse[at] : INFINITY;   // +inf: the row's probabilities are 0
+        rowdata[buf * 128 + 64 + lane] = there ? delta[at] : 0.f;
+      }
+      if (even && first + 64 <= row1) {
+        const T *x, *y;
+        address(first, x, y);
+        dma.whole(x, y, pair);
+      } else {
+        // (behind the last row: that row again, with probabilities of 0)
+        dma.rows([&](int m, const T*& x, const T*& y) { address(min(first + m, row1 - 1), x, y); }, pair);
+      }
+    };
+    // A tile is sent for AHEAD tiles before it is worked on, to where the tile before the present one was: every wave has passed the barrier behind that.
+    int next = rt, buf = 0;
+    for (int k = 0; k < AHEAD && k < n; ++k, next = after(next)) send(next, k);
+    for (int k = 0; k < n; ++k) {
+      if (AHEAD == 2 && k + 1 < n) dma_wait<LOADS>();
+      else dma_wait<0>();
+      if (k + AHEAD < n) send(next, buf == 0 ? BUFS - 1 : buf - 1);
+      next = after(next);
+      work(buf, rt);
+      rt = after(rt);
+      buf = buf == BUFS - 1 ? 0 : buf + 1;
+    }
+  } else {
+    Mover<T, NDT, 256> mv;
+    mv.init(a.dh, places);
+    float pre_l = 0.f, pre_d = 0.f;
+    auto fetch = [&](int tile) {
+      const int first = row0 + tile * 64;
+      if (even && first + 64 <= row1) {
+        const T *x, *y;
+        address(first, x, y);
+        mv.fetch_whole(x, y);
+      } else {
+        mv.fetch([&](int m, const T*& x, const T*& y) {
+          address(first + m, x, y);
+          return first + m < row1;
+        });
+      }
+      if (threadIdx.x < 64) {
+        const bool there = first + lane < row1;
+        const long at = stat(min(first + lane, row1 - 1));
+        pre_l = there ? lse[at] : INFINITY;                       // +inf: the row's probabilities are 0
+        pre_d = there ? delta[at] : 0.f;
+      }
+    };
+    if (n > 0) fetch(rt);
+    for (int k = 0; k < n; ++k) {
+      mv.deposit(lds + (k & 1) * 2 * W::TILE);
+      if (threadIdx.x < 64) {
+        rowdata[(k & 1) * 128 + lane] = pre_l;
+        rowdata[(k & 1) * 128 + 64 + lane] = pre_d;
+      }
+      __syncthreads();
+      if (k + 1 < n) fetch(after(rt));
+      work(k & 1, rt);
+      rt = after(rt);
+    }
   }
 #pragma unroll
   for (int t = 0; t < KT; ++t) {
@@ -1050,7 +1168,7 @@ int run_dq(const WinArgs& a, const void* q, const void* k, const void* v, const 
 template <typename T, int NDT, int KT>
 int run_dkv(const WinArgs& a, const void* q, const void* k, const void* v, const void* dout, const float* lse, const float* delta, void* dk, void* dv, float* part,
             hipStream_t st) {
-  const size_t smem = 4 * WT<T, NDT>::TILE + 2 * 128 * 4;
+  const size_t smem = dkv_bufs<T, NDT>() * (2 * WT<T, NDT>::TILE + 128 * 4);
   if (int rc = set_lds(win_dkv_kernel<T, NDT, KT>, smem)) return rc;
   const int nkb = (a.Tk + 64 * KT - 1) / (64 * KT) - a.nsink;
   const long wgs = (long)a.B * a.Hkv * (nkb + a.nsink * a.nsplit);
