@@ -358,6 +358,69 @@ __device__ __forceinline__ void softmax_step(const WinArgs& a, f32x4 (&s)[4][RT]
   }
 }
 
+// Pairs of 64-key tiles in LDS: the one in use and those on their way.  Three where they leave room for as many workgroups as the registers do -- wide heads only where
+// few workgroups share the keys, one on a CU --, and where loads go straight to LDS.
+template <typename T, int NDT, bool SPLIT> constexpr int key_bufs() { return sizeof(T) == 2 && (NDT <= 4 || SPLIT) ? 3 : 2; }
+
+// A workgroup's walk over its tiles [kt0, kt1) of keys: work(tile's LDS, first key) on each, loads one or two tiles ahead.
+template <typename T, int NDT, int BUFS, typename F>
+__device__ __forceinline__ void walk_keys(const WinArgs& a, const TileWalk& walk, int kt0, int kt1, const T* kb_, const T* vb_, unsigned char* lds, F&& work) {
+  typedef WT<T, NDT> W;
+  const auto places = [&](int row, unsigned& x, unsigned& y) { x = row * (unsigned)a.k_ts; y = row * (unsigned)a.v_ts; };
+  const auto whole = [&](int s0) { return s0 + 64 <= walk.hi && (s0 >= walk.lo || s0 + 64 <= a.sinks); };
+  if constexpr (sizeof(T) == 2) {
+    constexpr int AHEAD = BUFS - 1, LOADS = Dma<T, NDT, 256>::LOADS;
+    Dma<T, NDT, 256> dma;
+    dma.init(a.dh, places);
+    const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(size_t)((lds_ptr_t)lds));
+    auto send = [&](int kt, int buf) {
+      const int s0 = walk.key0(kt);
+      const unsigned pair = lds0 + buf * 2 * W::TILE;
+      if (whole(s0)) dma.whole(kb_ + s0 * a.k_ts, vb_ + s0 * a.v_ts, pair);
+      else
+        dma.rows([&](int m, const T*& x, const T*& y) {
+          // what no row here sees is not read: the nearest key that one sees instead, its probabilities are 0
+          int s = s0 + m;
+          if (s >= walk.hi || (s < walk.lo && s >= a.sinks)) s = walk.lo < walk.hi ? max(walk.lo, min(s, walk.hi - 1)) : 0;
+          x = kb_ + s * a.k_ts;
+          y = vb_ + s * a.v_ts;
+        }, pair);
+    };
+    // A tile is sent for AHEAD tiles before it is worked on, to where the tile before the present one was: every wave has passed the barrier behind that.
+    const int n = kt1 - kt0;
+    for (int k = 0; k < AHEAD && k < n; ++k) send(kt0 + k, k);
+    int buf = 0;
+    for (int k = 0; k < n; ++k) {
+      if (AHEAD == 2 && k + 1 < n) dma_wait<LOADS>();
+      else dma_wait<0>();
+      if (k + AHEAD < n) send(kt0 + k + AHEAD, buf == 0 ? BUFS - 1 : buf - 1);
+      work(lds + buf * 2 * W::TILE, walk.key0(kt0 + k));
+      buf = buf == BUFS - 1 ? 0 : buf + 1;
+    }
+  } else {
+    Mover<T, NDT, 256> mv;
+    mv.init(a.dh, places);
+    auto fetch = [&](int s0) {
+      if (whole(s0)) return mv.fetch_whole(kb_ + s0 * a.k_ts, vb_ + s0 * a.v_ts);
+      mv.fetch([&](int row, const T*& x, const T*& y) {
+        const int s = s0 + row;
+        x = kb_ + s * a.k_ts;
+        y = vb_ + s * a.v_ts;
+        return s < walk.hi && (s >= walk.lo || s < a.sinks);                     // what no row here sees is not read
+      });
+    };
+    if (kt0 < kt1) fetch(walk.key0(kt0));
+    for (int kt = kt0; kt < kt1; ++kt) {
+      unsigned char* tiles = lds + ((kt - kt0) & 1) * 2 * W::TILE;
+      // the buffer's readers of two tiles ago have all passed the barrier of the tile in between
+      mv.deposit(tiles);
+      __syncthreads();
+      if (kt + 1 < kt1) fetch(walk.key0(kt + 1));
+      work(tiles, walk.key0(kt));
+    }
+  }
+}
+
 // Where several workgroups share a row block's keys: part[entry][head][share][row][dh] sums, behind them [entry][head][share][row] maximum and sum.
 __device__ __forceinline__ long share_row(const WinArgs& a, int b, int h, int split, int row) { return (((long)b * a.Hkv + h) * a.nsplit + split) * a.rows + row; }
 __device__ __forceinline__ float2* share_stat(const WinArgs& a, float* part, long n) {
@@ -382,7 +445,7 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_fwd_kernel(const W
   const T* qb = q_ + b * a.q_bs;
   const T* kb_ = k_ + b * a.k_bs + h * a.k_hs;
   const T* vb_ = v_ + b * a.v_bs + h * a.v_hs;
-  zero_lds<T>(lds, 4 * W::TILE);                                               // (channels past dh are never written again)
+  zero_lds<T>(lds, 2 * key_bufs<T, NDT, SPLIT>() * W::TILE);                                               // (channels past dh are never written again)
   typename W::frag qf[RT][NK];
   int pos[RT];
 #pragma unroll
@@ -397,19 +460,8 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_fwd_kernel(const W
   for (int t = 0; t < RT; ++t)
 #pragma unroll
     for (int ks = 0; ks < NK; ++ks) landed(qf[t][ks]);
-  Mover<T, NDT, 256> mv;
-  mv.init(a.dh, [&](int row, unsigned& x, unsigned& y) { x = row * (unsigned)a.k_ts; y = row * (unsigned)a.v_ts; });
   const int per = SPLIT ? (walk.n + a.nsplit - 1) / a.nsplit : walk.n;
   const int kt0 = split * per, kt1 = min(walk.n, kt0 + per);
-  auto fetch = [&](int s0) {
-    if (s0 + 64 <= walk.hi && (s0 >= walk.lo || s0 + 64 <= a.sinks)) return mv.fetch_whole(kb_ + s0 * a.k_ts, vb_ + s0 * a.v_ts);
-    mv.fetch([&](int row, const T*& x, const T*& y) {
-      const int s = s0 + row;
-      x = kb_ + s * a.k_ts;
-      y = vb_ + s * a.v_ts;
-      return s < walk.hi && (s >= walk.lo || s < a.sinks);                     // what no row here sees is not read
-    });
-  };
   float m[RT], l[RT];
   f32x4 o[RT][NDT];
 #pragma unroll
@@ -441,17 +493,11 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_fwd_kernel(const W
     for (int m2 = 0; m2 < 2; ++m2) wmma_transposed<T, NDT, RT>(Vs, m2, ph[2 * m2], ph[2 * m2 + 1], o, lane);
   };
 
-  if (kt0 < kt1) fetch(walk.key0(kt0));
-  for (int kt = kt0; kt < kt1; ++kt) {
-    unsigned char* Ks = lds + ((kt - kt0) & 1) * 2 * W::TILE;
-    // the buffer's readers of two tiles ago have all passed the barrier of the tile in between
-    mv.deposit(Ks);
-    __syncthreads();
-    if (kt + 1 < kt1) fetch(walk.key0(kt + 1));
-    const int s0 = walk.key0(kt), sight = w0 < a.rows ? tile_sight(a, walk.klen, s0, wp0, wp1) : 0;
+  walk_keys<T, NDT, key_bufs<T, NDT, SPLIT>()>(a, walk, kt0, kt1, kb_, vb_, lds, [&](const unsigned char* Ks, int s0) {
+    const int sight = w0 < a.rows ? tile_sight(a, walk.klen, s0, wp0, wp1) : 0;
     if (sight == 2) compute(Ks, s0, std::false_type{});
     else if (sight == 1) compute(Ks, s0, std::true_type{});
-  }
+  });
 
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
@@ -679,7 +725,7 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_dq_kernel(const Wi
   const T* qb = q_ + b * a.q_bs;
   const T* kb_ = k_ + b * a.k_bs + h * a.k_hs;
   const T* vb_ = v_ + b * a.v_bs + h * a.v_hs;
-  zero_lds<T>(lds, 4 * W::TILE);
+  zero_lds<T>(lds, 2 * key_bufs<T, NDT, false>() * W::TILE);
   typename W::frag qf[RT][NK], gf[RT][NK];
   int pos[RT];
   float ls[RT], dl[RT];
@@ -718,17 +764,6 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_dq_kernel(const Wi
       landed(gf[t][ks]);
     }
   }
-  Mover<T, NDT, 256> mv;
-  mv.init(a.dh, [&](int row, unsigned& x, unsigned& y) { x = row * (unsigned)a.k_ts; y = row * (unsigned)a.v_ts; });
-  auto fetch = [&](int s0) {
-    if (s0 + 64 <= walk.hi && (s0 >= walk.lo || s0 + 64 <= a.sinks)) return mv.fetch_whole(kb_ + s0 * a.k_ts, vb_ + s0 * a.v_ts);
-    mv.fetch([&](int row, const T*& x, const T*& y) {
-      const int s = s0 + row;
-      x = kb_ + s * a.k_ts;
-      y = vb_ + s * a.v_ts;
-      return s < walk.hi && (s >= walk.lo || s < a.sinks);                     // what no row here sees is not read
-    });
-  };
   f32x4 acc[RT][NDT];
 #pragma unroll
   for (int t = 0; t < RT; ++t)
@@ -779,16 +814,11 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_dq_kernel(const Wi
       wmma_transposed<T, NDT, RT>(Ks, m2, dsh[0], dsh[1], acc, lane);
     }
   };
-  if (walk.n > 0) fetch(walk.key0(0));
-  for (int kt = 0; kt < walk.n; ++kt) {
-    unsigned char* Ks = lds + (kt & 1) * 2 * W::TILE;
-    mv.deposit(Ks);
-    __syncthreads();
-    if (kt + 1 < walk.n) fetch(walk.key0(kt + 1));
-    const int s0 = walk.key0(kt), sight = w0 < a.rows ? tile_sight(a, walk.klen, s0, wp0, wp1) : 0;
+  walk_keys<T, NDT, key_bufs<T, NDT, false>()>(a, walk, 0, walk.n, kb_, vb_, lds, [&](const unsigned char* Ks, int s0) {
+    const int sight = w0 < a.rows ? tile_sight(a, walk.klen, s0, wp0, wp1) : 0;
     if (sight == 2) compute(Ks, s0, std::false_type{});
     else if (sight == 1) compute(Ks, s0, std::true_type{});
-  }
+  });
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
     const int row = w0 + 16 * t + r;
@@ -1125,7 +1155,7 @@ template <typename K> int set_lds(K kernel, size_t bytes) {
 
 template <typename T, int NDT, int RT, bool SPLIT>
 int run_fwd(const WinArgs& a, const void* q, const void* k, const void* v, void* out, float* lse, float* part, hipStream_t st) {
-  const size_t smem = 4 * WT<T, NDT>::TILE;
+  const size_t smem = 2 * key_bufs<T, NDT, SPLIT>() * WT<T, NDT>::TILE;
   if (int rc = set_lds(win_fwd_kernel<T, NDT, RT, SPLIT>, smem)) return rc;
   const dim3 grid((a.rows + 64 * RT - 1) / (64 * RT), a.Hkv, a.B * a.nsplit), block(256);
   hipLaunchKernelGGL((win_fwd_kernel<T, NDT, RT, SPLIT>), grid, block, smem, st, a, (const T*)q, (const T*)k, (const T*)v, (T*)out, lse, part);
@@ -1158,7 +1188,7 @@ int fwd_t(WinArgs a, const void* q, const void* k, const void* v, void* out, flo
 }
 template <typename T, int NDT, int RT>
 int run_dq(const WinArgs& a, const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse, float* delta, void* dq, hipStream_t st) {
-  const size_t smem = 4 * WT<T, NDT>::TILE;
+  const size_t smem = 2 * key_bufs<T, NDT, false>() * WT<T, NDT>::TILE;
   if (int rc = set_lds(win_dq_kernel<T, NDT, RT>, smem)) return rc;
   hipLaunchKernelGGL((win_dq_kernel<T, NDT, RT>), dim3((a.rows + 64 * RT - 1) / (64 * RT), a.Hkv, a.B), dim3(256), smem, st, a, (const T*)q, (const T*)k, (const T*)v,
                      (const T*)out, (const T*)dout, lse, delta, (T*)dq);
