@@ -17,11 +17,11 @@
 // window borders).  The blocks that hold sinks see every later row: their rows are dealt over several workgroups and joined.
 // Two passes cost 7 products instead of 5, but no atomics: results repeat bit for bit.
 //
-// Bound: vector issue beside the matrix pipe -- about nine vector instructions per score and pass, the exponential among them at a quarter rate --, and in the
-// dk / dv pass the staging of its rows (compiled out it takes 292 of 412 us).  Measured, 30001 frames, 16 heads over 4, 64 channels, 1024 keys per row,
-// bf16: forward 243 us (0.52 PFLOP/s of its two products), dq 258 (0.74 of three), dk / dv 382 + 7 (0.67 of four).  8 x 375 frames, 12 heads of 40
-// channels, window 64 + 64: 10, 11, 12 us.  fp32, 2 x 499 frames: 23, 29, 52 + 4 us.  Streams are bound by the cache's bytes and the length of a wave's
-// chain: one fp16 frame of 64 entries, 4 key heads, 1028 keys: 15 us (68 MB, 4.5 TB/s); 16 frames against 65536 keys of 128 channels: 28 + 5 us (67 MB, 3 TB/s
+// Bound: vector issue.  The forward pass keeps the vector unit busy 98 % of its time, more than half of that with the exponentials (a quarter rate each); dq 84 %, beside
+// 40 % of the matrix pipe; dk / dv half and a third: two waves per SIMD (its accumulators) leave gaps.  Measured, 30001 frames, 16 heads over 4, 64 channels, 1024 keys per
+// row, bf16: forward 226 us (0.57 PFLOP/s of its two products), dq 249 (0.77 of three), dk / dv 360 + 7 (0.71 of four).  8 x 375 frames, 12 heads of 40
+// channels, window 64 + 64: 10, 11, 12 us.  fp32, 2 x 499 frames: 23, 29, 51 + 4 us.  Streams are bound by the cache's bytes and the length of a wave's
+// chain: one fp16 frame of 64 entries, 4 key heads, 1028 keys: 15 us (68 MB, 4.5 TB/s); 16 frames against 65536 keys of 128 channels: 25.5 + 5 us (67 MB, 3.3 TB/s
 // with the partial sums' 17 MB).
 #pragma once
 #include "window_attention.h"
@@ -201,8 +201,8 @@ template <typename T, int NDT, int NT> struct Mover {
   }
 };
 
-// The same pair of tiles loaded straight into LDS (16-bit modes: rows without padding), 1 KiB of neighbouring places per wave and load: no registers in between, so that two
-// tiles can be on their way.  Lane i of a load fills the i-th 16 bytes behind the wave's; the twist is in WHICH piece of its row it asks for.
+// The same pair of tiles loaded straight into LDS (16-bit modes: rows without padding), 1 KiB of neighbouring places per wave and load: no registers in between (dk / dv of
+// 64 channels: 254 -> 236), no LDS writes.  Lane i of a load fills the i-th 16 bytes behind the wave's; the twist is in WHICH piece of its row it asks for.
 // (Issued from an asm statement: the compiler neither counts these loads nor drains them in front of LDS reads, `dma_wait` and the barrier order them.)
 typedef __attribute__((address_space(3))) const unsigned char* lds_ptr_t;
 template <typename T, int NDT, int NT> struct Dma {
@@ -358,9 +358,9 @@ __device__ __forceinline__ void softmax_step(const WinArgs& a, f32x4 (&s)[4][RT]
   }
 }
 
-// Pairs of 64-key tiles in LDS: the one in use and those on their way.  Three where they leave room for as many workgroups as the registers do -- wide heads only where
-// few workgroups share the keys, one on a CU --, and where loads go straight to LDS.
-template <typename T, int NDT, bool SPLIT> constexpr int key_bufs() { return sizeof(T) == 2 && (NDT <= 4 || SPLIT) ? 3 : 2; }
+// Pairs of 64-key tiles in LDS: the one in use and those on their way.  A second one on its way helps where workgroups share the keys and a CU holds one of them
+// (16 frames against 65536: 28 -> 25.5 us); with several on a CU the others' work covers the loads (ten minutes of audio, forward: two 226 us, three 234).
+template <typename T, bool SPLIT> constexpr int key_bufs() { return sizeof(T) == 2 && SPLIT ? 3 : 2; }
 
 // A workgroup's walk over its tiles [kt0, kt1) of keys: work(tile's LDS, first key) on each, loads one or two tiles ahead.
 template <typename T, int NDT, int BUFS, typename F>
@@ -445,7 +445,7 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_fwd_kernel(const W
   const T* qb = q_ + b * a.q_bs;
   const T* kb_ = k_ + b * a.k_bs + h * a.k_hs;
   const T* vb_ = v_ + b * a.v_bs + h * a.v_hs;
-  zero_lds<T>(lds, 2 * key_bufs<T, NDT, SPLIT>() * W::TILE);                                               // (channels past dh are never written again)
+  zero_lds<T>(lds, 2 * key_bufs<T, SPLIT>() * W::TILE);                                               // (channels past dh are never written again)
   typename W::frag qf[RT][NK];
   int pos[RT];
 #pragma unroll
@@ -493,7 +493,7 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_fwd_kernel(const W
     for (int m2 = 0; m2 < 2; ++m2) wmma_transposed<T, NDT, RT>(Vs, m2, ph[2 * m2], ph[2 * m2 + 1], o, lane);
   };
 
-  walk_keys<T, NDT, key_bufs<T, NDT, SPLIT>()>(a, walk, kt0, kt1, kb_, vb_, lds, [&](const unsigned char* Ks, int s0) {
+  walk_keys<T, NDT, key_bufs<T, SPLIT>()>(a, walk, kt0, kt1, kb_, vb_, lds, [&](const unsigned char* Ks, int s0) {
     const int sight = w0 < a.rows ? tile_sight(a, walk.klen, s0, wp0, wp1) : 0;
     if (sight == 2) compute(Ks, s0, std::false_type{});
     else if (sight == 1) compute(Ks, s0, std::true_type{});
@@ -725,7 +725,7 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_dq_kernel(const Wi
   const T* qb = q_ + b * a.q_bs;
   const T* kb_ = k_ + b * a.k_bs + h * a.k_hs;
   const T* vb_ = v_ + b * a.v_bs + h * a.v_hs;
-  zero_lds<T>(lds, 2 * key_bufs<T, NDT, false>() * W::TILE);
+  zero_lds<T>(lds, 2 * key_bufs<T, false>() * W::TILE);
   typename W::frag qf[RT][NK], gf[RT][NK];
   int pos[RT];
   float ls[RT], dl[RT];
@@ -814,7 +814,7 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_dq_kernel(const Wi
       wmma_transposed<T, NDT, RT>(Ks, m2, dsh[0], dsh[1], acc, lane);
     }
   };
-  walk_keys<T, NDT, key_bufs<T, NDT, false>()>(a, walk, 0, walk.n, kb_, vb_, lds, [&](const unsigned char* Ks, int s0) {
+  walk_keys<T, NDT, key_bufs<T, false>()>(a, walk, 0, walk.n, kb_, vb_, lds, [&](const unsigned char* Ks, int s0) {
     const int sight = w0 < a.rows ? tile_sight(a, walk.klen, s0, wp0, wp1) : 0;
     if (sight == 2) compute(Ks, s0, std::false_type{});
     else if (sight == 1) compute(Ks, s0, std::true_type{});
@@ -841,7 +841,6 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_dq_kernel(const Wi
 // ------------------------------------------------------------------------------------------------ backward: dk, dv
 // A workgroup owns 64 KT keys (16 KT per wave) of one key head and walks the 64-row tiles that see them: nkb blocks per head without sinks, and
 // nsplit workgroups (partial sums) for each of the nsink blocks that hold them.
-template <typename T, int NDT> constexpr int dkv_bufs() { return sizeof(T) == 2 && NDT <= 4 ? 3 : 2; }   // (three of wide heads: one workgroup per CU)
 template <typename T, int NDT, int KT>
 __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_dkv_kernel(const WinArgs a, const T* __restrict__ q_, const T* __restrict__ k_, const T* __restrict__ v_,
                                                       const T* __restrict__ dout, const float* __restrict__ lse, const float* __restrict__ delta,
@@ -850,8 +849,7 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_dkv_kernel(const W
   constexpr int NK = W::NK;
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   constexpr bool DMA = sizeof(T) == 2;
-  constexpr int BUFS = dkv_bufs<T, NDT>();                        // tiles of rows in LDS: the one in use and those on their way
-  float* rowdata = reinterpret_cast<float*>(lds + 2 * BUFS * W::TILE);   // as many buffers of 64 x (lse | -D)
+  float* rowdata = reinterpret_cast<float*>(lds + 4 * W::TILE);   // two buffers of 64 x (lse | -D)
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
   // one dimension: all blocks without sinks first (each XCD a contiguous range: neighbours read the same rows), then the sink blocks' shares, which are
   // short and fill the CUs that the last round of the others leaves idle
@@ -873,7 +871,7 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_dkv_kernel(const W
   const int klen = a.key_len ? max(0, min(a.key_len[b], a.Tk)) : a.Tk;
   const int s0 = kb * 64 * KT, k0 = s0 + wave * 16 * KT;                   // first key of the workgroup, of the wave
   const T* qb = q_ + b * a.q_bs;
-  zero_lds<T>(lds, 2 * BUFS * W::TILE);
+  zero_lds<T>(lds, 4 * W::TILE);
   typename W::frag kf[KT][NK], vf[KT][NK];
   int rlo[KT], rhi[KT];                                           // rows [rlo, rhi) see this lane's keys
 #pragma unroll
@@ -1021,14 +1019,13 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_dkv_kernel(const W
     Dma<T, NDT, 256> dma;
     dma.init(a.dh, places);
     const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(size_t)((lds_ptr_t)lds));
-    constexpr int AHEAD = BUFS - 1, LOADS = Dma<T, NDT, 256>::LOADS;
     auto send = [&](int tile, int buf) {
       const int first = row0 + tile * 64;
       const unsigned pair = lds0 + buf * 2 * W::TILE;
       if (first + 64 <= row1) {
-        if (wave == (tile & 3)) {   // in front of the tile's own loads: `dma_wait` counts the newest
+        if (wave == (tile & 3)) {
           const long at = stat(first + lane);
-          const unsigned dst = lds0 + 2 * BUFS * W::TILE + buf * 512;
+          const unsigned dst = lds0 + 4 * W::TILE + buf * 512;
           dma.word(lse + at, dst);
           dma.word(delta + at, dst + 256);
         }
@@ -1047,17 +1044,15 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_dkv_kernel(const W
         dma.rows([&](int m, const T*& x, const T*& y) { address(min(first + m, row1 - 1), x, y); }, pair);
       }
     };
-    // A tile is sent for AHEAD tiles before it is worked on, to where the tile before the present one was: every wave has passed the barrier behind that.
-    int next = rt, buf = 0;
-    for (int k = 0; k < AHEAD && k < n; ++k, next = after(next)) send(next, k);
+    // A tile is sent for when the one in front of it is worked on, to where the one in front of that was: every wave has passed the barrier behind it.  (Two on their way
+    // measured no better: with two workgroups on a CU the other's work covers the loads.)
+    if (n > 0) send(rt, 0);
     for (int k = 0; k < n; ++k) {
-      if (AHEAD == 2 && k + 1 < n) dma_wait<LOADS>();
-      else dma_wait<0>();
-      if (k + AHEAD < n) send(next, buf == 0 ? BUFS - 1 : buf - 1);
-      next = after(next);
-      work(buf, rt);
-      rt = after(rt);
-      buf = buf == BUFS - 1 ? 0 : buf + 1;
+      dma_wait<0>();
+      const int next = after(rt);
+      if (k + 1 < n) send(next, (k + 1) & 1);
+      work(k & 1, rt);
+      rt = next;
     }
   } else {
     Mover<T, NDT, 256> mv;
@@ -1155,7 +1150,7 @@ template <typename K> int set_lds(K kernel, size_t bytes) {
 
 template <typename T, int NDT, int RT, bool SPLIT>
 int run_fwd(const WinArgs& a, const void* q, const void* k, const void* v, void* out, float* lse, float* part, hipStream_t st) {
-  const size_t smem = 2 * key_bufs<T, NDT, SPLIT>() * WT<T, NDT>::TILE;
+  const size_t smem = 2 * key_bufs<T, SPLIT>() * WT<T, NDT>::TILE;
   if (int rc = set_lds(win_fwd_kernel<T, NDT, RT, SPLIT>, smem)) return rc;
   const dim3 grid((a.rows + 64 * RT - 1) / (64 * RT), a.Hkv, a.B * a.nsplit), block(256);
   hipLaunchKernelGGL((win_fwd_kernel<T, NDT, RT, SPLIT>), grid, block, smem, st, a, (const T*)q, (const T*)k, (const T*)v, (T*)out, lse, part);
@@ -1188,7 +1183,7 @@ int fwd_t(WinArgs a, const void* q, const void* k, const void* v, void* out, flo
 }
 template <typename T, int NDT, int RT>
 int run_dq(const WinArgs& a, const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse, float* delta, void* dq, hipStream_t st) {
-  const size_t smem = 2 * key_bufs<T, NDT, false>() * WT<T, NDT>::TILE;
+  const size_t smem = 2 * key_bufs<T, false>() * WT<T, NDT>::TILE;
   if (int rc = set_lds(win_dq_kernel<T, NDT, RT>, smem)) return rc;
   hipLaunchKernelGGL((win_dq_kernel<T, NDT, RT>), dim3((a.rows + 64 * RT - 1) / (64 * RT), a.Hkv, a.B), dim3(256), smem, st, a, (const T*)q, (const T*)k, (const T*)v,
                      (const T*)out, (const T*)dout, lse, delta, (T*)dq);
@@ -1198,7 +1193,7 @@ int run_dq(const WinArgs& a, const void* q, const void* k, const void* v, const 
 template <typename T, int NDT, int KT>
 int run_dkv(const WinArgs& a, const void* q, const void* k, const void* v, const void* dout, const float* lse, const float* delta, void* dk, void* dv, float* part,
             hipStream_t st) {
-  const size_t smem = dkv_bufs<T, NDT>() * (2 * WT<T, NDT>::TILE + 128 * 4);
+  const size_t smem = 2 * (2 * WT<T, NDT>::TILE + 128 * 4);
   if (int rc = set_lds(win_dkv_kernel<T, NDT, KT>, smem)) return rc;
   const int nkb = (a.Tk + 64 * KT - 1) / (64 * KT) - a.nsink;
   const long wgs = (long)a.B * a.Hkv * (nkb + a.nsink * a.nsplit);
