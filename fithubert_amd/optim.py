@@ -141,16 +141,20 @@ class ManyAdamW(torch.optim.Optimizer):
         for k, group in enumerate(self.param_groups):
             if all(p.grad is None for p in group["params"]):
                 continue
-            group["steps"] += 1
+            step = group["steps"] + 1
             for ps, moments in self._sets(k, group):
                 by = {}
                 for p in ps:
                     if p.grad is not None:
                         by.setdefault(p.grad.dtype, None)
                 for dt in by:   # one launch per gradient type; the others' tensors sit it out
-                    adamw_many(ps, [p.grad if p.grad is not None and p.grad.dtype == dt else None for p in ps], moments, step=group["steps"], lr=float(group["lr"]),
-                               betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], grad_scale=grad_scale, seed=group["steps"])
+                    adamw_many(ps, [p.grad if p.grad is not None and p.grad.dtype == dt else None for p in ps], moments, step=step, lr=float(group["lr"]),
+                               betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], grad_scale=grad_scale, seed=step)
+            group["steps"] = step   # (a refused call leaves the count)
         return loss
+
+    def __getstate__(self):   # copies and pickles carry the moments too
+        return dict(super().__getstate__(), _moments=self._moments)
 
     def state_dict(self):
         """torch's form with the flat moments of each group under 'moments' (in the order of its parameters, one set per device and type)"""

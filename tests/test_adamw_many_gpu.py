@@ -237,3 +237,29 @@ def test_streams_and_a_captured_step():
     with pytest.raises(RuntimeError, match="capture"):
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
             opt.step()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_copies_carry_the_moments_and_a_refused_step_counts_nothing(bits):
+    import copy
+    g = torch.Generator(device=DEV).manual_seed(6)
+    ps = [torch.nn.Parameter(torch.randn(n, device=DEV, generator=g)) for n in (300, 7)]
+    opt = ManyAdamW(ps, lr=1e-2, bits=bits)
+    grads = [torch.randn(p.shape, device=DEV, generator=g) for p in ps]
+
+    def step(o):
+        for p, t in zip(o.param_groups[0]["params"], grads):
+            p.grad = t.clone()
+        o.step()
+    step(opt)
+    twin = copy.deepcopy(opt)
+    held = [p.detach().clone() for p in ps]
+    step(twin)
+    assert all(torch.equal(p, h) for p, h in zip(ps, held)) and twin.param_groups[0]["params"][0] is not ps[0]
+    ps[1].data, was = ps[1].data.repeat(2)[::2], ps[1].data       # no longer contiguous: refused before anything is written
+    ps[1].grad = None
+    with pytest.raises(ValueError):
+        opt.step()
+    ps[1].data = was
+    step(opt)
+    assert all(torch.equal(a, b) for a, b in zip(ps, twin.param_groups[0]["params"])) and opt.param_groups[0]["steps"] == 2
