@@ -93,10 +93,10 @@ __global__ void __launch_bounds__(256) adapter_down_kernel(const Segs g, const T
     if (live) u.v = ld16(p);
     return u.f;
   };
-  for (int s = s0 + (int)blockIdx.y; s < g.n; s += (int)gridDim.y) {
-    const int b = max(g.begin(s), i0), e = min(g.begin(s + 1), i1);
-    if (g.begin(s) >= i1) break;
-    const int a = g.adapter(s);
+  bool more = true;   // (a segment that reaches i1 is the last: the next one need not be looked at)
+  for (int s = s0 + (int)blockIdx.y; s < g.n && more; s += (int)gridDim.y) {
+    const int begin = g.begin(s), end = g.begin(s + 1), a = g.adapter(s), b = max(begin, i0), e = min(end, i1);
+    more = end < i1;
     if (b >= e || a < 0) continue;
     const T* fa = f + (long)a * K * R;
     const T* xr[RT];
@@ -159,10 +159,10 @@ __global__ void __launch_bounds__(256) adapter_up_kernel(const Segs g, const T* 
   f32x4 acc[4];
 #pragma unroll
   for (int n = 0; n < 4; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int s = g.first_at(i0, threadIdx.x & 63); s < g.n; ++s) {
-    const int b = max(g.begin(s), i0), e = min(g.begin(s + 1), i1);
-    if (g.begin(s) >= i1) break;
-    const int a = g.adapter(s);
+  bool more = true;   // (a segment that reaches i1 is the last: the next one need not be looked at)
+  for (int s = g.first_at(i0, threadIdx.x & 63); s < g.n && more; ++s) {
+    const int begin = g.begin(s), end = g.begin(s + 1), a = g.adapter(s), b = max(begin, i0), e = min(end, i1);
+    more = end < i1;
     if (b >= e || a < 0) continue;
     const T* fa = f + (long)a * N * R;
     const bool mine = i0 + r >= b && i0 + r < e;
@@ -254,11 +254,6 @@ template <typename T> struct AdapterExtend {
     }
   }
   typedef typename AT<T>::frag frag;
-  __device__ __forceinline__ frag row_frag(int row, int b, int e, int k0) const {
-    frag fh = zero_frag((frag*)nullptr);
-    if (row >= b && row < e && k0 < R) fh = *reinterpret_cast<const frag*>(h + (long)row * R + k0);
-    return fh;
-  }
   template <int NN, int NM> __device__ __forceinline__ void operator()(f32x4 (&acc)[NN][NM], int row0, int col0, int lane) const {
     // nothing below may be computed in front of the main loop and held across it: that loop counts its vector-memory operations, so it may not spill
     asm volatile("" : "+v"(lane));
@@ -267,30 +262,31 @@ template <typename T> struct AdapterExtend {
     asm volatile("" : "+s"(row0), "+s"(col0));
     const int r = lane & 15, q = lane >> 4, row1 = min(row0 + 16 * NM, g.M);
     if (row0 >= g.M || col0 >= N) return;
-    for (int s = g.first_at(row0, lane); s < g.n; ++s) {
-      const int b = max(g.begin(s), row0), e = min(g.begin(s + 1), row1);
-      if (g.begin(s) >= row1) break;
-      const int a = g.adapter(s);
+    bool more = true;   // (a segment that reaches row1 is the last: the next one need not be looked at)
+    for (int s = g.first_at(row0, lane); s < g.n && more; ++s) {
+      const int begin = g.begin(s), end = g.begin(s + 1), a = g.adapter(s), b = max(begin, row0), e = min(end, row1);
+      more = end < row1;
       if (b >= e || a < 0) continue;
       const T* fa = f + (long)a * N * R;
       for (int k = 0; k < R; k += AT<T>::KD) {
-        const int k0 = k + ElemTraits<T>::VEC * q;
-        frag ff[NN];
+        const int k0 = k + ElemTraits<T>::VEC * q, kc = min(k0, R - ElemTraits<T>::VEC);
+        // all operands in flight at once: rows, columns and ranks past the edge read the last ones, their products are dropped or zero
+        frag ff[NN], fh[NM];
 #pragma unroll
-        for (int n = 0; n < NN; ++n) {
-          const int col = col0 + 16 * n + r;
-          ff[n] = zero_frag((frag*)nullptr);
-          if (col < N && k0 < R) ff[n] = *reinterpret_cast<const frag*>(fa + (long)col * R + k0);
-        }
+        for (int n = 0; n < NN; ++n) ff[n] = *reinterpret_cast<const frag*>(fa + (long)min(col0 + 16 * n + r, N - 1) * R + kc);
+#pragma unroll
+        for (int m = 0; m < NM; ++m) fh[m] = *reinterpret_cast<const frag*>(h + (long)min(row0 + 16 * m + r, g.M - 1) * R + kc);
+#pragma unroll
+        for (int n = 0; n < NN; ++n)
+          if (k0 >= R) ff[n] = zero_frag((frag*)nullptr);
 #pragma unroll
         for (int m = 0; m < NM; ++m) {
           if (b >= row0 + 16 * m + 16 || e <= row0 + 16 * m) continue;
           const int row = row0 + 16 * m + r;
-          const bool mine = row >= b && row < e;   // rows of other requests keep their sum (a zero times this adapter's infinity would reach them)
-          const frag fh = row_frag(row, b, e, k0);
+          const bool mine = row >= b && row < e;   // rows of other requests keep their sum
 #pragma unroll
           for (int n = 0; n < NN; ++n) {
-            const f32x4 t = mma<T>(ff[n], fh, acc[n][m]);
+            const f32x4 t = mma<T>(ff[n], fh[m], acc[n][m]);
 #pragma unroll
             for (int c = 0; c < 4; ++c) acc[n][m][c] = mine ? t[c] : acc[n][m][c];
           }
