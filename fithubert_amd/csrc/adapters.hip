@@ -10,9 +10,9 @@
 //         GEMM's residual operand.
 // outer:  dA and dB in one launch: a workgroup owns 64 columns of one adapter's factor and walks that adapter's rows, whichever segments they lie in, 32
 //         at a time per wave; long walks are dealt over several workgroups whose partial sums are added in order (no atomics).
-// Measured, forward and backward of 16384 x 1024 -> 4096, rank 16, 4 adapters, 32 requests, bf16: h 10 us, y 136 (1.0 PFLOP/s), turn 5, G 36 (134 MB, 3.7 TB/s), dx 133,
-// dA and dB 26 + 5.  Forward of 9973 x 480 -> 1440, rank 8: 6 + 28 us -- 234 tiles of 256 x 256 for 256 CUs, each with eight steps of K: bound by filling and emptying
-// one tile.  32 one-row requests, 768 -> 768, fp16: 4.7 + 6.9 us.  fp32, 1497 x 480 -> 480, rank 32, both directions: 75 us of kernels (y 20, dx 22, the rest 4 to 8 each).
+// Measured, forward and backward of 16384 x 1024 -> 4096, rank 16, 4 adapters, 32 requests, bf16: h 10 us, y 131 (1.05 PFLOP/s), turn 5, G 36 (134 MB, 3.7 TB/s), dx 133,
+// dA and dB 26 + 5.  Forward of 9973 x 480 -> 1440, rank 8: 6 + 25.5 us -- 234 tiles of 256 x 256 for 256 CUs, each with eight steps of K: bound by filling and emptying
+// one tile.  32 one-row requests, 768 -> 768, fp16: 4.7 + 6.9 us.  fp32, 1497 x 480 -> 480, rank 32, both directions: 73 us of kernels (y 19, dx 21, the rest 4 to 8 each).
 #include "gemm_loops.cuh"
 #include "kernels.h"
 #include "attn_frag.cuh"
