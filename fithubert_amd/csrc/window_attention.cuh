@@ -17,8 +17,8 @@
 // window borders).  The blocks that hold sinks see every later row: their rows are dealt over several workgroups and joined.
 // Two passes cost 7 products instead of 5, but no atomics: results repeat bit for bit.
 //
-// Bound: vector issue.  The forward pass keeps the vector unit busy 98 % of its time, more than half of that with the exponentials (a quarter rate each); dq 84 %, beside
-// 40 % of the matrix pipe; dk / dv half and a third: two waves per SIMD (its accumulators) leave gaps.  Measured, 30001 frames, 16 heads over 4, 64 channels, 1024 keys per
+// Bound: vector issue.  Counted with four cycles per vector instruction and sixteen per exponential, the forward's instructions take all of its time, more than half of it
+// the exponentials'; dq's 88 %, beside 43 % of the matrix pipe; dk / dv's 55 % and 37 %: two waves per SIMD (its accumulators) leave gaps.  Measured, 30001 frames, 16 heads over 4, 64 channels, 1024 keys per
 // row, bf16: forward 226 us (0.57 PFLOP/s of its two products), dq 249 (0.77 of three), dk / dv 360 + 7 (0.71 of four).  8 x 375 frames, 12 heads of 40
 // channels, window 64 + 64: 10, 11, 12 us.  fp32, 2 x 499 frames: 23, 29, 51 + 4 us.  Streams are bound by the cache's bytes and the length of a wave's
 // chain: one fp16 frame of 64 entries, 4 key heads, 1028 keys: 15 us (68 MB, 4.5 TB/s); 16 frames against 65536 keys of 128 channels: 25.5 + 5 us (67 MB, 3.3 TB/s
