@@ -879,10 +879,12 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_dkv_kernel(const W
     const int s = k0 + 16 * t + r;
     rlo[t] = max(0, min(a.Tq, s - a.right - base)) * a.G;
     rhi[t] = s >= klen ? 0 : s < a.sinks ? a.rows : max(0, min(a.Tq, s + a.left - base + 1)) * a.G;
+    // a key that no row sees is not read: with zeros its dP is finite, so that its probabilities of 0 leave 0 of it
+    const bool met = s < klen && rlo[t] < rhi[t];
 #pragma unroll
     for (int ks = 0; ks < NK; ++ks) {
-      kf[t][ks] = gfrag<T>(k_ + b * a.k_bs + h * a.k_hs + s * a.k_ts, s < klen, ks, lane, a.dh);
-      vf[t][ks] = gfrag<T>(v_ + b * a.v_bs + h * a.v_hs + s * a.v_ts, s < klen, ks, lane, a.dh);
+      kf[t][ks] = gfrag<T>(k_ + b * a.k_bs + h * a.k_hs + s * a.k_ts, met, ks, lane, a.dh);
+      vf[t][ks] = gfrag<T>(v_ + b * a.v_bs + h * a.v_hs + s * a.v_ts, met, ks, lane, a.dh);
     }
   }
   // rows that see a key of this block: frames [f0, f1), then the workgroup's share of their 64-row tiles

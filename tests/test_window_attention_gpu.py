@@ -327,3 +327,22 @@ def test_refusals_on_the_gpu():
     g = torch.autograd.grad(y, q, torch.ones_like(y), create_graph=True)[0]
     with pytest.raises(RuntimeError):                        # no second derivatives
         torch.autograd.grad(g.sum(), q)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,Tq,Tk,Hq,Hkv,dh,left,right,sinks", [(2, 40, 300, 4, 2, 64, 30, 0, 0), (2, 40, 300, 4, 2, 40, 30, 7, 3), (2, 3, 200, 6, 2, 128, 5, 2, 1), (3, 70, 500, 2, 2, 96, 0, 0, 70),
+                                                                (8, 40, 1024, 8, 8, 64, 100, 3, 2)])
+def test_keys_that_no_row_sees_take_no_gradient(dtype, B, Tq, Tk, Hq, Hkv, dh, left, right, sinks):
+    """Queries in the middle of a cache: frames in front of the window, between the sinks and the window, and behind the last row's view may hold anything in the backward pass too."""
+    q, k, v, dout = inputs(31, dtype, B, Tq, Tk, Hq, Hkv, dh)
+    starts, lens = [Tk // 2 - 11 * b for b in range(B)], [Tk - 7 * b for b in range(B)]
+    kw = dict(left=left, right=right, sinks=sinks, q_start=torch.tensor(starts, device=DEV), key_len=torch.tensor(lens, device=DEV))
+    clean = check(q, k, v, dout, left, right, sinks, key_len=lens, q_start=starts)
+    unseen = ~seen(Tq, Tk, kw["key_len"], kw["q_start"], left, right, sinks).any(1)
+    assert unseen[:, sinks:starts[-1] - left].all() and unseen[:, starts[0] + Tq + right:].all()
+    for bad in (math.inf, -math.inf, math.nan, torch.finfo(dtype).min):
+        k2, v2 = k.clone(), v.clone()
+        k2[unseen], v2[unseen] = bad, bad
+        dirty = run(q, k2, v2, dout, **kw)
+        assert (dirty["dk"][unseen] == 0).all() and (dirty["dv"][unseen] == 0).all(), bad
+        assert all(torch.equal(clean[n], dirty[n]) for n in clean), bad
