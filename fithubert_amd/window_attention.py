@@ -126,8 +126,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, left:
     gives zeros and takes part in no gradient.  Keys that no row of the call sees may hold anything; an infinity or NaN in a key that some rows see
     may reach rows near them that do not (0 x inf), one in a row's query or gradient the gradients of keys near those it sees.  ``scale`` > 0, default dh ** -0.5.
 
-    16-bit modes round the probabilities (backward: and dS) to the element type in front of the second products; softmax and sums are fp32.  Nothing
-    depends on the order of atomics: equal calls give equal bits."""
+    16-bit modes round the probabilities (backward: and dS) to the element type in front of the second products; softmax and sums are fp32.  In fp16 a dS above
+    65504 is infinite and one below 2^-25 is 0: scale the loss so that gradients lie between.  Nothing depends on the order of atomics: equal calls give equal bits."""
     if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
         raise ValueError(f"q [B][Tq][Hq][dh], k and v [B][Tk][Hkv][dh]: got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     if q.dtype not in _DT or k.dtype != q.dtype or v.dtype != q.dtype:

@@ -269,7 +269,7 @@ int fh_attention_backward_bias(int dtype, const void* qkv, const void* out, cons
  * of 16 bytes; frames and heads at most 2^23 elements apart), so a packed q|k|v projection or a longer cache is read in place; query head h reads key head h / (Hq / Hkv).
  * out, dout, dq [B][Tq][Hq][dh] and dk, dv [B][Tk][Hkv][dh] are contiguous; lse: B * Tq * Hq floats that the backward reads (forward: NULL
  * when there is none).  dq, dk, dv are written, not added to (keys that no row sees: 0).  dh <= 128, a multiple of 8; 16-bit modes round the
- * probabilities and dS to the element type before the second products, sums and softmax are fp32.  No atomics: results repeat bit for bit.
+ * probabilities and dS = scale P (dP - D) to the element type before the second products (fp16: finite up to 65504), sums and softmax are fp32.  No atomics: results repeat bit for bit.
  * scratch: fh_window_attention_scratch_bytes(dtype, d, 0 forward | 1 backward) bytes, 16-byte aligned (0: NULL will do).  A few rows
  * against long caches are split over the keys and joined through it.
  * ------------------------------------------------------------------------------------------ */

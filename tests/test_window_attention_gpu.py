@@ -346,3 +346,17 @@ def test_keys_that_no_row_sees_take_no_gradient(dtype, B, Tq, Tk, Hq, Hkv, dh, l
         dirty = run(q, k2, v2, dout, **kw)
         assert (dirty["dk"][unseen] == 0).all() and (dirty["dv"][unseen] == 0).all(), bad
         assert all(torch.equal(clean[n], dirty[n]) for n in clean), bad
+
+
+@pytest.mark.parametrize("T,Hq,Hkv,dh,left,right,sinks,v_size,k_size", [(60, 4, 2, 64, 2, 0, 0, 2, 0.25), (200, 4, 2, 64, 31, 3, 2, 8, 0.125), (150, 2, 2, 128, 9, 0, 0, 4, 0.25)])
+def test_large_fp16_gradients_stay_finite(T, Hq, Hkv, dh, left, right, sinks, v_size, k_size):
+    """A scaled loss: P (dP - D) lies past fp16's 65504 while dS = scale P (dP - D) and every result lie below it.  (The bounds are the other tests'.)"""
+    q, k, v, dout = (t * f for t, f in zip(inputs(41, torch.float16, 2, T, T, Hq, Hkv, dh), (k_size, k_size, v_size, 8000)))
+    G, scale = Hq // Hkv, dh ** -0.5
+    mask = seen(T, T, torch.full((2,), T, device=DEV), torch.zeros(2, dtype=torch.long, device=DEV), left, right, sinks)[:, None]
+    Q, K, V, dO = (t.double().permute(0, 2, 1, 3) for t in (q, k, v, dout))
+    K, V = K.repeat_interleave(G, 1), V.repeat_interleave(G, 1)
+    P = torch.softmax((Q @ K.transpose(2, 3).contiguous() * scale).masked_fill(~mask, -math.inf), -1)
+    raw = P * (dO @ V.transpose(2, 3).contiguous() - (dO * (P @ V)).sum(-1, keepdim=True))
+    assert raw.abs().max() > 1.5 * 65504 and scale * raw.abs().max() < 65504
+    check(q, k, v, dout, left, right, sinks)
