@@ -263,8 +263,6 @@ template <typename T, int NDT, int NT> struct Dma {
 // all of this wave's loads but the N newest are there, and so is what every wave wrote; then the others' too
 template <int N> __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory"); }
 
-__device__ __forceinline__ int clip_pos(int p) { return max(-FAR, min(FAR, p)); }
-
 // (x, y, z) of the grid in an order that keeps neighbouring x on one XCD: they read the same keys
 __device__ __forceinline__ void win_block(int& x, int& y, int& z) {
   const int lg = fh_xcd_logical_block(), gx = gridDim.x, gy = gridDim.y;
@@ -431,7 +429,7 @@ __device__ __forceinline__ float2* share_stat(const WinArgs& a, float* part, lon
 }
 
 template <typename T, int NDT, int RT, bool SPLIT>
-__global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_fwd_kernel(const WinArgs a, const T* __restrict__ q_, const T* __restrict__ k_, const T* __restrict__ v_,
+__global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_fwd_kernel(WinArgs a, const T* __restrict__ q_, const T* __restrict__ k_, const T* __restrict__ v_,
                                                           T* __restrict__ out, float* __restrict__ lse, float* __restrict__ part) {
   typedef WT<T, NDT> W;
   constexpr int NK = W::NK;
@@ -440,7 +438,7 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_fwd_kernel(const W
   int blk, h, bz;
   win_block(blk, h, bz);
   const int split = SPLIT ? bz % a.nsplit : 0, b = SPLIT ? bz / a.nsplit : bz;
-  const int base = a.q_start ? clip_pos(a.q_start[b]) : 0;
+  const int base = a.enter(b);
   const int g0 = blk * 64 * RT, g1 = min(g0 + 64 * RT, a.rows) - 1;            // the workgroup's rows
   const int w0 = g0 + wave * 16 * RT, w1 = min(w0 + 16 * RT, a.rows) - 1;                // the wave's
   const TileWalk walk(a, b, base + a.frame(g0), base + a.frame(g1));
@@ -537,7 +535,7 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_fwd_kernel(const W
 // time, so the four waves of a workgroup walk tiles of their own, without a barrier: keys go straight from memory into the first product's operand
 // registers, values through a tile of LDS that only this wave uses, and both are requested a tile ahead.  The waves' sums meet at the end.
 template <typename T, int NDT, int TT>
-__global__ void __launch_bounds__(256, NDT * TT * (int)sizeof(T) > 12 ? 1 : 2) win_few_kernel(const WinArgs a, const T* __restrict__ q_, const T* __restrict__ k_,
+__global__ void __launch_bounds__(256, NDT * TT * (int)sizeof(T) > 12 ? 1 : 2) win_few_kernel(WinArgs a, const T* __restrict__ q_, const T* __restrict__ k_,
                                                                                     const T* __restrict__ v_, T* __restrict__ out, float* __restrict__ lse,
                                                                                     float* __restrict__ part) {
   typedef WT<T, NDT> W;
@@ -545,7 +543,7 @@ __global__ void __launch_bounds__(256, NDT * TT * (int)sizeof(T) > 12 ? 1 : 2) w
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
   const int split = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
-  const int base = a.q_start ? clip_pos(a.q_start[b]) : 0;
+  const int base = a.enter(b);
   const int wp0 = base, wp1 = base + a.Tq - 1;
   const TileWalk walk(a, b, wp0, wp1);
   const T* qb = q_ + b * a.q_bs;
@@ -711,7 +709,7 @@ __global__ void __launch_bounds__(256) win_join_kernel(const WinArgs a, float* _
 
 // ------------------------------------------------------------------------------------------------ backward: dq, and D for the other pass
 template <typename T, int NDT, int RT>
-__global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_dq_kernel(const WinArgs a, const T* __restrict__ q_, const T* __restrict__ k_, const T* __restrict__ v_,
+__global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_dq_kernel(WinArgs a, const T* __restrict__ q_, const T* __restrict__ k_, const T* __restrict__ v_,
                                                          const T* __restrict__ out, const T* __restrict__ dout, const float* __restrict__ lse,
                                                          float* __restrict__ delta, T* __restrict__ dq) {
   typedef WT<T, NDT> W;
@@ -720,7 +718,7 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_dq_kernel(const Wi
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
   int blk, h, b;
   win_block(blk, h, b);
-  const int base = a.q_start ? clip_pos(a.q_start[b]) : 0;
+  const int base = a.enter(b);
   const int g0 = blk * 64 * RT, g1 = min(g0 + 64 * RT, a.rows) - 1;
   const int w0 = g0 + wave * 16 * RT, w1 = min(w0 + 16 * RT, a.rows) - 1;
   const TileWalk walk(a, b, base + a.frame(g0), base + a.frame(g1));
@@ -846,7 +844,7 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_dq_kernel(const Wi
 // A workgroup owns 64 KT keys (16 KT per wave) of one key head and walks the 64-row tiles that see them: nkb blocks per head without sinks, and
 // nsplit workgroups (partial sums) for each of the nsink blocks that hold them.
 template <typename T, int NDT, int KT>
-__global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_dkv_kernel(const WinArgs a, const T* __restrict__ q_, const T* __restrict__ k_, const T* __restrict__ v_,
+__global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_dkv_kernel(WinArgs a, const T* __restrict__ q_, const T* __restrict__ k_, const T* __restrict__ v_,
                                                       const T* __restrict__ dout, const float* __restrict__ lse, const float* __restrict__ delta,
                                                       T* __restrict__ dk, T* __restrict__ dv, float* __restrict__ part, int nkb) {
   typedef WT<T, NDT> W;
@@ -871,7 +869,7 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_dkv_kernel(const W
     kb = lg - bh * nkb + a.nsink;
   }
   const int b = bh / a.Hkv, h = bh - b * a.Hkv;
-  const int base = a.q_start ? clip_pos(a.q_start[b]) : 0;
+  const int base = a.enter(b);
   const int klen = a.key_len ? max(0, min(a.key_len[b], a.Tk)) : a.Tk;
   const int s0 = kb * 64 * KT, k0 = s0 + wave * 16 * KT;                   // first key of the workgroup, of the wave
   const T* qb = q_ + b * a.q_bs;

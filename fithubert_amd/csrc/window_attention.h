@@ -2,7 +2,8 @@
 #pragma once
 #include "common.cuh"
 
-constexpr int FAR = 1 << 29;       // "no limit", and the largest position
+constexpr int FAR = 1 << 29;             // more than the keys or the rows of an entry
+constexpr int NO_LIMIT = 0x7fffffff;     // of left or right
 
 struct WinArgs {
   int B, Tq, Tk, Hq, Hkv, G, dh, left, right, sinks;
@@ -19,6 +20,14 @@ struct WinArgs {
     if (magic == 0u) return row;
     const int f = (int)__umulhi((unsigned)row, magic);
     return f * G > row ? f - 1 : f;
+  }
+  // The position of entry b's first row, clipped to +- FAR, and left and right as they are from there: what counts is where the first row's view begins and ends, and an end
+  // clipped to +- FAR, past all keys whatever the row, hides and shows the same.  Sums and differences of positions, limits and keys then fit 32 bits.
+  __device__ __forceinline__ int enter(int b) {
+    const int first = q_start ? q_start[b] : 0, base = max(-FAR, min(FAR, first));
+    left = left == NO_LIMIT ? base + FAR : base - (int)max((long)-FAR, min((long)FAR, (long)first - left));
+    right = right == NO_LIMIT ? FAR - base : (int)max((long)-FAR, min((long)FAR, (long)first + right)) - base;
+    return base;
   }
 };
 

@@ -21,8 +21,8 @@ int check(int dtype, const fh_window_attention_desc* d) {
 WinArgs args_of(const fh_window_attention_desc* d) {
   WinArgs a;
   a.B = d->B; a.Tq = d->Tq; a.Tk = d->Tk; a.Hq = d->Hq; a.Hkv = d->Hkv; a.G = d->Hq / d->Hkv; a.dh = d->dh;
-  a.left = d->left < 0 || d->left > FAR ? FAR : d->left;
-  a.right = d->right < 0 || d->right > FAR ? FAR : d->right;
+  a.left = d->left < 0 ? NO_LIMIT : d->left;
+  a.right = d->right < 0 ? NO_LIMIT : d->right;
   a.sinks = d->sinks < 0 ? 0 : d->sinks > d->Tk ? d->Tk : d->sinks;
   a.scale = d->scale;
   a.c = d->scale * 1.4426950408889634f;

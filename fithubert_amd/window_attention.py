@@ -122,7 +122,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, left:
     filled -- are read in place when addresses and strides are multiples of 16 bytes, copied otherwise.
 
     Query i of entry b stands at position p = ``q_start[b]`` + i (default 0; required as soon as Tq != Tk) and sees key s when s < ``key_len[b]``
-    (default Tk), s <= p + ``right`` and (s >= p - ``left`` or s < ``sinks``); a negative ``left`` or ``right`` is no limit.  A row that sees no key
+    (default Tk), s <= p + ``right`` and (s >= p - ``left`` or s < ``sinks``); a ``left`` or ``right`` that is negative, or 2^31 - 1 and more, is no limit.  A row that sees no key
     gives zeros and takes part in no gradient.  Keys that no row of the call sees may hold anything; an infinity or NaN in a key that some rows see
     may reach rows near them that do not (0 x inf), one in a row's query or gradient the gradients of keys near those it sees.  ``scale`` > 0, default dh ** -0.5.
 

@@ -360,3 +360,16 @@ def test_large_fp16_gradients_stay_finite(T, Hq, Hkv, dh, left, right, sinks, v_
     raw = P * (dO @ V.transpose(2, 3).contiguous() - (dO * (P @ V)).sum(-1, keepdim=True))
     assert raw.abs().max() > 1.5 * 65504 and scale * raw.abs().max() < 65504
     check(q, k, v, dout, left, right, sinks)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("Tq", [3, 40])
+@pytest.mark.parametrize("left,right", [(-1, 0), (-1, -1), (0, -1), (7, -1), (2 ** 29 + 10, 0), (2 ** 30 + 7, 2 ** 30), (2 ** 31 - 1, 3), (5, 2 ** 31 - 2), (2 ** 31 - 2, 2 ** 31 - 2)])
+def test_positions_far_away(dtype, Tq, left, right):
+    """Positions, and limits, up to the ends of 32 bits: a row far behind all keys sees them exactly when its limit reaches back that far."""
+    starts = [2 ** 31 - 1, 2 ** 30 + 5, 2 ** 29 + 15, 2 ** 29 - 3, 0, -1, -2 ** 29 + 1, -2 ** 29 - 40, -2 ** 30 - 2, -2 ** 31]
+    q, k, v, dout = inputs(51, dtype, len(starts), Tq, 50, 4, 2, 32)
+    check(q, k, v, dout, -1 if left >= 2 ** 31 - 1 else left, right, 2 if right == 0 else 0, q_start=starts)
+    want = run(q, k, v, dout, left=-1 if left >= 2 ** 31 - 1 else left, right=right, q_start=torch.tensor(starts, device=DEV))
+    got = run(q, k, v, dout, left=left, right=right, q_start=torch.tensor(starts, device=DEV))
+    assert all(torch.equal(want[n], got[n]) for n in want)
