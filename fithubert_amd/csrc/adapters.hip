@@ -270,7 +270,7 @@ template <typename T> struct AdapterExtend {
       const T* fa = f + (long)a * N * R;
       for (int k = 0; k < R; k += AT<T>::KD) {
         const int k0 = k + ElemTraits<T>::VEC * q, kc = min(k0, R - ElemTraits<T>::VEC);
-        // all operands in flight at once: rows, columns and ranks past the edge read the last ones, their products are dropped or zero
+        // all operands in flight at once: rows and columns past the edge read the last ones, their products are dropped; ranks past it are zeros in both operands (h may be infinite)
         frag ff[NN], fh[NM];
 #pragma unroll
         for (int n = 0; n < NN; ++n) ff[n] = *reinterpret_cast<const frag*>(fa + (long)min(col0 + 16 * n + r, N - 1) * R + kc);
@@ -279,6 +279,9 @@ template <typename T> struct AdapterExtend {
 #pragma unroll
         for (int n = 0; n < NN; ++n)
           if (k0 >= R) ff[n] = zero_frag((frag*)nullptr);
+#pragma unroll
+        for (int m = 0; m < NM; ++m)
+          if (k0 >= R) fh[m] = zero_frag((frag*)nullptr);
 #pragma unroll
         for (int m = 0; m < NM; ++m) {
           if (b >= row0 + 16 * m + 16 || e <= row0 + 16 * m) continue;

@@ -260,3 +260,20 @@ def test_broadcast_inputs_and_one_leaf_twice(dtype):
     dx, da = torch.autograd.grad(y, (row, one), s["dy"])
     want = run(s)
     assert torch.equal(dx, want["dx"].sum(0, keepdim=True)) and torch.equal(da, want["da"] + want["db"].transpose(1, 2))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K,N,R", [(1024, 512, 1024, 8), (4096, 1536, 1536, 8), (4096, 1536, 1536, 40), (40, 512, 512, 24), (300, 512, 512, 8)])
+def test_a_product_past_the_type_gives_infinity_in_its_row(dtype, M, K, N, R):
+    """h (backward: G) of one row overflows: its row of y (dx) is infinite, as infinity times positive factors is, not NaN; no other row notices."""
+    s = make(61, dtype, M, K, N, R, 2, [0, M // 3, M], [0, 1])
+    s["a"], s["b"] = s["a"].abs() + 0.25, s["b"].abs() + 0.25
+    clean = run(s)
+    big = 6e4 if dtype == torch.float16 else 2e37   # (times 0.25 K or 0.25 N: past either type; the projection's own sum stays inside 32 bits)
+    for row in (5, M // 3 + 4):
+        s2 = dict(s, x=s["x"].clone(), dy=s["dy"].clone())
+        s2["x"][row], s2["dy"][row] = big, big
+        dirty = run(s2)
+        for n in ("y", "dx"):
+            assert (dirty[n][row] == float("inf")).all(), n
+            assert torch.equal(dirty[n][:row], clean[n][:row]) and torch.equal(dirty[n][row + 1:], clean[n][row + 1:]), n
