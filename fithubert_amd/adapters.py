@@ -51,7 +51,7 @@ def _forward(x, weight, bias, a, b, scaling, start, which):
         with torch.cuda.device(dev):
             return _forward(x, weight, bias, a, b, scaling, start, which)
     d = _desc(x, a, weight.shape[0], scaling, start, which)
-    h, y = x.new_empty((d.M, d.R)), x.new_empty((d.M, d.N))
+    h, y = x.new_empty((x.shape[0], a.shape[1])), x.new_empty((x.shape[0], weight.shape[0]))
     scratch = _scratch(dt, d, 0, dev)
     L.check(L.lib().fh_adapter_linear_forward(dt, C.byref(d), x.data_ptr(), weight.data_ptr(), _ptr(bias), a.data_ptr(), b.data_ptr(), h.data_ptr(), y.data_ptr(),
                                               _ptr(scratch), _stream(dev.index)), "fh_adapter_linear_forward")

@@ -213,3 +213,22 @@ def test_live_requests_frame_by_frame(dtype):
     start = torch.arange(0, B * T + 1, T, dtype=torch.int32, device=DEV)
     want = expected(s, H, start, which, left, 0, sinks, torch.full((B,), T, device=DEV))
     near({"y": torch.stack(rows, 1)}, {"y": want["y"]})
+
+
+def _operators():
+    """name -> (a differentiable input, the operator as a function of it)"""
+    g = torch.Generator(device=DEV).manual_seed(71)
+    r = lambda *s: torch.randn(*s, device=DEV, generator=g)  # noqa: E731
+    q, x = r(2, 9, 4, 16), r(10, 16)
+    rest = r(24, 16), r(24), r(2, 8, 16), r(2, 24, 8), torch.ones(2, device=DEV), torch.tensor([0, 4, 10], device=DEV, dtype=torch.int32), torch.tensor([1, 0], device=DEV, dtype=torch.int32)
+    return {"window_attention": (q, lambda t: window_attention(t, q, q, left=3, right=0)), "adapter_linear": (x, lambda t: adapter_linear(t, *rest))}
+
+
+@pytest.mark.parametrize("name", ["window_attention", "adapter_linear"])
+def test_compiled_programs_call_the_kernels(name):
+    x, f = _operators()[name]
+    leaf = x.clone().requires_grad_(True)
+    g = torch.compile(lambda t: f(t * 2) + 1, backend="eager")
+    assert torch.equal(g(x), f(x * 2) + 1) and torch.equal(g(x + 1), f((x + 1) * 2) + 1)
+    y = g(leaf)
+    assert torch.equal(torch.autograd.grad(y, leaf, torch.ones_like(y))[0], torch.autograd.grad(f(leaf * 2) + 1, leaf, torch.ones_like(y))[0])
