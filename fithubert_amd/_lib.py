@@ -7,6 +7,12 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+from typing import Iterable, Optional
+
+import torch   # (owns device memory and streams; also see lib())
+from torch.autograd import forward_ad
+
+_PROXY = torch._C._TorchDispatchModeKey.PROXY
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 # FH_LIB_PATH: another build of the SAME interface (same-box A/B of kernel changes, tools/scratch/ab.sh); the loader still checks
@@ -70,7 +76,6 @@ def lib() -> C.CDLL:
                 "(fithubert_amd has no CPU / eager fallback)")
         # torch owns device memory and streams: its HIP runtime (torch/lib/libamdhip64.so, same SONAME as ROCm's)
         # must be the one this library binds to, so torch is imported before the dlopen.
-        import torch  # noqa: F401
         _lib = C.CDLL(LIB_PATH)
         _declare(_lib)
     return _lib
@@ -244,6 +249,15 @@ def drop(p: float = 0.0, seed: int = 0, site: int = 0) -> Drop:
 def check(rc: int, what: str) -> None:
     if rc != 0:
         raise RuntimeError(f"{what} failed with code {rc}")
+
+
+def native_call(name: str, tensors: Iterable[Optional[torch.Tensor]]) -> None:
+    """Refuses, for an operator that calls the library past torch's dispatcher, what that call would answer wrongly without a word: a program that is being recorded from torch's own
+    operations would keep the outputs' allocation and no kernel (uninitialised values when it runs), a forward-mode derivative among `tensors` would be dropped."""
+    if torch._C._get_tracing_state() is not None or torch._C._get_dispatch_mode(_PROXY) is not None or torch._ops._get_dispatch_mode_pre_dispatch(_PROXY) is not None:
+        raise RuntimeError(f"{name} cannot be recorded (torch.jit.trace, make_fx): the program would hold its outputs without the kernels that write them")
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{name} has no forward-mode derivative")
 
 
 def operand(t_ptr, layout, ld, rpb=0, bstride=0, gstride=0, nseg=1, tshift=(0, 0), tvalid=0, segoff=(0, 0), seg1_limit=0):

@@ -59,6 +59,7 @@ def _forward(x, weight, bias, a, b, scaling, start, which):
 
 
 def _backward(x, weight, a, b, scaling, start, which, h, dy, need):
+    L.native_call("adapter_linear", (x, weight, a, b, scaling, dy))
     dt, dev = _DT[x.dtype], x.device
     if torch.cuda.current_device() != dev.index:
         with torch.cuda.device(dev):
@@ -100,7 +101,8 @@ def adapter_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.T
 
     K and N are multiples of 8; a rank that is no multiple of 8 is padded with zeros (copies of the factors in every call: better keep them padded), at
     most 128.  16-bit modes round x lora_a^T * scaling (backward: dy lora_b * scaling) to the element type, sums are fp32 and the
-    gradients of the factors leave fp32 sums rounded once.  ``weight``, ``bias`` and ``scaling`` take no gradient: one that requires it is refused."""
+    gradients of the factors leave fp32 sums rounded once.  ``weight``, ``bias`` and ``scaling`` take no gradient: one that requires it is refused.
+    The call cannot be recorded (torch.jit.trace, make_fx) and has no forward-mode derivative: both are refused."""
     if x.dim() < 2 or weight.dim() != 2 or lora_a.dim() != 3 or lora_b.dim() != 3:
         raise ValueError(f"x [..][K], weight [N][K], lora_a [n][R][K], lora_b [n][N][R]: got {tuple(x.shape)}, {tuple(weight.shape)}, {tuple(lora_a.shape)}, {tuple(lora_b.shape)}")
     (N, K), (n, R) = weight.shape, lora_a.shape[:2]
@@ -122,6 +124,7 @@ def adapter_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.T
     grad = torch.is_grad_enabled()
     if grad and (weight.requires_grad or scaling.requires_grad or (bias is not None and bias.requires_grad)):
         raise ValueError("the shared projection and the scalings are frozen: detach weight, bias and scaling")
+    L.native_call("adapter_linear", (x, weight, bias, lora_a, lora_b, scaling))
     if R % 8:
         lora_a, lora_b = F.pad(lora_a, (0, 0, 0, -R % 8)), F.pad(lora_b, (0, -R % 8))
     flat = _dense(x if x.dim() == 2 else x.reshape(-1, K))

@@ -14,6 +14,7 @@ chance with draws that are a function of (seed, place) alone.
 from __future__ import annotations
 
 from array import array
+from itertools import chain
 from operator import attrgetter
 from typing import List, Sequence, Tuple
 
@@ -62,6 +63,7 @@ def adamw_many(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mo
         raise ValueError(f"{len(params)} parameters and {len(grads)} gradients")
     if not params:
         return
+    L.native_call("adamw_many", chain(params, grads))
     with torch.no_grad():
         dev, pdt = params[0].device, params[0].dtype
         if pdt not in _DT or dev.type != "cuda":

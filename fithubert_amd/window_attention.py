@@ -82,6 +82,7 @@ def _forward(q, k, v, d, want_lse):
 
 
 def _backward(q, k, v, out, lse, dout, d):
+    L.native_call("window_attention", (q, k, v, dout))
     dt, dev = _DT[q.dtype], q.device
     if torch.cuda.current_device() != dev.index:
         with torch.cuda.device(dev):
@@ -127,7 +128,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, left:
     may reach rows near them that do not (0 x inf), one in a row's query or gradient the gradients of keys near those it sees.  ``scale`` > 0, default dh ** -0.5.
 
     16-bit modes round the probabilities (backward: and dS) to the element type in front of the second products; softmax and sums are fp32.  In fp16 a dS above
-    65504 is infinite and one below 2^-25 is 0: scale the loss so that gradients lie between.  Nothing depends on the order of atomics: equal calls give equal bits."""
+    65504 is infinite and one below 2^-25 is 0: scale the loss so that gradients lie between.  Nothing depends on the order of atomics: equal calls give equal bits.
+    The call cannot be recorded (torch.jit.trace, make_fx) and has no forward-mode derivative: both are refused."""
     if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
         raise ValueError(f"q [B][Tq][Hq][dh], k and v [B][Tk][Hkv][dh]: got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     if q.dtype not in _DT or k.dtype != q.dtype or v.dtype != q.dtype:
@@ -142,6 +144,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, left:
     scale = dh ** -0.5 if scale is None else float(scale)
     if not 0 < scale < float("inf"):
         raise ValueError(f"scale {scale}")
+    L.native_call("window_attention", (q, k, v))
     far = (1 << 31) - 1
     q, k, v = _aligned(q), _aligned(k), _aligned(v)
     key_len, q_start = _per_entry(key_len, B, q.device, "key_len"), _per_entry(q_start, B, q.device, "q_start")

@@ -232,3 +232,33 @@ def test_compiled_programs_call_the_kernels(name):
     assert torch.equal(g(x), f(x * 2) + 1) and torch.equal(g(x + 1), f((x + 1) * 2) + 1)
     y = g(leaf)
     assert torch.equal(torch.autograd.grad(y, leaf, torch.ones_like(y))[0], torch.autograd.grad(f(leaf * 2) + 1, leaf, torch.ones_like(y))[0])
+
+
+@pytest.mark.parametrize("name", ["window_attention", "adapter_linear"])
+def test_no_derivative_is_lost_and_no_trace_is_empty(name):
+    """Forward-mode derivatives and recorded programs: a native call would drop the one and leave the other with an output that nothing writes, so both are refused."""
+    import torch.autograd.forward_ad as fwAD
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, f = _operators()[name]
+    want = f(x)
+    leaf = x.clone().requires_grad_(True)
+    dy = torch.ones_like(want)
+    grad = torch.autograd.grad(f(leaf), leaf, dy)[0]
+    back = lambda t: torch.autograd.grad(f(t), t, dy)[0]  # noqa: E731
+    for nograd in (False, True):
+        with fwAD.dual_level(), torch.set_grad_enabled(not nograd):
+            for t in (x, leaf):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    f(fwAD.make_dual(t, torch.ones_like(x)))
+            assert torch.equal(f(x), want)                       # (no tangent: nothing to lose)
+    with fwAD.dual_level():
+        y = f(leaf)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(y, leaf, fwAD.make_dual(dy, dy))
+    for t, fn in ((x, f), (leaf, f), (leaf, back)):
+        with pytest.raises(RuntimeError, match="recorded"):
+            torch.jit.trace(fn, (t,), check_trace=False)
+        for kw in ({}, dict(pre_dispatch=True)):
+            with pytest.raises(RuntimeError, match="recorded"):
+                make_fx(fn, **kw)(t)
+    assert torch.equal(f(x), want) and torch.equal(back(leaf), grad)

@@ -157,3 +157,30 @@ def test_window_attention_refuses_limits():
     for kw in (dict(scale=0.0), dict(scale=float("inf")), dict(scale=float("nan"))):
         with pytest.raises(ValueError):
             window_attention(q, q, q, **kw)
+
+
+def test_native_calls_refuse_what_cannot_see_them():
+    """Forward-mode derivatives and recorded programs: a native call would drop the one and leave the other with an output that nothing writes."""
+    import torch.autograd.forward_ad as fwAD
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x = torch.ones(3)
+
+    def f(t):
+        L.native_call("f", (t, None))
+        return t.new_empty(3).fill_(2)
+    assert (f(x) == 2).all()
+    with fwAD.dual_level():
+        assert (f(x) == 2).all()
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            f(fwAD.make_dual(x, x))
+    with pytest.raises(RuntimeError, match="recorded"):
+        torch.jit.trace(f, (x,), check_trace=False)
+    for kw in ({}, dict(tracing_mode="fake"), dict(pre_dispatch=True)):
+        with pytest.raises(RuntimeError, match="recorded"):
+            make_fx(f, **kw)(x)
+    assert (f(x) == 2).all()
+    p = [torch.zeros(300)]
+    with fwAD.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        adamw_many([fwAD.make_dual(p[0], p[0])], p, adamw_moments(p), step=1, lr=1e-3)
+    with pytest.raises(RuntimeError, match="recorded"):
+        make_fx(lambda t: adamw_many([t], [t], adamw_moments([t]), step=1, lr=1e-3))(p[0])
