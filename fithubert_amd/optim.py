@@ -109,7 +109,8 @@ class ManyAdamW(torch.optim.Optimizer):
     """``torch.optim.AdamW`` in one launch per parameter group (and type), with ``bits`` = 32 or 8 bits per moment.
 
     The step count is the group's own (a parameter without a gradient is left out of a step and still shares the count).  ``step`` takes a
-    ``grad_scale`` (1 / (world * accumulation * loss scale)).  Sparse gradients and steps inside a graph capture are refused: the step number
+    ``grad_scale`` (1 / (world * accumulation * loss scale)).  The moments belong to a group's parameters, types and devices as its first step meets them: a later step or
+    ``state_dict`` with others is refused.  Sparse gradients and steps inside a graph capture are refused: the step number
     would be the same on every replay."""
 
     def __init__(self, params, lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, bits: int = 32):
@@ -120,15 +121,16 @@ class ManyAdamW(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, bits=bits, steps=0))
         self._moments = {}   # (group, device, type) -> [tensors, moments]
 
-    def _sets(self, k, group):
+    def _sets(self, k, group, anew=False):
         sets = {}
         for p in group["params"]:
             sets.setdefault((k, str(p.device), str(p.dtype)), []).append(p)
         for key, ps in sets.items():
             held = self._moments.get(key)
             if held is None or len(held[0]) != len(ps) or any(a is not b for a, b in zip(held[0], ps)):
-                if held is not None:
-                    raise RuntimeError("parameters were added to a group after its first step: add them as a group of their own")
+                if group["steps"] and not anew:   # (zero moments under a running count: its bias corrections would multiply the step)
+                    raise RuntimeError("a group's parameters changed after its first step: add new ones as a group of their own; where a type or a device changed, "
+                                       "make a new optimizer and load this one's state_dict (taken before the change) into it")
                 self._moments[key] = held = [ps, adamw_moments(ps, group["bits"])]
             yield held
 
@@ -172,7 +174,7 @@ class ManyAdamW(torch.optim.Optimizer):
         for k, (group, sets) in enumerate(zip(self.param_groups, saved)):
             if sets is None:
                 continue
-            here = list(self._sets(k, group))
+            here = list(self._sets(k, group, anew=True))
             if len(here) != len(sets):
                 raise ValueError(f"group {k}: the state holds {len(sets)} sets of moments, the parameters make {len(here)}")
             for (_, mine), theirs in zip(here, sets):

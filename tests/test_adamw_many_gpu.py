@@ -263,3 +263,22 @@ def test_copies_carry_the_moments_and_a_refused_step_counts_nothing(bits):
     ps[1].data = was
     step(opt)
     assert all(torch.equal(a, b) for a, b in zip(ps, twin.param_groups[0]["params"])) and opt.param_groups[0]["steps"] == 2
+
+
+def test_a_step_after_a_change_of_type_is_refused():
+    layer = torch.nn.Linear(20, 30).to(DEV)
+    opt = ManyAdamW(layer.parameters(), lr=1e-2)
+
+    def step():
+        for p in layer.parameters():
+            p.grad = torch.ones_like(p)
+        opt.step()
+    step()
+    layer.half()
+    held = [p.detach().clone() for p in layer.parameters()]
+    with pytest.raises(RuntimeError, match="changed"):
+        step()
+    assert all(torch.equal(p, h) for p, h in zip(layer.parameters(), held)) and opt.param_groups[0]["steps"] == 1
+    layer.float()
+    step()
+    assert opt.param_groups[0]["steps"] == 2

@@ -184,3 +184,29 @@ def test_native_calls_refuse_what_cannot_see_them():
         adamw_many([fwAD.make_dual(p[0], p[0])], p, adamw_moments(p), step=1, lr=1e-3)
     with pytest.raises(RuntimeError, match="recorded"):
         make_fx(lambda t: adamw_many([t], [t], adamw_moments([t]), step=1, lr=1e-3))(p[0])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_moments_do_not_start_anew_under_a_running_count(bits):
+    """Parameters that change type after their first step keep no moments that fit: going on with zeros and the old step number would multiply the step."""
+    layer = torch.nn.Linear(20, 30)
+    opt = ManyAdamW(layer.parameters(), bits=bits)
+    group = opt.param_groups[0]
+    list(opt._sets(0, group))                              # (what the first step does ...)
+    layer.double()                                         # nothing is lost before it has counted
+    layer.float()
+    list(opt._sets(0, group))
+    group["steps"] = 1                                     # (... and counts)
+    opt._moments[next(iter(opt._moments))][1][-1].fill_(3)
+    saved = opt.state_dict()
+    layer.bfloat16()
+    with pytest.raises(RuntimeError, match="changed"):
+        list(opt._sets(0, group))
+    with pytest.raises(RuntimeError, match="changed"):
+        opt.state_dict()
+    layer.float()
+    assert (list(opt._sets(0, group))[0][1][-1] == 3).all()
+    layer.bfloat16()
+    other = ManyAdamW(layer.parameters(), bits=bits)       # the way over: an optimizer of the new parameters that loads the state
+    other.load_state_dict(saved)
+    assert other.param_groups[0]["steps"] == 1 and (list(other._sets(0, other.param_groups[0]))[0][1][-1] == 3).all()
