@@ -59,10 +59,19 @@ def adamw_many(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mo
     to nearest once, so a change below half its spacing is lost.  ``seed`` draws the rounding of 8-bit moments: give each step its own
     (the step's number will do).  Runs on the current stream of the tensors' device; all scalars are part of the launch, so a captured
     call repeats the same ``step`` and ``seed`` on every replay."""
+    call = _checked(params, grads, moments, step, lr, betas, eps, weight_decay, grad_scale, seed)
+    if call is not None:
+        _launch(*call)
+
+
+def _checked(params, grads, moments, step, lr, betas, eps, weight_decay, grad_scale, seed):
+    """adamw_many up to its launch, every refusal included: what `_launch` takes (the gradients' contiguous copies among it), None where there is nothing to do"""
     if len(params) != len(grads):
         raise ValueError(f"{len(params)} parameters and {len(grads)} gradients")
+    if step < 1 or not all(0 <= b < 1 for b in betas):
+        raise ValueError(f"step {step} counts from 1, betas {betas} lie in [0, 1)")
     if not params:
-        return
+        return None
     L.native_call("adamw_many", chain(params, grads))
     with torch.no_grad():
         dev, pdt = params[0].device, params[0].dtype
@@ -70,7 +79,7 @@ def adamw_many(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mo
             raise ValueError(f"parameters are fp32, bf16 or fp16 tensors on the GPU, got {pdt} on {dev}")
         held = [g for g in grads if g is not None]
         if not held:
-            return
+            return None
         gdt = held[0].dtype
         if gdt not in _DT:
             raise ValueError(f"gradients are fp32, bf16 or fp16, got {gdt}")
@@ -95,14 +104,19 @@ def adamw_many(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mo
         want = [(torch.float32, nb * BLOCK)] * 2 if bits == 32 else [(torch.float8_e4m3fn, nb * BLOCK), (torch.float32, nb)] * 2
         if bits is None or any(t.dtype != d or t.numel() != k or t.device != dev or not t.is_contiguous() for t, (d, k) in zip(moments, want)):
             raise ValueError(f"moments do not fit the parameters ({nb} blocks on {dev}): make them with adamw_moments")
-        n = len(params)
         mp = [t.data_ptr() for t in moments]
+        if (mp[0] | mp[len(mp) // 2]) & 15:
+            raise ValueError("moments lie at multiples of 16 bytes")
         m, ms, v, vs = (mp[0], None, mp[1], None) if bits == 32 else mp
-        at, gat, sizes = array("Q", at), array("Q", gat), array("q", sizes)
-        with torch.cuda.device(dev):
-            L.check(L.lib().fh_adamw_many(_DT[pdt], _DT[gdt], at.buffer_info()[0], gat.buffer_info()[0], sizes.buffer_info()[0], n, bits, m, ms, v, vs, lr, betas[0],
-                                          betas[1], eps, weight_decay, step, grad_scale, seed & 0xFFFFFFFF, torch.cuda.current_stream(dev).cuda_stream), "fh_adamw_many")
-        torch.autograd.graph.increment_version(params if held is grads else [p for p, g in zip(params, held) if g is not None])
+        scalars = lr, betas[0], betas[1], eps, weight_decay, step, grad_scale, seed & 0xFFFFFFFF
+        return dev, (_DT[pdt], _DT[gdt]), array("Q", at), array("Q", gat), array("q", sizes), (bits, m, ms, v, vs), scalars, params, held, held is grads
+
+
+def _launch(dev, types, at, gat, sizes, moments, scalars, params, held, every):
+    with torch.cuda.device(dev):
+        L.check(L.lib().fh_adamw_many(*types, at.buffer_info()[0], gat.buffer_info()[0], sizes.buffer_info()[0], len(sizes), *moments, *scalars,
+                                      torch.cuda.current_stream(dev).cuda_stream), "fh_adamw_many")
+    torch.autograd.graph.increment_version(params if every else [p for p, g in zip(params, held) if g is not None])
 
 
 class ManyAdamW(torch.optim.Optimizer):
@@ -142,19 +156,25 @@ class ManyAdamW(torch.optim.Optimizer):
                 loss = closure()
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("ManyAdamW.step inside a graph capture would repeat one step number: call adamw_many with scalars of your own")
+        calls, steps = [], []   # (every refusal comes before the first launch: a refused step leaves all parameters, moments and counts)
         for k, group in enumerate(self.param_groups):
             if all(p.grad is None for p in group["params"]):
                 continue
             step = group["steps"] + 1
+            steps.append((group, step))
             for ps, moments in self._sets(k, group):
                 by = {}
                 for p in ps:
                     if p.grad is not None:
                         by.setdefault(p.grad.dtype, None)
                 for dt in by:   # one launch per gradient type; the others' tensors sit it out
-                    adamw_many(ps, [p.grad if p.grad is not None and p.grad.dtype == dt else None for p in ps], moments, step=step, lr=float(group["lr"]),
-                               betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], grad_scale=grad_scale, seed=step)
-            group["steps"] = step   # (a refused call leaves the count)
+                    calls.append(_checked(ps, [p.grad if p.grad is not None and p.grad.dtype == dt else None for p in ps], moments, step, float(group["lr"]), group["betas"],
+                                          group["eps"], group["weight_decay"], grad_scale, step))
+        for call in calls:
+            if call is not None:
+                _launch(*call)
+        for group, step in steps:
+            group["steps"] = step
         return loss
 
     def __getstate__(self):   # copies and pickles carry the moments too

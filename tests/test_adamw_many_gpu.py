@@ -282,3 +282,36 @@ def test_a_step_after_a_change_of_type_is_refused():
     layer.float()
     step()
     assert opt.param_groups[0]["steps"] == 2
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_refused_step_writes_nothing(bits):
+    """Several types of parameters and gradients, several groups: a refusal in any of them comes before the first launch."""
+    g = torch.Generator(device=DEV).manual_seed(16)
+    make = lambda n, dt: torch.nn.Parameter(torch.randn(n, device=DEV, generator=g).to(dt))  # noqa: E731
+    ps = [make(300, torch.float32), make(70, torch.bfloat16), make(600, torch.float32), make(40, torch.float32), make(50, torch.bfloat16)]
+    twins = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+    a, b = (ManyAdamW([{"params": t[:3]}, {"params": t[3:], "lr": 1e-3}], lr=1e-2, bits=bits) for t in (ps, twins))
+    grads = [torch.randn(p.shape, device=DEV, generator=g).to(p.dtype) for p in ps]
+
+    def step(opt, params):
+        for p, t in zip(params, grads):
+            p.grad = t.clone()
+        opt.step()
+    step(a, ps)
+    step(b, twins)
+    for i in (4, 2, 1):
+        held, moments = [p.detach().clone() for p in ps], a.state_dict()["moments"]
+        was = ps[i].data
+        ps[i].data = was.repeat_interleave(2)[::2]           # the same values, not contiguous
+        ps[i].grad = None
+        with pytest.raises(ValueError):
+            step(a, ps)
+        assert all(torch.equal(p, h) for p, h in zip(ps, held)) and [x["steps"] for x in a.param_groups] == [1, 1]
+        now = a.state_dict()["moments"]
+        assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for k in range(2) for m, n in zip(moments[k], now[k]) for x, y in zip(m, n))
+        ps[i].grad = None
+        ps[i].data = was
+    step(a, ps)
+    step(b, twins)
+    assert all(torch.equal(p, t) for p, t in zip(ps, twins)) and [x["steps"] for x in a.param_groups] == [2, 2]
