@@ -105,8 +105,8 @@ def _checked(params, grads, moments, step, lr, betas, eps, weight_decay, grad_sc
         if bits is None or any(t.dtype != d or t.numel() != k or t.device != dev or not t.is_contiguous() for t, (d, k) in zip(moments, want)):
             raise ValueError(f"moments do not fit the parameters ({nb} blocks on {dev}): make them with adamw_moments")
         mp = [t.data_ptr() for t in moments]
-        if (mp[0] | mp[len(mp) // 2]) & 15:
-            raise ValueError("moments lie at multiples of 16 bytes")
+        if nb and (len(set(mp)) != len(mp) or (mp[0] | mp[len(mp) // 2]) & 15):
+            raise ValueError("moments are tensors of their own, m and v at multiples of 16 bytes")
         m, ms, v, vs = (mp[0], None, mp[1], None) if bits == 32 else mp
         scalars = lr, betas[0], betas[1], eps, weight_decay, step, grad_scale, seed & 0xFFFFFFFF
         return dev, (_DT[pdt], _DT[gdt]), array("Q", at), array("Q", gat), array("q", sizes), (bits, m, ms, v, vs), scalars, params, held, held is grads

@@ -315,3 +315,13 @@ def test_a_refused_step_writes_nothing(bits):
     step(a, ps)
     step(b, twins)
     assert all(torch.equal(p, t) for p, t in zip(ps, twins)) and [x["steps"] for x in a.param_groups] == [2, 2]
+
+
+def test_one_tensor_is_not_two_moments():
+    p, g = torch.ones(300, device=DEV), torch.ones(300, device=DEV)
+    for bits in (32, 8):
+        m = adamw_moments([p], bits)
+        for bad in (dict(step=0), dict(step=1, betas=(0.9, 1.0)), dict(step=1, betas=(-0.1, 0.9)), dict(step=1, moments=m[:len(m) // 2] * 2)):
+            with pytest.raises(ValueError):
+                adamw_many([p], [g], lr=1e-3, **dict(dict(moments=m), **bad))
+        assert (p == 1).all() and all((t.view(torch.uint8) == 0).all() for t in m)
