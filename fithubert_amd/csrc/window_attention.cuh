@@ -841,8 +841,8 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_dq_kernel(WinArgs 
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dk, dv
-// A workgroup owns 64 KT keys (16 KT per wave) of one key head and walks the 64-row tiles that see them: nkb blocks per head without sinks, and
-// nsplit workgroups (partial sums) for each of the nsink blocks that hold them.
+// A workgroup owns 64 KT keys (16 KT per wave) of one key head and walks the 64-row tiles that see them: nkb blocks per head, and where the blocks that hold sinks are
+// shared (nsink of them) nsplit workgroups with partial sums for each.
 template <typename T, int NDT, int KT>
 __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_dkv_kernel(WinArgs a, const T* __restrict__ q_, const T* __restrict__ k_, const T* __restrict__ v_,
                                                       const T* __restrict__ dout, const float* __restrict__ lse, const float* __restrict__ delta,
@@ -853,7 +853,7 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_dkv_kernel(WinArgs
   constexpr bool DMA = sizeof(T) == 2;
   float* rowdata = reinterpret_cast<float*>(lds + 4 * W::TILE);   // two buffers of 64 x (lse | -D)
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
-  // one dimension: all blocks without sinks first (each XCD a contiguous range: neighbours read the same rows), then the sink blocks' shares, which are
+  // one dimension: all blocks that are not shared first (each XCD a contiguous range: neighbours read the same rows), then the sink blocks' shares, which are
   // short and fill the CUs that the last round of the others leaves idle
   const int heads = a.B * a.Hkv, whole = heads * nkb, lin = blockIdx.x;
   const bool shared = lin >= whole;

@@ -14,7 +14,7 @@ struct WinArgs {
   int rows;                        // Tq * G
   unsigned magic;                  // floor(2^32 / G) + 1 (G = 1: 0)
   int nsplit;                      // forward: workgroups that share a row block's keys; dk / dv: that share a sink block's rows
-  int nsink;                       // dk / dv: key blocks that hold sinks
+  int nsink;                       // dk / dv: key blocks that hold sinks, where several workgroups share each
   // frame of a row (row < 2^29: the product is at most one too large)
   __device__ __forceinline__ int frame(int row) const {
     if (magic == 0u) return row;
@@ -49,11 +49,17 @@ static inline WinPlan fwd_plan(const WinArgs& a, int dtype) {
   p.nsplit = n < 2 ? 1 : n > 256 ? 256 : (int)n;
   return p;
 }
-// sink blocks (of `keys` keys) and the workgroups that share each one's rows
+// Sink blocks (of `keys` keys) and the workgroups that share each one's rows: one per 1024 rows, but no more than four per CU in all -- where sinks are many their blocks fill the chip
+// by themselves, and the shares' partial sums would only be written and read (30001 frames, all of them sinks, 4 key heads: 3.9 GB).  A block that nobody shares is
+// one like the others: no partial sums, no join.
 static inline void bwd_sinks(WinArgs& a, int keys) {
   a.nsink = (a.sinks + keys - 1) / keys;
+  const long blocks = (long)a.B * a.Hkv * a.nsink, fill = blocks > 0 ? (1023 + blocks) / blocks : 1;
   long n = (a.rows + 1023) / 1024;
-  a.nsplit = n < 1 ? 1 : n > 64 ? 64 : (int)n;
+  if (n > 64) n = 64;
+  if (n > fill) n = fill;
+  if (n < 2) a.nsink = 0;
+  a.nsplit = n < 2 ? 1 : (int)n;
 }
 // 16-key (16-row) tiles per wave of the backward passes: two where that still gives every CU two workgroups, and where the accumulators fit
 static inline int bwd_tiles(const WinArgs& a, int dtype, long blocks128, bool dkv) {

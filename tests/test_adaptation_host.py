@@ -210,3 +210,19 @@ def test_moments_do_not_start_anew_under_a_running_count(bits):
     other = ManyAdamW(layer.parameters(), bits=bits)       # the way over: an optimizer of the new parameters that loads the state
     other.load_state_dict(saved)
     assert other.param_groups[0]["steps"] == 1 and (list(other._sets(0, other.param_groups[0]))[0][1][-1] == 3).all()
+
+
+@pytest.mark.parametrize("sinks", [1, 64, 1000, 30001])
+@pytest.mark.parametrize("B,Hq,Hkv,T", [(1, 16, 4, 30001), (8, 16, 16, 30001), (64, 12, 12, 1500), (2, 12, 12, 499)])
+def test_window_attention_workspace_stays_in_proportion(B, Hq, Hkv, T, sinks):
+    """The sink blocks' partial sums: no more workgroups than fill the chip share them, so the workspace is at most 1024 blocks of 128 keys (dk and dv, fp32) beside D,
+    and nothing where no block is shared."""
+    sinks = min(sinks, T)
+    for dtype in (0, 1, 2):
+        d = _win(B=B, Tq=T, Tk=T, Hq=Hq, Hkv=Hkv, left=1023, sinks=sinks, q_bs=T * Hq * 64, q_ts=Hq * 64, k_bs=T * Hkv * 64, k_ts=Hkv * 64, v_bs=T * Hkv * 64, v_ts=Hkv * 64)
+        n = L.lib().fh_window_attention_scratch_bytes(dtype, C.byref(d), 1)
+        rows = B * T * Hq * 4
+        blocks = B * Hkv * -(-sinks // 64)
+        assert rows <= n <= rows + 16 + (1024 + blocks) * 128 * 2 * 64 * 4, (dtype, n)
+        if blocks >= 1024 * 2 or T * (Hq // Hkv) <= 1024:
+            assert n <= rows + 16, (dtype, n)
