@@ -325,3 +325,34 @@ def test_one_tensor_is_not_two_moments():
             with pytest.raises(ValueError):
                 adamw_many([p], [g], lr=1e-3, **dict(dict(moments=m), **bad))
         assert (p == 1).all() and all((t.view(torch.uint8) == 0).all() for t in m)
+
+
+def test_optimizer_with_8_bit_moments_moves_as_torch_does():
+    """The first step reads no code (its moments are zero): as torch's but for fp32 roundings.  Each later one reads m and r = sqrt(v) as e4m3 codes, rounded by chance: off by at most half
+    a code's spacing of 2^-3 in rms, 1/16.  m carries 5 such errors, each weighed by 0.9 a step: 0.106 of it; r's reach v doubled, 5 of them: 0.28 of v, 0.14 of r; together 0.18 of
+    each step.  The gradients keep their direction, so the steps add up and the movement |t - start| is off by no more than that in norm; 0.25 is allowed.  (No step at all: 1.  The wrong way: 2.  A rate
+    1.3 times too large: 0.3.)"""
+    shapes = [(40, 33), (300,), (7, 5, 13), (1000,)]
+    g = torch.Generator(device=DEV).manual_seed(5)
+    start = [torch.randn(s, device=DEV, generator=g) for s in shapes]
+    mine, theirs = ([p.clone().requires_grad_(True) for p in start] for _ in range(2))
+    groups = lambda ps: [{"params": ps[:2], "lr": 1e-2}, {"params": ps[2:], "weight_decay": 0.0}]  # noqa: E731
+    a = ManyAdamW(groups(mine), lr=1e-3, betas=(0.9, 0.99), weight_decay=0.1, bits=8)
+    b = torch.optim.AdamW(groups(theirs), lr=1e-3, betas=(0.9, 0.99), weight_decay=0.1)
+    sched = [torch.optim.lr_scheduler.LambdaLR(o, lambda k: 1 / (k + 1)) for o in (a, b)]
+    base = [torch.randn(s, device=DEV, generator=g) for s in shapes]
+    for k in range(6):
+        for p, t, d in zip(mine, theirs, base):
+            p.grad = d + 0.3 * torch.randn(d.shape, device=DEV, generator=g)
+            t.grad = p.grad.clone()
+        rates = [group["lr"] for group in a.param_groups]
+        a.step()
+        b.step()
+        for s in sched:
+            s.step()
+        for i, (p, t, s) in enumerate(zip(mine, theirs, start)):
+            p, t, s = p.detach().double(), t.detach().double(), s.double()
+            if k == 0:   # the decay and the sum round p twice each, the quotient and the rate 16 times 2^-24 of the step
+                assert ((p - t).abs() <= 4 * 2.0 ** -24 * s.abs() + 32 * 2.0 ** -24 * rates[i // 2]).all(), i
+            else:
+                assert (p - t).norm() < 0.25 * (t - s).norm(), (k, i)
