@@ -188,17 +188,24 @@ class ManyAdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         d = dict(state_dict)
+        if "moments" not in d:
+            raise ValueError("a state of ManyAdamW's own: this one holds no 'moments'")
         saved = d.pop("moments")
-        super().load_state_dict(d)
-        self._moments = {}
-        for k, (group, sets) in enumerate(zip(self.param_groups, saved)):
-            if sets is None:
-                continue
-            here = list(self._sets(k, group, anew=True))
-            if len(here) != len(sets):
-                raise ValueError(f"group {k}: the state holds {len(sets)} sets of moments, the parameters make {len(here)}")
-            for (_, mine), theirs in zip(here, sets):
-                if [(t.shape, t.dtype) for t in mine] != [(t.shape, t.dtype) for t in theirs]:
-                    raise ValueError(f"group {k}: the state's moments do not fit the parameters")
-                for a, b in zip(mine, theirs):
-                    a.copy_(b)
+        before = {n: self.__dict__[n] for n in ("state", "param_groups", "_moments")}
+        try:
+            super().load_state_dict(d)
+            self._moments = {}
+            for k, (group, sets) in enumerate(zip(self.param_groups, saved)):
+                if sets is None:
+                    continue
+                here = list(self._sets(k, group, anew=True))
+                if len(here) != len(sets):
+                    raise ValueError(f"group {k}: the state holds {len(sets)} sets of moments, the parameters make {len(here)}")
+                for (_, mine), theirs in zip(here, sets):
+                    if [(t.shape, t.dtype) for t in mine] != [(t.shape, t.dtype) for t in theirs]:
+                        raise ValueError(f"group {k}: the state's moments do not fit the parameters")
+                    for a, b in zip(mine, theirs):
+                        a.copy_(b)
+        except BaseException:   # (what was there goes on: not the new counts over moments of zeros)
+            self.__dict__.update(before)
+            raise

@@ -226,3 +226,22 @@ def test_window_attention_workspace_stays_in_proportion(B, Hq, Hkv, T, sinks):
         assert rows <= n <= rows + 16 + (1024 + blocks) * 128 * 2 * 64 * 4, (dtype, n)
         if blocks >= 1024 * 2 or T * (Hq // Hkv) <= 1024:
             assert n <= rows + 16, (dtype, n)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_refused_state_leaves_the_optimizer(bits):
+    make = lambda *sizes: ManyAdamW([{"params": [torch.nn.Parameter(torch.zeros(n)) for n in s]} for s in sizes], bits=bits)  # noqa: E731
+    opt, other = make((300, 7), (600,)), make((300, 7), (900,))
+    for o, x in ((opt, 3), (other, 4)):
+        for k, group in enumerate(o.param_groups):
+            for _, moments in list(o._sets(k, group)):
+                moments[-1].fill_(x)
+            group["steps"] = x
+    with pytest.raises(ValueError):
+        opt.load_state_dict(other.state_dict())
+    without = {k: v for k, v in other.state_dict().items() if k != "moments"}
+    with pytest.raises(ValueError):                        # (torch.optim.AdamW's, say)
+        opt.load_state_dict(without)
+    assert [g["steps"] for g in opt.param_groups] == [3, 3]
+    for k, group in enumerate(opt.param_groups):
+        assert all((m[-1] == 3).all() for _, m in opt._sets(k, group))
