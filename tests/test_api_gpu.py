@@ -692,3 +692,40 @@ def test_layerwise_distillation_behind_a_tr_conv_in_the_middle_of_the_stack(rec_
     check(sm.engine.param_views(sm.engine.grads), "training_step")
     v = task.validation_step(b)["v_loss"]
     assert v == v and abs(v.item() - lo.item()) < 5e-2 * abs(lo.item())             # eval forward = the training forward at dropout 0
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bf16", "float16"])
+def test_a_forward_beside_the_teacher_has_the_bits_of_one_alone(dtype):
+    """The student's forward while the frozen teacher's runs on its own stream (what every training step does) against the same forward on an idle GPU: nothing is shared, so every
+    activation is the same bit for bit -- conv 0's fp32 output was not, now and then, while its unit was compiled with packed fp32 arithmetic."""
+    import copy
+    cfg = yaml.safe_load(open(os.path.join(ROOT, "conf", "fithubert.yaml")))
+    cfg["distiller"].update(encoder_layers=2, dropout=0.0, attention_dropout=0.0, activation_dropout=0.0, dropout_input=0.0)
+    cfg["train"].update(distil_random_layer=1)
+    from fithubert_amd.dataset import fixed_length_batch
+    from fithubert_amd.distill import W2V2Distil
+    from fithubert_amd.teacher import TeacherConfig
+    tc = TeacherConfig.base("hubert")
+    tc.encoder_layers = 2
+    task = W2V2Distil(copy.deepcopy(cfg), dtype=dtype, device=DEV, teacher_cfg=tc, seed=3, teacher_native_frontend=True)
+    forward = lambda b: task.engine.forward(b["x"], None, training=2, heads_on=task.student_model._heads_on, seed=1)  # noqa: E731
+    names = ["c0_mean", "c0_rstd", "y0"] + [f"{n}{i}" for i in range(1, len(task.engine.cfg.conv_layers())) for n in "zy"]
+    names += ["ln0", "features", "x0", "psum", "x1", "qkv", "attn", "xa", "h", "xo", "pred"]
+    for batch in (fixed_length_batch(2, 16000, seed=200, device=DEV), fixed_length_batch(8, 16000, seed=201, device=DEV)):
+        for _ in range(2):                   # (the first passes measure GEMM loops)
+            task.teacher_hiddens(batch)
+            forward(batch)
+        torch.cuda.synchronize()
+        hid = task.teacher_hiddens(batch)
+        torch.cuda.synchronize()
+        ws = forward(batch)
+        torch.cuda.synchronize()
+        want = {n: ws.view(n).clone() for n in names}
+        for k in range(20):
+            got, ev = task._teacher_async(batch)
+            ws = forward(batch)
+            torch.cuda.current_stream().wait_event(ev)
+            torch.cuda.synchronize()
+            for n in names:
+                assert torch.equal(ws.view(n), want[n]), (n, k)
+            assert torch.equal(got, hid), k

@@ -121,3 +121,12 @@ def test_gemm_table_roundtrip(tmp_path):
     assert sorted(zip(k2, p2, s2)) == sorted(zip(keys, paths, sks))
     lib.fh_gemm_tune(-1)
     assert L.load_gemm_table(str(tmp_path / "missing.json")) == 0
+
+
+def test_units_are_compiled_without_packed_fp32_arithmetic():
+    """v_pk_add / mul / fma_f32 give wrong results now and then (conv 0's fp32 forward beside another stream's work): all units but the 16-bit GEMM loops are built without them."""
+    import glob
+    from fithubert_amd import build
+    units = {os.path.basename(f) for f in glob.glob(os.path.join(build.CSRC, "*.hip"))}
+    packed = {u for u in units if "-packed-fp32-ops" not in build.file_flags(u)}
+    assert packed == {"gemm_bf16.hip", "gemm_f16.hip"} and "conv0.hip" in units

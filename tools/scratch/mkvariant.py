@@ -15,7 +15,7 @@ else:
     for spec in sys.argv[2:]:
         unit, _, flags = spec.partition(":")
         o = f"/tmp/var_{name}_{unit}.o"
-        cmd = [B.HIPCC] + B.FLAGS + list(B.FILE_FLAGS.get(unit, ())) + [f for f in flags.split(",") if f] + ["-c", os.path.join(B.CSRC, unit), "-o", o]
+        cmd = [B.HIPCC] + B.FLAGS + list(B.file_flags(unit)) + [f for f in flags.split(",") if f] + ["-c", os.path.join(B.CSRC, unit), "-o", o]
         subprocess.run(cmd, check=True, stderr=subprocess.DEVNULL)
         objs[unit] = o
     subprocess.run([B.HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", out] + list(objs.values()), check=True)
