@@ -13,15 +13,16 @@
 // instead of v because an e4m3 code spans 2^-9 .. 448 = 18.8 binades: for v itself that would lose elements whose gradients are
 // 700 times smaller than their block's largest, for the root 5 * 10^5 times.  What is rounded is the new moment in fp32 -- the
 // parameter moves by the unrounded one --, and it is rounded UP with the probability of its fraction: rounded to nearest, an
-// average whose step (1 - b2) is far below a code's spacing of 1/16 would never leave its code.  The draws are 16 bits each of one
+// average whose step (1 - b2) is far below a code's spacing of 1/16 would never leave its code.  That keeps the average of r, not of v = r^2, which gains the
+// rounding's variance: under steady gradients v is held 1 % (b2 = 0.9) to 5 % (0.98, 0.99) too large on average and stays there, so steps are up to 2.5 % shorter.  The draws are 16 bits each of one
 // hash of (seed, place), so a step can be repeated.  A root that is not zero never becomes zero (it divides).  An element that is
 // not finite is held as the code's NaN and does not enter its block's scale: it harms itself alone, as it would in 32 bits.
 // This file is compiled without contraction into fused multiply-adds: codes are a discontinuous function of the moments, and this
 // way each is the same on every path and in any restatement that follows the formulas in fp32.
 //
 // Bound by HBM: 28 bytes per fp32 element with fp32 gradients and 32-bit moments, 16.06 with 8-bit ones, 10.06 with bf16 parameters and
-// gradients.  Measured (a copy runs at 5.2 TB/s): 300 M bf16 parameters, 8-bit moments, 380 tensors: 600 us = 5.0 TB/s; 30 M fp32
-// parameters, 8-bit moments, 200 tensors: 102 us = 4.8 TB/s of kernel time (two launches).  With the compiler's IEEE division and square
+// gradients.  Measured (a copy runs at 5.0 to 5.2 TB/s): 300 M bf16 parameters, 8-bit moments, 380 tensors: 596 us = 5.1 TB/s; 30 M fp32
+// parameters, 8-bit moments, 200 tensors: 87 us of kernel time (two launches; 5.6 TB/s, some of its 488 MB stay in the last cache from pass to pass).  With the compiler's IEEE division and square
 // root, a software rounding to e4m3 and four elements per lane everywhere the first took 934 us: the arithmetic was the bound, not the bytes.
 #include "common.cuh"
 #include "kernels.h"

@@ -10,9 +10,11 @@
 //         GEMM's residual operand.
 // outer:  dA and dB in one launch: a workgroup owns 64 columns of one adapter's factor and walks that adapter's rows, whichever segments they lie in, 32
 //         at a time per wave; long walks are dealt over several workgroups whose partial sums are added in order (no atomics).
-// Measured, forward and backward of 16384 x 1024 -> 4096, rank 16, 4 adapters, 32 requests, bf16: h 10 us, y 131 (1.05 PFLOP/s), turn 5, G 36 (134 MB, 3.7 TB/s), dx 133,
-// dA and dB 26 + 5.  Forward of 9973 x 480 -> 1440, rank 8: 6 + 25.5 us -- 234 tiles of 256 x 256 for 256 CUs, each with eight steps of K: bound by filling and emptying
-// one tile.  32 one-row requests, 768 -> 768, fp16: 4.7 + 6.9 us.  fp32, 1497 x 480 -> 480, rank 32, both directions: 73 us of kernels (y 19, dx 21, the rest 4 to 8 each).
+// Rounding in 16-bit modes: h and G, which are the next products' operands.  Sums are fp32 and y (dx) is rounded once where the adapters' part is added inside the projection's product;
+// where it is added as a residual (see `project`) the part itself is rounded once more on its way.
+// Measured, warm, forward and backward of 16384 x 1024 -> 4096, rank 16, 4 adapters, 32 requests, bf16: h 11 us, y 122 (1.12 PFLOP/s of the projection alone), turn 5, G 45 (134 MB, 3.0 TB/s), dx 121,
+// dA and dB 26 + 5; the call 322.  Forward of 9973 x 480 -> 1440, rank 8: 6 + 27 us, the call 28 -- 234 tiles of 256 x 256 for 256 CUs, each with eight steps of K: bound by filling and emptying
+// one tile.  32 one-row requests, 768 -> 768, fp16: 4.9 + 6.7 us.  fp32, 1497 x 480 -> 480, rank 32, both directions: 70 us of kernels (y 19, dx 21, the rest 4 to 8 each).
 #include "gemm_loops.cuh"
 #include "kernels.h"
 #include "attn_frag.cuh"
@@ -690,7 +692,8 @@ size_t partial_bytes(const fh_adapter_desc* d) { return outer_bytes(d, d->K) + o
 
 template <typename T> int down(const Segs& g, const void* x, const void* f, void* out, int K, int R, hipStream_t st) {
   if (g.M == 0) return 0;
-  // 32-row tiles where they still fill the chip twice over and requests are long enough to share them (16384 x 4096, rank 16: 50 -> 36 us)
+  // 32-row tiles where they still fill the chip twice over (two workgroups per CU: 16384 rows, the only size measured, 4096 columns, rank 16: 50 -> 36 us) and requests are
+  // long enough on average to share them
   const bool wide = g.M >= 16384 && R <= 64 && (long)g.n * 64 <= g.M;
   const int tile = wide ? 32 : 16, tiles = (g.M + tile - 1) / tile;
   const long per = 1 + ((long)tile * g.n + g.M - 1) / g.M;   // segments that a tile touches
@@ -736,10 +739,11 @@ template <typename T> int outer(const fh_adapter_desc* d, const void* G, const v
 //   few rows (forward)        adapter_few_kernel, by its number of workgroups: with the whole of h's kernel, bf16 and rank 16, us against the next line's:
 //                             1 x 480 -> 1440 7.2 | 18, 256 x 4096 -> 1024 35 | 44 (256 workgroups), 512 x 480 -> 1440 12.7 | 12.4 (720), 512 x 1024 -> 4096 48 | 35
 //                             (2048), but 56 | 56 with one-row requests; fp32: 512 x 4096 -> 1024 98 | 131 (512), 1024 x 768 -> 768 36 | 33 (768)
-//   requests under 16 rows    the part on its own first (16-row tiles, many of them), then the GEMM's residual operand: a large tile would walk its requests one by one
+//   requests under 16 rows    (on average) the part on its own first (16-row tiles, many of them), then the GEMM's residual operand: a large tile would walk its requests one by one.
+//                             In 16-bit modes the part is rounded to the element type in between, off by half a step of itself, beside y's own rounding
 //   fp32                      adapter_gemm_f32_kernel
 //   16-bit                    inside the GEMM: the 256 x 256 8-phase loop where its tiles give work to a good part of the CUs, else the 64 x 64 one-trip loop (it takes W by
-//                             its rows: forward only; a small backward goes as short requests do)
+//                             its rows: forward only; a small backward -- under 96 tiles, or N under 128 -- goes as short requests do, with their rounding of the part)
 template <typename T, int YL>
 int project(int dtype, const fh_adapter_desc* d, GemmParams& p, const void* h, const void* f, hipStream_t st) {
   const Segs g = segs_of(d);

@@ -17,12 +17,12 @@
 // window borders).  The blocks that hold sinks see every later row: their rows are dealt over several workgroups and joined.
 // Two passes cost 7 products instead of 5, but no atomics: results repeat bit for bit.
 //
-// Bound: vector issue.  Counted with four cycles per vector instruction and sixteen per exponential, the forward's instructions take all of its time, more than half of it
-// the exponentials'; dq's 88 %, beside 43 % of the matrix pipe; dk / dv's 55 % and 37 %: two waves per SIMD (its accumulators) leave gaps.  Measured, 30001 frames, 16 heads over 4, 64 channels, 1024 keys per
-// row, bf16: forward 226 us (0.57 PFLOP/s of its two products), dq 249 (0.77 of three), dk / dv 360 + 7 (0.71 of four).  8 x 375 frames, 12 heads of 40
-// channels, window 64 + 64: 10, 11, 12 us.  fp32, 2 x 499 frames: 23, 29, 51 + 4 us.  Streams are bound by the cache's bytes and the length of a wave's
-// chain: one fp16 frame of 64 entries, 4 key heads, 1028 keys: 15 us (68 MB, 4.5 TB/s); 16 frames against 65536 keys of 128 channels: 25.5 + 5 us (67 MB, 3.3 TB/s
-// with the partial sums' 17 MB).
+// Bound, 30001 frames, 16 heads over 4, 64 channels, 1024 keys per row, bf16, by the counters: the forward's vector instructions occupy 76 % of its SIMD cycles (9.6 per score, of which the
+// MFMAs and the exponentials are 1.1 each), beside 31 % of the matrix pipe; dq's 63 % and 43 %; dk / dv's 40 % and 37 %: two waves per SIMD (its accumulators) leave gaps.
+// Measured there, warm, after 60 passes: forward 185 us (0.68 PFLOP/s of its two products), dq 210 (0.90 of three), dk / dv 292 + 6 (0.86 of four); the call 691.  8 x 375 frames, 12 heads
+// of 40 channels, window 64 + 64: 10, 11, 11 us.  fp32, 2 x 499 frames: 22, 29, 49 us.  Streams are bound by the cache's bytes and the length of a wave's
+// chain: one fp16 frame of 64 entries, 4 key heads, 1028 keys: 15.6 us (68 MB, 4.3 TB/s); 16 frames against 65536 keys of 128 channels: 24 + 5 us (67 MB, 3.5 TB/s
+// with the partial sums' 17 MB).  (The comparisons of variants further down were taken a few passes after an idle GPU, where the same kernels take about a quarter longer.)
 #pragma once
 #include "window_attention.h"
 #include "attn_frag.cuh"
@@ -73,8 +73,8 @@ template <typename T> __device__ __forceinline__ uint32_t pack_pair(float a, flo
   }
 }
 
-// The second products' operand, a 16-row accumulator tile at a time.  16-bit modes round the probabilities (or dS) to the element type here: off by at most
-// 2^-8 (bf16), 2^-11 (fp16) of each; they are packed as soon as they exist, which halves the registers that wait for the other half.
+// The second products' operand, a 16-row accumulator tile at a time.  16-bit modes round the probabilities (or dS) to the element type here, the matrix pipe's rate for
+// the second products: off by at most 2^-8 (bf16), 2^-11 (fp16) of each; they are packed as soon as they exist, which halves the registers that wait for the other half.
 template <typename T> struct Half2 {
   typedef uint2 type;
   static __device__ __forceinline__ uint2 pack(const f32x4& p) { return make_uint2(pack_pair<T>(p[0], p[1]), pack_pair<T>(p[2], p[3])); }
@@ -753,7 +753,7 @@ __global__ void __launch_bounds__(256, (WT<T, NDT>::OCC)) win_dq_kernel(WinArgs 
 #pragma unroll
       for (int e = 0; e < W::VEC; ++e) d = fmaf(fx[e], fy[e], d);
     }
-    dl[t] = xor_sum(d);
+    dl[t] = xor_sum(d);   // (of the rounded output: in 32 bits it would cost its bytes again in both directions)
     if (live && q == 0) delta[orow] = -dl[t];   // (as the other pass wants it)
   }
   __syncthreads();

@@ -119,7 +119,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, left:
     """softmax(scale q k^T over the visible keys) v -> [B][Tq][Hq][dh].
 
     ``q`` [B][Tq][Hq][dh], ``k``, ``v`` [B][Tk][Hkv][dh]: fp32, bf16 or fp16 on one GPU, dh a multiple of 8 up to 128, Hq a multiple of Hkv (query head h
-    reads key head h // (Hq // Hkv)).  Any strides with contiguous channels -- slices of a packed q|k|v projection, a cache longer than it is
+    reads key head h // (Hq // Hkv)), up to 65535 entries.  Any strides with contiguous channels -- slices of a packed q|k|v projection, a cache longer than it is
     filled -- are read in place when addresses and strides are multiples of 16 bytes, copied otherwise.
 
     Query i of entry b stands at position p = ``q_start[b]`` + i (default 0; required as soon as Tq != Tk) and sees key s when s < ``key_len[b]``
@@ -127,7 +127,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, left:
     gives zeros and takes part in no gradient.  Keys that no row of the call sees may hold anything; an infinity or NaN in a key that some rows see
     may reach rows near them that do not (0 x inf), one in a row's query or gradient the gradients of keys near those it sees.  ``scale`` > 0, default dh ** -0.5.
 
-    16-bit modes round the probabilities (backward: and dS) to the element type in front of the second products; softmax and sums are fp32.  In fp16 a dS above
+    16-bit modes round the probabilities (backward: and dS) to the element type in front of the second products, and the backward pass takes sum(dout out) from the rounded
+    output; softmax and sums are fp32.  In fp16 a dS above
     65504 is infinite and one below 2^-25 is 0: scale the loss so that gradients lie between.  Nothing depends on the order of atomics: equal calls give equal bits.
     The call cannot be recorded (torch.jit.trace, make_fx) and has no forward-mode derivative: both are refused."""
     if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:

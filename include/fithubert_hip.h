@@ -268,14 +268,14 @@ int fh_attention_backward_bias(int dtype, const void* qkv, const void* out, cons
  * q [B][Tq][Hq][dh], k, v [B][Tk][Hkv][dh] by the strides below (elements, not negative; channels contiguous; addresses and strides multiples
  * of 16 bytes; frames and heads at most 2^23 elements apart), so a packed q|k|v projection or a longer cache is read in place; query head h reads key head h / (Hq / Hkv).
  * out, dout, dq [B][Tq][Hq][dh] and dk, dv [B][Tk][Hkv][dh] are contiguous; lse: B * Tq * Hq floats that the backward reads (forward: NULL
- * when there is none).  dq, dk, dv are written, not added to (keys that no row sees: 0).  dh <= 128, a multiple of 8; 16-bit modes round the
- * probabilities and dS = scale P (dP - D) to the element type before the second products (fp16: finite up to 65504), sums and softmax are fp32.  No atomics: results repeat bit for bit.
+ * when there is none).  dq, dk, dv are written, not added to (keys that no row sees: 0).  dh <= 128, a multiple of 8; 16-bit modes take D
+ * from the rounded out and round the probabilities and dS = scale P (dP - D) to the element type before the second products (fp16: finite up to 65504), sums and softmax are fp32.  No atomics: results repeat bit for bit.
  * scratch: fh_window_attention_scratch_bytes(dtype, d, 0 forward | 1 backward) bytes, 16-byte aligned (0: NULL will do).  A few rows
  * against long caches are split over the keys and joined through it.
  * ------------------------------------------------------------------------------------------ */
 typedef struct {
   int B, Tq, Tk, Hq, Hkv, dh;
-  int left, right, sinks; /* left / right < 0: no limit on that side */
+  int left, right, sinks; /* left / right < 0, or 2^31 - 1: no limit on that side */
   float scale;
   const int* key_len;     /* device [B], clipped to [0, Tk]; NULL: Tk */
   const int* q_start;     /* device [B]; NULL: 0 */
@@ -297,7 +297,8 @@ int fh_window_attention_backward(int dtype, const fh_window_attention_desc* d, c
  * [0, n_adapters), rows in front of the first and behind the last segment: the shared projection alone.  Several segments may name one
  * adapter.  h [M][R] (dtype) receives scaling[a] x A_a^T, 0 on rows without an adapter: what the backward reads.
  * Backward (W and bias are frozen): dx = dy W + G A_a with G = scaling[a] dy B_a; da = sum G^T x; db = sum dy^T h -- in the element type,
- * written, 0 for an adapter without rows.  dx, da or db may be NULL.  16-bit modes round h and G to the element type, sums are fp32; no atomics.
+ * written, 0 for an adapter without rows.  dx, da or db may be NULL.  16-bit modes round h and G to the element type -- and
+ * the adapters' part of y (dx) where it is added to the projection's product in a launch of its own: short segments, small backward passes --, sums are fp32; no atomics.
  * K, N, R multiples of 8, R <= 128; every tensor contiguous and 16-byte aligned.
  * scratch: fh_adapter_scratch_bytes(dtype, d, 0 forward | 1 backward) bytes, 16-byte aligned (0: NULL will do).
  * ------------------------------------------------------------------------------------------ */
@@ -368,7 +369,7 @@ int fh_adamw_amp(float* p, const float* g, float* m, float* v, long n, float lr_
  * p, g, n: HOST arrays of device pointers and element counts (g[i] NULL: tensor i and its moments are left as they are).  The moments of all
  * tensors lie in one flat buffer of fh_adamw_many_blocks(n, count) blocks of 256 elements, every tensor padded to whole blocks (zeros).
  * bits = 32: m, v fp32.  bits = 8: m and sqrt(v) as e4m3 codes (bytes) over one fp32 scale per block (m_scale, v_scale; largest magnitude / 448),
- * rounded up with the probability of their fraction; the draws are a hash of (seed, place), a root that is not zero stays so, an
+ * rounded up with the probability of their fraction; the draws are a hash of (seed, place), the root is right on average (its square up to 5 % too large), a root that is not zero stays so, an
  * element that is not finite is held as NaN and stays out of the scale.  p and g may lie at any element's address (16-byte aligned ones are faster); m and v
  * at 16 bytes.  One launch per 160 tensors; the table travels in the launch's arguments. */
 long fh_adamw_many_blocks(const long* n, int count);
