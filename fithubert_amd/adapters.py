@@ -100,8 +100,8 @@ def adapter_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.T
     name one adapter; both tensors stay on the device and are not looked at on the host.
 
     K and N are multiples of 8; a rank that is no multiple of 8 is padded with zeros (copies of the factors in every call: better keep them padded), at
-    most 128.  16-bit modes round x lora_a^T * scaling (backward: dy lora_b * scaling) to the element type; where requests are short (under 16 rows on average), and in small
-    backward passes, the adapter's part of y (dx) is rounded once more before it is added.  Sums are fp32 and the gradients of the factors leave them rounded once.  ``weight``, ``bias`` and ``scaling`` take no gradient: one that requires it is refused.
+    most 128.  16-bit modes round x lora_a^T * scaling (backward: dy lora_b * scaling) to the element type; where many requests are short (under 16 rows on average in
+    a batch that is too large for the kernel of few rows) the adapter's part of y (dx) is rounded once more before it is added.  Sums are fp32 and the gradients of the factors leave them rounded once.  ``weight``, ``bias`` and ``scaling`` take no gradient: one that requires it is refused.
     The call cannot be recorded (torch.jit.trace, make_fx) and has no forward-mode derivative: both are refused."""
     if x.dim() < 2 or weight.dim() != 2 or lora_a.dim() != 3 or lora_b.dim() != 3:
         raise ValueError(f"x [..][K], weight [N][K], lora_a [n][R][K], lora_b [n][N][R]: got {tuple(x.shape)}, {tuple(weight.shape)}, {tuple(lora_a.shape)}, {tuple(lora_b.shape)}")

@@ -10,8 +10,8 @@
 //         GEMM's residual operand.
 // outer:  dA and dB in one launch: a workgroup owns 64 columns of one adapter's factor and walks that adapter's rows, whichever segments they lie in, 32
 //         at a time per wave; long walks are dealt over several workgroups whose partial sums are added in order (no atomics).
-// Rounding in 16-bit modes: h and G, which are the next products' operands.  Sums are fp32 and y (dx) is rounded once where the adapters' part is added inside the projection's product;
-// where it is added as a residual (see `project`) the part itself is rounded once more on its way.
+// Rounding in 16-bit modes: h and G, which are the next products' operands.  Sums are fp32 and y (dx) is rounded once, the adapters' part being added inside the projection's product; but
+// for many short requests (see `project`) the part is a residual operand and rounded on its way to it.
 // Measured, warm, forward and backward of 16384 x 1024 -> 4096, rank 16, 4 adapters, 32 requests, bf16: h 11 us, y 122 (1.12 PFLOP/s of the projection alone), turn 5, G 45 (134 MB, 3.0 TB/s), dx 121,
 // dA and dB 26 + 5; the call 322.  Forward of 9973 x 480 -> 1440, rank 8: 6 + 27 us, the call 28 -- 234 tiles of 256 x 256 for 256 CUs, each with eight steps of K: bound by filling and emptying
 // one tile.  32 one-row requests, 768 -> 768, fp16: 4.9 + 6.7 us.  fp32, 1497 x 480 -> 480, rank 32, both directions: 70 us of kernels (y 19, dx 21, the rest 4 to 8 each).
@@ -688,6 +688,22 @@ size_t outer_bytes(const fh_adapter_desc* d, int C) {
   return n > 1 ? al16((size_t)n * d->n_adapters * C * d->R * 4) : 0;
 }
 
+// Whether requests are short on average, and the workgroups of adapter_few_kernel (see `project`)
+bool brief(const fh_adapter_desc* d) { return (long)d->n_segments * 16 > d->M; }
+long few_blocks(long M, long N) { return (M + 63) / 64 * ((N + 15) / 16); }
+constexpr long FEW_BRIEF = 2048;
+// Whether a 16-bit product of M x N with the reduction K takes the 256 x 256 8-phase loop: with W by its rows where its tiles give work to a good part of the CUs; with W by its columns, where the
+// loop for small products needs W turned first, from 36 tiles on.  Both directions, rank 8 to 64, us with W turned | with the large loop: 18 tiles (600 rows, 2304 -> 1536) 93 | 128, 24 (3000, 1440 ->
+// 480) 93 | 108, 32 (2000, 1024 -> 1024) 77 | 85, 36 (1400, 2304 -> 1536) 169 | 162, 48 (3000, 1024 -> 1024) 98 | 97, 72 (3000, 2304 -> 1536) 236 | 194.
+bool large(long M, long N, long K, bool strided) {
+  const long tiles = (M + 255) / 256 * ((N + 255) / 256);
+  return K >= 128 && (tiles >= 96 || (strided && tiles >= 36 && N >= 128));
+}
+// Whether the backward pass turns W for dx: the loops for small products read it by its rows only.
+bool turns_weight(int dtype, const fh_adapter_desc* d) {
+  return dtype != 0 && (brief(d) ? few_blocks(d->M, d->K) <= FEW_BRIEF : !large(d->M, d->K, d->N, true));
+}
+
 size_t partial_bytes(const fh_adapter_desc* d) { return outer_bytes(d, d->K) + outer_bytes(d, d->N); }
 
 template <typename T> int down(const Segs& g, const void* x, const void* f, void* out, int K, int R, hipStream_t st) {
@@ -739,24 +755,22 @@ template <typename T> int outer(const fh_adapter_desc* d, const void* G, const v
 //   few rows (forward)        adapter_few_kernel, by its number of workgroups: with the whole of h's kernel, bf16 and rank 16, us against the next line's:
 //                             1 x 480 -> 1440 7.2 | 18, 256 x 4096 -> 1024 35 | 44 (256 workgroups), 512 x 480 -> 1440 12.7 | 12.4 (720), 512 x 1024 -> 4096 48 | 35
 //                             (2048), but 56 | 56 with one-row requests; fp32: 512 x 4096 -> 1024 98 | 131 (512), 1024 x 768 -> 768 36 | 33 (768)
-//   requests under 16 rows    (on average) the part on its own first (16-row tiles, many of them), then the GEMM's residual operand: a large tile would walk its requests one by one.
-//                             In 16-bit modes the part is rounded to the element type in between, off by half a step of itself, beside y's own rounding
+//   requests under 16 rows    (on average; past the line above) the part on its own first (16-row tiles, many of them), then the GEMM's residual operand: a large tile would walk its
+//                             requests one by one.  In 16-bit modes the part is rounded to the element type in between, off by half a step of itself, beside y's own rounding
 //   fp32                      adapter_gemm_f32_kernel
-//   16-bit                    inside the GEMM: the 256 x 256 8-phase loop where its tiles give work to a good part of the CUs, else the 64 x 64 one-trip loop (it takes W by
-//                             its rows: forward only; a small backward -- under 96 tiles, or N under 128 -- goes as short requests do, with their rounding of the part)
+//   16-bit                    inside the GEMM: the 256 x 256 8-phase loop where `large` says so, else the 64 x 64 one-trip loop (it takes W by its rows: a small backward pass turns W first)
 template <typename T, int YL>
 int project(int dtype, const fh_adapter_desc* d, GemmParams& p, const void* h, const void* f, hipStream_t st) {
   const Segs g = segs_of(d);
   const AdapterExtend<T> ext{g, (const T*)h, (const T*)f, p.N, d->R};
-  const bool brief = (long)d->n_segments * 16 > p.M;
-  const long few = (long)((p.M + 63) / 64) * ((p.N + 15) / 16);
-  if (YL == FH_R_CONTIG && few <= (brief ? 2048 : sizeof(T) == 4 ? 512 : 400)) {
+  const long few = few_blocks(p.M, p.N);
+  if (YL == FH_R_CONTIG && few <= (brief(d) ? FEW_BRIEF : sizeof(T) == 4 ? 512 : 400)) {
     hipLaunchKernelGGL((adapter_few_kernel<T>), dim3((p.N + 15) / 16, (p.M + 63) / 64), dim3(256), 0, st, g, (const T*)p.X.p, (const T*)p.Y.p, p.ep.bias, (const T*)h, (const T*)f,
                        (T*)p.C, p.Kseg, p.N, d->R);
     FH_CHECK_LAUNCH();
     return 0;
   }
-  if (!brief) {
+  if (!brief(d)) {
     if constexpr (sizeof(T) == 4) {
       const long tiles = (long)((p.M + 63) / 64) * ((p.N + 63) / 64);
       if (tiles <= 0x7fffffffL) {
@@ -767,7 +781,7 @@ int project(int dtype, const fh_adapter_desc* d, GemmParams& p, const void* h, c
       }
     } else {
       const long tiles = (long)((p.M + 255) / 256) * ((p.N + 255) / 256);
-      if (tiles >= 96 && tiles <= 0x7fffffffL && p.Kseg >= 128) {
+      if (large(p.M, p.N, p.Kseg, YL == FH_R_STRIDED) && tiles <= 0x7fffffffL) {
         const size_t smem = 131072;
         if (int rc = (int)hipFuncSetAttribute((const void*)adapter_gemm_kernel<T, YL>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return rc;
         hipLaunchKernelGGL((adapter_gemm_kernel<T, YL>), dim3((unsigned)tiles), dim3(512), smem, st, p, ext);
@@ -810,6 +824,7 @@ int backward_t(int dtype, const fh_adapter_desc* d, const void* x, const void* w
   float* part = (float*)(scratch + al16((size_t)d->M * d->R * sizeof(T)));
   T* at = (T*)((char*)part + partial_bytes(d));
   T* bt = at + (long)d->n_adapters * d->K * d->R;
+  T* wt = bt + (long)d->n_adapters * d->N * d->R;
   if ((dx || da) && d->M > 0) {
     const int rt = (d->R + 63) / 64;
     hipLaunchKernelGGL((adapter_turn_kernel<T>), dim3(rt * ((d->K + 63) / 64 + (d->N + 63) / 64), d->n_adapters), dim3(256), 0, st, (const T*)a, (const T*)b, at, bt, d->K,
@@ -820,10 +835,19 @@ int backward_t(int dtype, const fh_adapter_desc* d, const void* x, const void* w
   if (dx && d->M > 0) {
     GemmParams p = fh_gemm_params();
     p.X = fh_operand(dy, FH_R_CONTIG, d->N);
-    p.Y = fh_operand(w, FH_R_STRIDED, d->K);
     p.C = dx;
     p.M = d->M; p.N = d->K; p.Kseg = d->N; p.ldc = d->K;
-    if (int rc = project<T, FH_R_STRIDED>(dtype, d, p, G, at, st)) return rc;
+    int rc;
+    if (turns_weight(dtype, d)) {
+      hipLaunchKernelGGL((adapter_turn_kernel<T>), dim3((d->N + 63) / 64 * ((d->K + 63) / 64)), dim3(256), 0, st, (const T*)w, (const T*)nullptr, wt, (T*)nullptr, d->K, 0, d->N);
+      FH_CHECK_LAUNCH();
+      p.Y = fh_operand(wt, FH_R_CONTIG, d->N);
+      rc = project<T, FH_R_CONTIG>(dtype, d, p, G, at, st);
+    } else {
+      p.Y = fh_operand(w, FH_R_STRIDED, d->K);
+      rc = project<T, FH_R_STRIDED>(dtype, d, p, G, at, st);
+    }
+    if (rc) return rc;
   }
   if (da || db) return outer<T>(d, G, x, da, h, dy, db, part, st);
   return 0;
@@ -836,7 +860,8 @@ extern "C" {
 long fh_adapter_scratch_bytes(int dtype, const fh_adapter_desc* d, int backward) {
   if (check(dtype, d)) return -1;
   if (!backward) return 0;
-  return (long)(al16((size_t)d->M * d->R * fh_esize(dtype)) + partial_bytes(d) + (size_t)d->n_adapters * d->R * ((size_t)d->K + d->N) * fh_esize(dtype));
+  return (long)(al16((size_t)d->M * d->R * fh_esize(dtype)) + partial_bytes(d) + (size_t)d->n_adapters * d->R * ((size_t)d->K + d->N) * fh_esize(dtype) +
+                (turns_weight(dtype, d) ? (size_t)d->K * d->N * fh_esize(dtype) : 0));
 }
 
 int fh_adapter_linear_forward(int dtype, const fh_adapter_desc* d, const void* x, const void* w, const float* bias, const void* a, const void* b,

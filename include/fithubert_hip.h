@@ -298,7 +298,7 @@ int fh_window_attention_backward(int dtype, const fh_window_attention_desc* d, c
  * adapter.  h [M][R] (dtype) receives scaling[a] x A_a^T, 0 on rows without an adapter: what the backward reads.
  * Backward (W and bias are frozen): dx = dy W + G A_a with G = scaling[a] dy B_a; da = sum G^T x; db = sum dy^T h -- in the element type,
  * written, 0 for an adapter without rows.  dx, da or db may be NULL.  16-bit modes round h and G to the element type -- and
- * the adapters' part of y (dx) where it is added to the projection's product in a launch of its own: short segments, small backward passes --, sums are fp32; no atomics.
+ * the adapters' part of y (dx) where it is added to the projection's product in a launch of its own: many short segments --, sums are fp32; no atomics.
  * K, N, R multiples of 8, R <= 128; every tensor contiguous and 16-byte aligned.
  * scratch: fh_adapter_scratch_bytes(dtype, d, 0 forward | 1 backward) bytes, 16-byte aligned (0: NULL will do).
  * ------------------------------------------------------------------------------------------ */
